@@ -184,7 +184,7 @@ def prepare(case, seed):
                                    factor=_ROTARY["factor"], original_len=_ROTARY["original"])
         elif kind == "attention":
             s["plan"] = dev.PrefixAttention(case["heads"], case["kv_heads"], case["dim"], s["q"].shape[0],
-                                            case["prefix"], dtype=s["q"].dtype)
+                                            dtype=s["q"].dtype)
     return s
 
 
