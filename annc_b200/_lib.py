@@ -9,10 +9,13 @@ import os
 _PKG = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_PKG, "lib", "libannc_b200.so")
 
-ANNC_F32, ANNC_I32, ANNC_I64, ANNC_BOOL, ANNC_U64 = 1, 3, 9, 10, 23
+ANNC_F32, ANNC_I32, ANNC_I64, ANNC_BOOL, ANNC_BF16, ANNC_F16, ANNC_U64 = 1, 3, 9, 10, 14, 19, 23
+ERR_INVALID_ARGUMENT = 3
 ACT_NONE, ACT_RELU, ACT_SIGMOID = 0, 1, 2
 B_PLAIN, B_KN4 = 0, 1
 MATH_AUTO, MATH_FP32, MATH_TF32, MATH_BF16 = 0, 1, 2, 3
+ROTARY_HALF, ROTARY_INTERLEAVED = 0, 1
+ROTARY_UNSCALED, ROTARY_LINEAR, ROTARY_NTK, ROTARY_YARN = 0, 1, 2, 3
 IO_A_BF16, IO_B_BF16, IO_C_BF16, IO_SOFTMAX, IO_PAIR, IO_SINGLE = 1, 2, 4, 8, 16, 32
 
 
@@ -47,6 +50,36 @@ class GemmDesc(C.Structure):
                 ("io_flags", C.c_int32), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
 
 
+class GemmI8Desc(C.Structure):
+    _fields_ = [("m", C.c_int64), ("n", C.c_int64), ("k", C.c_int64),
+                ("lda", C.c_int64), ("ldb", C.c_int64), ("ldc", C.c_int64),
+                ("a", C.c_void_p), ("b", C.c_void_p), ("scale_a", C.c_void_p), ("scale_b", C.c_void_p),
+                ("bias", C.c_void_p), ("c", C.c_void_p), ("c_dtype", C.c_int32), ("activation", C.c_int32)]
+
+
+class RotaryHeads(C.Structure):
+    _fields_ = [("in_", C.c_void_p), ("out", C.c_void_p), ("heads", C.c_int64),
+                ("in_token", C.c_int64), ("in_head", C.c_int64), ("out_token", C.c_int64), ("out_head", C.c_int64)]
+
+
+class RotaryDesc(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("head_dim", C.c_int32), ("rot_dim", C.c_int32), ("layout", C.c_int32),
+                ("positions_dtype", C.c_int32), ("transposed", C.c_int32), ("tokens", C.c_int64),
+                ("positions", C.c_void_p), ("freq", C.c_void_p), ("size", C.c_float), ("reserved", C.c_int32),
+                ("x", RotaryHeads * 2)]
+
+
+class PrefixAttentionDesc(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("heads", C.c_int32), ("kv_heads", C.c_int32), ("head_dim", C.c_int32),
+                ("tokens", C.c_int64), ("sequences", C.c_int64), ("prefix_len", C.c_int64), ("own_rows", C.c_int64),
+                ("scale", C.c_float), ("reserved", C.c_int32)] + \
+        [f for name in ("q", "k_prefix", "v_prefix", "k_own", "v_own")
+         for f in ((name, C.c_void_p), (name + "_row", C.c_int64), (name + "_head", C.c_int64))] + \
+        [("own_begin", C.c_void_p), ("own_len", C.c_void_p), ("q_begin", C.c_void_p),
+         ("out", C.c_void_p), ("out_row", C.c_int64), ("out_head", C.c_int64), ("lse", C.c_void_p),
+         ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+
+
 ALLOC_FN = C.CFUNCTYPE(C.c_void_p, C.c_void_p, C.c_int, C.c_int32, C.c_int32, C.POINTER(C.c_int64))
 
 
@@ -65,6 +98,19 @@ def _load() -> C.CDLL:
     lib.annc_select_gemm_target.restype = C.c_char_p
     lib.annc_gemm_kernel_name.restype = C.c_char_p
     lib.annc_gemm_run.argtypes = [C.POINTER(GemmDesc), C.c_void_p]
+    lib.annc_gemm_i8_run.argtypes = [C.POINTER(GemmI8Desc), C.c_void_p]
+    lib.annc_gemm_i8_kernel_name.restype = C.c_char_p
+    lib.annc_gemm_i8_kernel_name.argtypes = [C.POINTER(GemmI8Desc)]
+    lib.annc_quantize_rows_dev.argtypes = [C.c_void_p, C.c_int32, C.c_int64, C.c_int64, C.c_int64, C.c_void_p,
+                                           C.c_int64, C.c_void_p, C.c_void_p]
+    lib.annc_i8_weight_dev.argtypes = [C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_int64,
+                                       C.c_int64, C.c_void_p]
+    lib.annc_rotary_frequencies.argtypes = [C.c_int32, C.c_double, C.c_int32, C.c_double, C.c_int64, C.c_double,
+                                            C.c_double, C.POINTER(C.c_double), C.POINTER(C.c_float)]
+    lib.annc_rotary_dev.argtypes = [C.POINTER(RotaryDesc), C.c_void_p]
+    lib.annc_prefix_attention_workspace_bytes.restype = C.c_size_t
+    lib.annc_prefix_attention_workspace_bytes.argtypes = [C.c_int64, C.c_int32, C.c_int32]
+    lib.annc_prefix_attention_dev.argtypes = [C.POINTER(PrefixAttentionDesc), C.c_void_p]
     lib.annc_embed_bag_workspace_bytes.restype = C.c_size_t
     lib.annc_embed_bag_workspace_bytes.argtypes = [C.c_int, C.c_int64]
     lib.annc_kn4_offset.restype = C.c_int64

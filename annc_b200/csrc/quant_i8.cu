@@ -1,0 +1,309 @@
+// 8-bit integer layers: quantisation per row, weights quantised per output channel, and the dispatcher of the
+// product  C[m,n] = act(sum_k A[m,k] B[n,k] * scale_a[m] * scale_b[n] + bias[n]).
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <cstdint>
+
+#include "common.h"
+#include "gemm_i8.h"
+
+namespace annc {
+namespace gemm_i8 {
+
+namespace {
+
+// ---------------------------------------------------------------- quantisation
+// A row's step is scale = max(max|x| / 127, 2^-126), nearest in fp32 (the lower end keeps it a normal number, so
+// that nothing below divides by zero), and q the whole number nearest to x / scale, halves to even.  A row with an
+// infinity or a NaN has the step NaN and q = 0: its products are NaN, as they would be in floating point.
+
+// The nearest whole number exactly, also where the quotient of two fp32 numbers lies next to a half: the first
+// guess may be one off, but the remainder x - q * scale has no more bits than fp32 holds (both are multiples of
+// the smaller one's last place and the difference is below one step), so that comparing it decides.
+__device__ __forceinline__ int quantize_one(float x, float scale, float inv) {
+  float q = rintf(x * inv);
+  const float rem = __fmaf_rn(-q, scale, x), twice = 2.0f * fabsf(rem);
+  if (twice >= scale) {  // beyond half a step: to the neighbour; just half: to the even one
+    const float other = q + (rem > 0.0f ? 1.0f : -1.0f);
+    if (twice > scale || ((int)q & 1)) q = other;
+  }
+  return (int)q;
+}
+// Largest |x| as the bits of a non-negative float, which order as the floats do, infinities and NaN on top.
+__device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+struct Step {
+  float scale, inv;
+  bool finite;
+};
+__device__ __forceinline__ Step step_of(uint32_t top) {
+  Step s;
+  s.finite = top < 0x7f800000u;
+  s.scale = s.finite ? fmaxf(__fdiv_rn(__uint_as_float(top), 127.0f), 1.17549435e-38f) : __uint_as_float(0x7fc00000u);
+  s.inv = __frcp_rn(s.scale);
+  return s;
+}
+
+__device__ __forceinline__ float to_float(float x) { return x; }
+__device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
+__device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
+
+struct QuantParams {
+  const void* x;
+  long long ld;
+  int8_t* q;
+  long long ldq;
+  float* scale;
+  long long rows;
+  int cols;
+};
+
+// TPR threads take a row (a warp or a block of 256); a thread keeps NV pieces of V values in registers between
+// the maximum and the rounding, so a row of up to TPR * NV * V values is read once; what is longer is read
+// again, from L2.  VEC: rows of whole 16-byte pieces at 16-byte addresses; else one value at a time.
+template <typename T, int TPR, bool VEC>
+__global__ void __launch_bounds__(256) quantize_rows_kernel(QuantParams p) {
+  constexpr int V = VEC ? 16 / (int)sizeof(T) : 1;
+  constexpr int NV = VEC ? 8 : 16;
+  const int t = threadIdx.x % TPR, lane = threadIdx.x & 31;
+  const long long row = (long long)blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
+  if (row >= p.rows) return;  // (whole warps, and with TPR = 256 whole blocks)
+  const T* x = static_cast<const T*>(p.x) + row * p.ld;
+  int8_t* q = p.q + row * p.ldq;
+  const int pieces = p.cols / V;
+
+  alignas(16) T keep[NV][V];
+  auto load = [&](int piece, T (&to)[V]) {
+    if (VEC) *reinterpret_cast<uint4*>(to) = __ldg(reinterpret_cast<const uint4*>(x) + piece);
+    else to[0] = x[piece];
+  };
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+    if (t + i * TPR < pieces) load(t + i * TPR, keep[i]);
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+    if (t + i * TPR < pieces) {
+#pragma unroll
+      for (int e = 0; e < V; ++e) top = max(top, abs_bits(to_float(keep[i][e])));
+    }
+  for (int c = t + NV * TPR; c < pieces; c += TPR) {
+    alignas(16) T v[V];
+    load(c, v);
+#pragma unroll
+    for (int e = 0; e < V; ++e) top = max(top, abs_bits(to_float(v[e])));
+  }
+  top = __reduce_max_sync(0xffffffffu, top);
+  if (TPR > 32) {
+    __shared__ uint32_t tops[8];
+    if (lane == 0) tops[threadIdx.x >> 5] = top;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < 8; ++w) top = max(top, tops[w]);
+  }
+  const Step s = step_of(top);
+  if (t == 0) p.scale[row] = s.scale;
+
+  auto store = [&](int piece, const T (&v)[V]) {
+    int8_t o[V < 4 ? 4 : V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) o[e] = s.finite ? (int8_t)quantize_one(to_float(v[e]), s.scale, s.inv) : (int8_t)0;
+    if (V == 1) {
+      q[piece] = o[0];
+    } else {
+      uint32_t w[V < 4 ? 1 : V / 4];
+#pragma unroll
+      for (int j = 0; j < (V < 4 ? 1 : V / 4); ++j)
+        w[j] = (uint32_t)(uint8_t)o[4 * j] | (uint32_t)(uint8_t)o[4 * j + 1] << 8 | (uint32_t)(uint8_t)o[4 * j + 2] << 16 |
+               (uint32_t)(uint8_t)o[4 * j + 3] << 24;
+      if (V == 8) *(reinterpret_cast<uint2*>(q) + piece) = make_uint2(w[0], w[V / 4 - 1]);
+      else *(reinterpret_cast<uint32_t*>(q) + piece) = w[0];
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+    if (t + i * TPR < pieces) store(t + i * TPR, keep[i]);
+  for (int c = t + NV * TPR; c < pieces; c += TPR) {
+    alignas(16) T v[V];
+    load(c, v);
+    store(c, v);
+  }
+}
+
+// fp32 [K,N] -> int8 [N,K] with a step per column: a block takes 32 columns, reads them for their maxima and
+// again (from L2) to round and turn them in shared memory.  A weight is converted once.
+__global__ void __launch_bounds__(256)
+i8_weight_kernel(const float* __restrict__ src, long long ldb, int8_t* __restrict__ dst, long long ldq,
+                 float* __restrict__ scale, int K, int N) {
+  __shared__ uint32_t tops[8][32];
+  __shared__ int8_t tile[32][132];
+  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+  const int n0 = blockIdx.x * 32, n = n0 + tx;
+  uint32_t top = 0;
+  if (n < N)
+    for (int k = ty; k < K; k += 8) top = max(top, abs_bits(src[(long long)k * ldb + n]));
+  tops[ty][tx] = top;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < 8; ++w) top = max(top, tops[w][tx]);
+  const Step s = step_of(top);
+  if (ty == 0 && n < N) scale[n] = s.scale;
+  for (int k0 = 0; k0 < K; k0 += 128) {
+    for (int r = ty; r < 128; r += 8)
+      tile[tx][r] = n < N && k0 + r < K && s.finite
+                        ? (int8_t)quantize_one(src[(long long)(k0 + r) * ldb + n], s.scale, s.inv) : (int8_t)0;
+    __syncthreads();
+    for (int c = ty; c < 32; c += 8)
+      if (n0 + c < N)
+        for (int r = tx; r < 128; r += 32)
+          if (k0 + r < K) dst[(long long)(n0 + c) * ldq + k0 + r] = tile[c][r];
+    __syncthreads();
+  }
+}
+
+// ---------------------------------------------------------------- CUDA-core product
+// Takes every pitch and address: tiles of 64 x 64, k in steps of 64 bytes, four products a __dp4a; a thread holds
+// 4 x 4 sums.  For operands whose rows are not at 16-byte addresses, which the tensor-core kernels do not take.
+constexpr int ST = 64;
+
+__global__ void __launch_bounds__(256) gemm_i8_simt_kernel(Params p) {
+  __shared__ __align__(16) int8_t sa[ST][ST + 4], sb[ST][ST + 4];  // rows of 17 words: no bank twice
+  const int m0 = blockIdx.y * ST, n0 = blockIdx.x * ST;
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  int acc[4][4] = {};
+  for (int k0 = 0; k0 < p.k; k0 += ST) {
+    for (int e = threadIdx.x; e < ST * ST; e += 256) {
+      const int r = e / ST, c = e % ST;
+      const bool in = k0 + c < p.k;
+      sa[r][c] = in && m0 + r < p.m ? p.a[(long long)(m0 + r) * p.lda + k0 + c] : (int8_t)0;
+      sb[r][c] = in && n0 + r < p.n ? p.b[(long long)(n0 + r) * p.ldb + k0 + c] : (int8_t)0;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int kk = 0; kk < ST; kk += 4) {
+      int va[4], vb[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        va[i] = *reinterpret_cast<const int*>(&sa[ty + 16 * i][kk]);
+        vb[i] = *reinterpret_cast<const int*>(&sb[tx + 16 * i][kk]);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][j] = __dp4a(va[i], vb[j], acc[i][j]);
+    }
+    __syncthreads();
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int r = m0 + ty + 16 * i;
+    if (r >= p.m) continue;
+    const float s = p.scale_a[r];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int c = n0 + tx + 16 * j;
+      if (c < p.n) store_out(p, r, c, finish(p, acc[i][j], s, p.scale_b[c], p.bias ? p.bias[c] : 0.0f));
+    }
+  }
+}
+
+int run_simt(const Params& p, cudaStream_t s) {
+  const dim3 grid((unsigned)((p.n + ST - 1) / ST), (unsigned)((p.m + ST - 1) / ST));
+  ANNC_REQUIRE(grid.y <= 65535, ANNC_ERR_UNSUPPORTED, "gemm i8: more rows than this layout of the operands allows");
+  gemm_i8_simt_kernel<<<grid, 256, 0, s>>>(p);
+  ANNC_CUDA(cudaGetLastError());
+  return ANNC_OK;
+}
+
+template <typename T>
+int launch_quantize(const QuantParams& p, cudaStream_t s) {
+  constexpr int V = 16 / (int)sizeof(T);
+  const bool vec = p.cols % V == 0 && p.ld % V == 0 && (reinterpret_cast<uintptr_t>(p.x) & 15) == 0 && p.ldq % V == 0 &&
+                   (reinterpret_cast<uintptr_t>(p.q) & (V - 1)) == 0;
+  const bool warp = p.rows >= 1024 && p.cols <= 32 * (vec ? 8 * V : 16);
+  const long long blocks = warp ? (p.rows + 7) / 8 : p.rows;
+  ANNC_REQUIRE(blocks <= 0x7fffffffLL, ANNC_ERR_UNSUPPORTED, "quantize rows: too many rows");
+  const unsigned g = (unsigned)blocks;
+  if (vec && warp) quantize_rows_kernel<T, 32, true><<<g, 256, 0, s>>>(p);
+  else if (vec) quantize_rows_kernel<T, 256, true><<<g, 256, 0, s>>>(p);
+  else if (warp) quantize_rows_kernel<T, 32, false><<<g, 256, 0, s>>>(p);
+  else quantize_rows_kernel<T, 256, false><<<g, 256, 0, s>>>(p);
+  ANNC_CUDA(cudaGetLastError());
+  return ANNC_OK;
+}
+
+int validate(const annc_gemm_i8_desc& d) {
+  ANNC_REQUIRE(d.m >= 0 && d.n >= 0 && d.k >= 0 && d.m < (1LL << 31) && d.n < (1LL << 31), ANNC_ERR_INVALID_ARGUMENT,
+               "gemm i8: bad extents");
+  // 131071 * 128 * 128 is below 2^31: no sum of so many products leaves 32 bits
+  ANNC_REQUIRE(d.k <= 131071, ANNC_ERR_UNSUPPORTED, "gemm i8: k above 131071 (the sums are kept in 32 bits)");
+  ANNC_REQUIRE(d.lda >= d.k && d.ldb >= d.k && d.ldc >= d.n, ANNC_ERR_INVALID_ARGUMENT, "gemm i8: bad leading dimension");
+  ANNC_REQUIRE(d.activation >= ANNC_ACT_NONE && d.activation <= ANNC_ACT_SIGMOID, ANNC_ERR_INVALID_ARGUMENT,
+               "gemm i8: bad activation");
+  ANNC_REQUIRE(d.c_dtype == ANNC_F32 || d.c_dtype == ANNC_BF16 || d.c_dtype == ANNC_F16, ANNC_ERR_INVALID_ARGUMENT,
+               "gemm i8: C is f32, bf16 or f16");
+  if (d.m == 0 || d.n == 0) return ANNC_OK;
+  ANNC_REQUIRE((d.k == 0 || (d.a && d.b)) && d.c && d.scale_a && d.scale_b, ANNC_ERR_INVALID_ARGUMENT, "gemm i8: null operand");
+  const uintptr_t es = d.c_dtype == ANNC_F32 ? 4 : 2;
+  ANNC_REQUIRE(((reinterpret_cast<uintptr_t>(d.scale_a) | reinterpret_cast<uintptr_t>(d.scale_b) |
+                 reinterpret_cast<uintptr_t>(d.bias)) & 3) == 0 && (reinterpret_cast<uintptr_t>(d.c) & (es - 1)) == 0,
+               ANNC_ERR_INVALID_ARGUMENT, "gemm i8: operand not aligned to its type");
+  return ANNC_OK;
+}
+
+Params params_of(const annc_gemm_i8_desc& d) {
+  return Params{d.a, d.b, d.scale_a, d.scale_b, d.bias, d.c, d.lda, d.ldb, d.ldc, (int)d.m, (int)d.n, (int)d.k,
+                d.c_dtype, d.activation};
+}
+
+}  // namespace
+}  // namespace gemm_i8
+}  // namespace annc
+
+using namespace annc;
+
+extern "C" {
+
+int annc_gemm_i8_run(const annc_gemm_i8_desc* desc, void* stream) {
+  ANNC_REQUIRE(desc, ANNC_ERR_INVALID_ARGUMENT, "gemm i8: null descriptor");
+  ANNC_TRY(gemm_i8::validate(*desc));
+  if (desc->m == 0 || desc->n == 0) return ANNC_OK;
+  return gemm_i8::run_simt(gemm_i8::params_of(*desc), static_cast<cudaStream_t>(stream));
+}
+
+const char* annc_gemm_i8_kernel_name(const annc_gemm_i8_desc* desc) {
+  if (!desc) return "";
+  return "simt_i8";
+}
+
+int annc_quantize_rows_dev(const void* x, int32_t dtype, int64_t rows, int64_t cols, int64_t ld, int8_t* q,
+                           int64_t ldq, float* scale, void* stream) {
+  ANNC_REQUIRE(dtype == ANNC_F32 || dtype == ANNC_BF16 || dtype == ANNC_F16, ANNC_ERR_INVALID_ARGUMENT,
+               "quantize rows: x is f32, bf16 or f16");
+  ANNC_REQUIRE(rows >= 0 && cols >= 0 && cols < (1LL << 30) && ld >= cols && ldq >= cols, ANNC_ERR_INVALID_ARGUMENT,
+               "quantize rows: bad extents");
+  if (rows == 0) return ANNC_OK;
+  ANNC_REQUIRE((cols == 0 || (x && q)) && scale, ANNC_ERR_INVALID_ARGUMENT, "quantize rows: null operand");
+  const uintptr_t es = dtype == ANNC_F32 ? 4 : 2;
+  ANNC_REQUIRE((reinterpret_cast<uintptr_t>(x) & (es - 1)) == 0 && (reinterpret_cast<uintptr_t>(scale) & 3) == 0,
+               ANNC_ERR_INVALID_ARGUMENT, "quantize rows: operand not aligned to its type");
+  const gemm_i8::QuantParams p{x, ld, q, ldq, scale, rows, (int)cols};
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (dtype == ANNC_F32) return gemm_i8::launch_quantize<float>(p, s);
+  if (dtype == ANNC_BF16) return gemm_i8::launch_quantize<__nv_bfloat16>(p, s);
+  return gemm_i8::launch_quantize<__half>(p, s);
+}
+
+int annc_i8_weight_dev(const float* b_kn, int64_t ldb, int8_t* b_nk, int64_t ldq, float* scale, int64_t k, int64_t n,
+                       void* stream) {
+  ANNC_REQUIRE(b_kn && b_nk && scale && k >= 1 && n >= 1 && k < (1LL << 30) && n < (1LL << 30) && ldb >= n && ldq >= k,
+               ANNC_ERR_INVALID_ARGUMENT, "i8 weight: bad arguments");
+  ANNC_REQUIRE(((reinterpret_cast<uintptr_t>(b_kn) | reinterpret_cast<uintptr_t>(scale)) & 3) == 0, ANNC_ERR_INVALID_ARGUMENT,
+               "i8 weight: operand not aligned to its type");
+  gemm_i8::i8_weight_kernel<<<(unsigned)((n + 31) / 32), 256, 0, static_cast<cudaStream_t>(stream)>>>(b_kn, ldb, b_nk, ldq,
+                                                                                                     scale, (int)k, (int)n);
+  ANNC_CUDA(cudaGetLastError());
+  return ANNC_OK;
+}
+
+}  // extern "C"

@@ -10,7 +10,9 @@ from typing import Optional, Sequence
 
 import torch
 
-from ._lib import (ACT_NONE, B_PLAIN, MATH_AUTO, BagTable, GemmDesc, check, lib)
+from ._lib import (ACT_NONE, ANNC_BF16, ANNC_F16, ANNC_F32, ANNC_I32, ANNC_I64, B_PLAIN, ERR_INVALID_ARGUMENT, MATH_AUTO,
+                   ROTARY_HALF, ROTARY_INTERLEAVED, ROTARY_LINEAR, ROTARY_NTK, ROTARY_UNSCALED, ROTARY_YARN, AnncError,
+                   BagTable, GemmDesc, GemmI8Desc, PrefixAttentionDesc, RotaryDesc, check, lib)
 
 
 def raw_stream() -> int:
@@ -325,3 +327,186 @@ class BagPrepass:
                                              C.c_int32(self.col), C.c_int64(self.batch),
                                              C.c_void_p(ws_ptr), C.c_size_t(self.ws_bytes),
                                              _stream()))
+
+
+# ---------------------------------------------------------------- sequence operators
+
+_DTYPES = {torch.float32: ANNC_F32, torch.bfloat16: ANNC_BF16, torch.float16: ANNC_F16}
+
+
+def _require(cond: bool, message: str) -> None:
+    if not cond:
+        raise AnncError(ERR_INVALID_ARGUMENT, message)
+
+
+def _operand(name: str, t: torch.Tensor, dtypes, shape) -> None:
+    """A tensor of the current device with one of the types and the shape (None: any extent), the values of its
+    last dimension adjacent."""
+    _require(t.is_cuda and t.device.index == torch.cuda.current_device(), f"{name}: not on the current CUDA device")
+    _require(t.dtype in dtypes, f"{name}: bad type {t.dtype}")
+    _require(t.dim() == len(shape) and all(w is None or w == g for w, g in zip(shape, t.shape)),
+             f"{name}: bad shape {tuple(t.shape)}")
+    _require(t.shape[-1] <= 1 or t.stride(-1) == 1, f"{name}: the values of the last dimension are not adjacent")
+
+
+def _pitch(t: torch.Tensor) -> int:
+    """Elements from row to row; a single row has any."""
+    return max(t.stride(0), t.shape[1]) if t.shape[0] <= 1 else t.stride(0)
+
+
+def i8_rows(rows: int, cols: int, device=None) -> torch.Tensor:
+    """i8[rows, cols] whose rows start on 16 bytes, as the tensor-core product wants its operands."""
+    return torch.empty((rows, max(cols + 15, 16) // 16 * 16), dtype=torch.int8, device=device or "cuda")[:, :cols]
+
+
+def quantize_rows(x: torch.Tensor, q: torch.Tensor, scale: torch.Tensor) -> None:
+    """annc_quantize_rows_dev: x f32 / bf16 / f16 [rows, cols] -> q i8[rows, cols] (i8_rows), scale f32[rows]."""
+    _operand("x", x, _DTYPES, (None, None))
+    _operand("q", q, (torch.int8,), x.shape)
+    _operand("scale", scale, (torch.float32,), (x.shape[0],))
+    rc = lib.annc_quantize_rows_dev(x.data_ptr(), _DTYPES[x.dtype], x.shape[0], x.shape[1], _pitch(x), q.data_ptr(),
+                                    _pitch(q), scale.data_ptr(), raw_stream())
+    if rc:
+        check(rc)
+
+
+def i8_weight(b_kn: torch.Tensor):
+    """f32 [K,N] -> (i8 [N,K] with rows on 16 bytes, f32 scale [N]) for gemm_i8 (annc_i8_weight_dev)."""
+    _operand("b_kn", b_kn, (torch.float32,), (None, None))
+    k, n = b_kn.shape
+    q = i8_rows(n, k, b_kn.device)
+    scale = torch.empty(n, dtype=torch.float32, device=b_kn.device)
+    check(lib.annc_i8_weight_dev(b_kn.data_ptr(), _pitch(b_kn), q.data_ptr(), q.stride(0), scale.data_ptr(), k, n,
+                                 raw_stream()))
+    return q, scale
+
+
+def gemm_i8_desc(a, scale_a, b, scale_b, c, bias=None, activation: int = ACT_NONE) -> GemmI8Desc:
+    """The checked descriptor of gemm_i8."""
+    m, n, k = a.shape[0], b.shape[0], a.shape[-1]
+    _operand("a", a, (torch.int8,), (None, None))
+    _operand("b", b, (torch.int8,), (None, k))
+    _operand("scale_a", scale_a, (torch.float32,), (m,))
+    _operand("scale_b", scale_b, (torch.float32,), (n,))
+    _operand("c", c, _DTYPES, (m, n))
+    if bias is not None:
+        _operand("bias", bias, (torch.float32,), (n,))
+    return GemmI8Desc(m, n, k, _pitch(a), _pitch(b), _pitch(c), a.data_ptr(), b.data_ptr(), scale_a.data_ptr(),
+                      scale_b.data_ptr(), None if bias is None else bias.data_ptr(), c.data_ptr(), _DTYPES[c.dtype],
+                      activation)
+
+
+def gemm_i8(a: torch.Tensor, scale_a: torch.Tensor, b: torch.Tensor, scale_b: torch.Tensor, c: torch.Tensor, *,
+            bias: Optional[torch.Tensor] = None, activation: int = ACT_NONE) -> None:
+    """annc_gemm_i8_run on the current stream: c = act(a b^T * scale_a[:, None] * scale_b + bias); a i8[m,k], b
+    i8[n,k], c f32 / bf16 / f16 [m,n]."""
+    rc = lib.annc_gemm_i8_run(C.byref(gemm_i8_desc(a, scale_a, b, scale_b, c, bias, activation)), raw_stream())
+    if rc:
+        check(rc)
+
+
+def gemm_i8_kernel_name(a, scale_a, b, scale_b, c, bias=None, activation: int = ACT_NONE) -> str:
+    """Name of the kernel family that gemm_i8 takes for these operands."""
+    return lib.annc_gemm_i8_kernel_name(C.byref(gemm_i8_desc(a, scale_a, b, scale_b, c, bias, activation))).decode()
+
+
+class Rotary:
+    """Rotary positions (annc_rotary_dev): holds the frequencies of annc_rotary_frequencies on the device.
+    layout "half" or "interleaved"; scaling "none", "linear", "ntk" or "yarn" by `factor`."""
+
+    def __init__(self, rot_dim: int, *, base: float = 10000.0, layout: str = "half", scaling: str = "none",
+                 factor: float = 1.0, original_len: int = 4096, beta_fast: float = 32.0, beta_slow: float = 1.0,
+                 device=None):
+        layouts = {"half": ROTARY_HALF, "interleaved": ROTARY_INTERLEAVED}
+        scalings = {"none": ROTARY_UNSCALED, "linear": ROTARY_LINEAR, "ntk": ROTARY_NTK, "yarn": ROTARY_YARN}
+        _require(layout in layouts, f"rotary: unknown layout {layout!r}")
+        _require(scaling in scalings, f"rotary: unknown scaling {scaling!r}")
+        self.rot_dim, self.layout = int(rot_dim), layouts[layout]
+        host = (C.c_double * max(self.rot_dim // 2, 1))()
+        size = C.c_float(0)
+        check(lib.annc_rotary_frequencies(self.rot_dim, base, scalings[scaling], factor, original_len, beta_fast,
+                                          beta_slow, host, C.byref(size)))
+        self.size = size.value
+        self.freq = torch.tensor(list(host), dtype=torch.float64, device=device or "cuda")
+
+    def run(self, positions: torch.Tensor, q: torch.Tensor, out_q: torch.Tensor, k: Optional[torch.Tensor] = None,
+            out_k: Optional[torch.Tensor] = None, *, transposed: bool = False) -> None:
+        """q [tokens, heads, head_dim] -> out_q (q itself: in place), and k likewise in the same launch; positions
+        i32 / i64 [tokens]."""
+        _operand("q", q, _DTYPES, (None, None, None))
+        tokens, _, dim = q.shape
+        _operand("out_q", out_q, (q.dtype,), q.shape)
+        _operand("positions", positions, (torch.int32, torch.int64), (tokens,))
+        _require(self.freq.device == q.device, "q: not on the device of the frequencies")
+        _require((k is None) == (out_k is None), "rotary: k and out_k go together")
+        d = RotaryDesc(_DTYPES[q.dtype], dim, self.rot_dim, self.layout,
+                       ANNC_I64 if positions.dtype == torch.int64 else ANNC_I32, int(transposed), tokens,
+                       positions.data_ptr(), self.freq.data_ptr(), self.size)
+        d.x[0] = (q.data_ptr(), out_q.data_ptr(), q.shape[1], q.stride(0), q.stride(1), out_q.stride(0), out_q.stride(1))
+        if k is not None:
+            _operand("k", k, (q.dtype,), (tokens, None, dim))
+            _operand("out_k", out_k, (q.dtype,), k.shape)
+            d.x[1] = (k.data_ptr(), out_k.data_ptr(), k.shape[1], k.stride(0), k.stride(1), out_k.stride(0),
+                      out_k.stride(1))
+        rc = lib.annc_rotary_dev(C.byref(d), raw_stream())
+        if rc:
+            check(rc)
+
+
+class PrefixAttention:
+    """Attention of up to max_tokens tokens that share one prefix (annc_prefix_attention_dev); holds the workspace.
+    One run() at a time: runs on different streams that may overlap, captured graphs among them, need a plan each."""
+
+    def __init__(self, heads: int, kv_heads: int, head_dim: int, max_tokens: int, *, dtype=torch.bfloat16, device=None):
+        _require(dtype in (torch.bfloat16, torch.float16), f"prefix attention: bad type {dtype}")
+        self.heads, self.kv_heads, self.head_dim = int(heads), int(kv_heads), int(head_dim)
+        self.max_tokens, self.dtype = int(max_tokens), dtype
+        self.ws_bytes = int(lib.annc_prefix_attention_workspace_bytes(self.max_tokens, self.heads, self.head_dim))
+        self.ws = torch.empty(self.ws_bytes, dtype=torch.uint8, device=device or "cuda")
+
+    def run(self, q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: torch.Tensor, out: torch.Tensor, *,
+            k_own: Optional[torch.Tensor] = None, v_own: Optional[torch.Tensor] = None,
+            own_begin: Optional[torch.Tensor] = None, own_len: Optional[torch.Tensor] = None,
+            q_begin: Optional[torch.Tensor] = None, scale: Optional[float] = None,
+            lse: Optional[torch.Tensor] = None) -> None:
+        """q, out [tokens, heads, head_dim]; k_prefix, v_prefix [prefix, kv_heads, head_dim]; k_own, v_own [rows,
+        kv_heads, head_dim] with own_begin i64[sequences] and own_len i32[sequences]; q_begin i32[sequences + 1],
+        without it a token is a sequence; scale head_dim ** -0.5 unless given; lse f32[tokens, heads]."""
+        heads, kv, dim = self.heads, self.kv_heads, self.head_dim
+        dt = (self.dtype,)
+        _operand("q", q, dt, (None, heads, dim))
+        tokens = q.shape[0]
+        _require(tokens <= self.max_tokens, f"q: more than the plan's {self.max_tokens} tokens")
+        _require(self.ws.device == q.device, "q: not on the plan's device")
+        _operand("out", out, dt, q.shape)
+        _operand("k_prefix", k_prefix, dt, (None, kv, dim))
+        _operand("v_prefix", v_prefix, dt, k_prefix.shape)
+        d = PrefixAttentionDesc(_DTYPES[self.dtype], heads, kv, dim, tokens, tokens, k_prefix.shape[0], 0,
+                                dim ** -0.5 if scale is None else scale, 0,
+                                q.data_ptr(), q.stride(0), q.stride(1),
+                                k_prefix.data_ptr(), k_prefix.stride(0), k_prefix.stride(1),
+                                v_prefix.data_ptr(), v_prefix.stride(0), v_prefix.stride(1))
+        if q_begin is not None:
+            _operand("q_begin", q_begin, (torch.int32,), (None,))
+            _require(q_begin.shape[0] >= 1, "q_begin: has one entry more than there are sequences")
+            d.sequences, d.q_begin = q_begin.shape[0] - 1, q_begin.data_ptr()
+        given = [x is not None for x in (k_own, v_own, own_begin, own_len)]
+        _require(all(given) or not any(given), "prefix attention: own keys need k_own, v_own, own_begin and own_len")
+        if k_own is not None:
+            _operand("k_own", k_own, dt, (None, kv, dim))
+            _operand("v_own", v_own, dt, k_own.shape)
+            _operand("own_begin", own_begin, (torch.int64,), (d.sequences,))
+            _operand("own_len", own_len, (torch.int32,), (d.sequences,))
+            d.own_rows = k_own.shape[0]
+            d.k_own, d.k_own_row, d.k_own_head = k_own.data_ptr(), k_own.stride(0), k_own.stride(1)
+            d.v_own, d.v_own_row, d.v_own_head = v_own.data_ptr(), v_own.stride(0), v_own.stride(1)
+            d.own_begin, d.own_len = own_begin.data_ptr(), own_len.data_ptr()
+        d.out, d.out_row, d.out_head = out.data_ptr(), out.stride(0), out.stride(1)
+        if lse is not None:
+            _operand("lse", lse, (torch.float32,), (tokens, heads))
+            _require(lse.is_contiguous(), "lse: not contiguous")
+            d.lse = lse.data_ptr()
+        d.workspace, d.workspace_bytes = self.ws.data_ptr(), self.ws_bytes
+        rc = lib.annc_prefix_attention_dev(C.byref(d), raw_stream())
+        if rc:
+            check(rc)

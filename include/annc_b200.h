@@ -131,7 +131,7 @@ void* annc_kernel_map_resolve(const char* kernel, const int* sizes, int num_size
 
 /* ---------------------------------------------------------------- tensors */
 
-enum { ANNC_F32 = 1, ANNC_I32 = 3, ANNC_I64 = 9, ANNC_BOOL = 10, ANNC_U64 = 23 };
+enum { ANNC_F32 = 1, ANNC_I32 = 3, ANNC_I64 = 9, ANNC_BOOL = 10, ANNC_BF16 = 14, ANNC_F16 = 19, ANNC_U64 = 23 };
 
 typedef struct annc_tensor {
   void* data;      /* host or device */
@@ -616,6 +616,126 @@ int annc_gemv_dev(int trans_a, int64_t m, int64_t n, float alpha, const float* a
 int annc_dot_interaction_dev(const float* z, int64_t batch, int features, int dim,
                              int64_t z_stride, float* out, int64_t out_stride, int math,
                              void* stream);
+
+/* ---- Sequence operators: ranking candidates against a user's history -------------------------
+ * No counterpart in the reference.  Device pointers only, nothing allocated, any stream; strides
+ * and leading dimensions in elements. */
+
+/* 8-bit integer layers.  annc_quantize_rows_dev rounds every row of x (f32, bf16 or f16) to
+ * q[r, c] = nearest whole number (halves to even) of x[r, c] / scale[r], with the step
+ * scale[r] = max(max|x[r, :]| / 127, 2^-126) rounded to f32 first.  A row that holds an infinity
+ * or a NaN has scale NaN and q = 0.  Bytes of q behind `cols` are left as they are.
+ * annc_i8_weight_dev does the same for every column of a weight f32[K,N] and stores it [N,K], once
+ * per weight.  Rows of q that start on 16 bytes (ldq and the address multiples of 16) let the
+ * product run on the tensor cores. */
+int annc_quantize_rows_dev(const void* x, int32_t dtype, int64_t rows, int64_t cols, int64_t ld,
+                           int8_t* q, int64_t ldq, float* scale, void* stream);
+int annc_i8_weight_dev(const float* b_kn, int64_t ldb, int8_t* b_nk, int64_t ldq, float* scale,
+                       int64_t k, int64_t n, void* stream);
+
+/* C[m,n] = act(sum_k A[m,k] B[n,k] * scale_a[m] * scale_b[n] + bias[n]).  The sums are exact
+ * (32-bit integers; k up to 131071); scalings, bias and activation are f32, C is rounded once. */
+typedef struct annc_gemm_i8_desc {
+  int64_t m, n, k;
+  int64_t lda, ldb, ldc;
+  const int8_t* a;               /* [m,k], a token per row           */
+  const int8_t* b;               /* [n,k], an output channel per row */
+  const float* scale_a;          /* [m] */
+  const float* scale_b;          /* [n] */
+  const float* bias;             /* [n] or NULL */
+  void* c;                       /* [m,n]; must not overlap an input */
+  int32_t c_dtype;               /* ANNC_F32, ANNC_BF16 or ANNC_F16 */
+  int32_t activation;            /* ANNC_ACT_* */
+} annc_gemm_i8_desc;
+
+int annc_gemm_i8_run(const annc_gemm_i8_desc* desc, void* stream);
+/* Name of the kernel family annc_gemm_i8_run picks for the descriptor. */
+const char* annc_gemm_i8_kernel_name(const annc_gemm_i8_desc* desc);
+
+/* Rotary positions: the first rot_dim values of every head are turned in pairs by the angle
+ * positions[token] * freq[pair] (worked out in 64 bits),
+ *   (a, b) -> size * (a cos - b sin, b cos + a sin),
+ * and the rest is copied.  Pairs are (j, j + rot_dim/2) or, interleaved, (2j, 2j + 1).
+ * transposed != 0 turns the other way (with size 1 that undoes the call; in general it takes a
+ * gradient back through it).  Queries and keys go in one call; in == out with equal strides works
+ * in place (the values behind rot_dim are then not touched), other overlaps are not allowed.
+ * annc_rotary_frequencies (host) fills freq[rot_dim / 2] and size: base^(-2j/rot_dim), for longer
+ * contexts than the model was trained on (original_len) scaled
+ *   LINEAR  freq / factor                       (original_len and the betas are not read)
+ *   NTK     base * factor^(rot_dim/(rot_dim-2)) in place of base                    (nor here)
+ *   YARN    pairs with at least beta_fast turns in original_len as they are, those with at most
+ *           beta_slow divided by factor, a linear ramp between; size = 0.1 ln(factor) + 1.
+ * The caller copies them to the device. */
+enum { ANNC_ROTARY_HALF = 0, ANNC_ROTARY_INTERLEAVED = 1 };
+enum { ANNC_ROTARY_UNSCALED = 0, ANNC_ROTARY_LINEAR = 1, ANNC_ROTARY_NTK = 2, ANNC_ROTARY_YARN = 3 };
+
+typedef struct annc_rotary_heads {
+  const void* in;                /* [tokens, heads, head_dim], the values of a head adjacent */
+  void* out;
+  int64_t heads;                 /* 0 = no such tensor */
+  int64_t in_token, in_head, out_token, out_head; /* strides */
+} annc_rotary_heads;
+
+typedef struct annc_rotary_desc {
+  int32_t dtype;                 /* ANNC_F32, ANNC_BF16 or ANNC_F16 */
+  int32_t head_dim, rot_dim;     /* rot_dim even, 2 .. 512, <= head_dim */
+  int32_t layout;                /* ANNC_ROTARY_HALF or _INTERLEAVED */
+  int32_t positions_dtype;       /* ANNC_I32 or ANNC_I64 */
+  int32_t transposed;
+  int64_t tokens;
+  const void* positions;         /* [tokens] */
+  const double* freq;            /* device, [rot_dim / 2] */
+  float size;
+  int32_t reserved;
+  annc_rotary_heads x[2];
+} annc_rotary_desc;
+
+int annc_rotary_frequencies(int32_t rot_dim, double base, int32_t scaling, double factor,
+                            int64_t original_len, double beta_fast, double beta_slow, double* freq,
+                            float* size);
+int annc_rotary_dev(const annc_rotary_desc* desc, void* stream);
+
+/* Attention of a batch whose sequences share one prefix of keys and values:
+ *   out[t, h, :] = sum_j p_j v_j,  p = softmax over the keys j that token t sees of
+ *   scale * q[t, h, :] . k_j  (key head h / (heads / kv_heads)).
+ * Every token sees the whole prefix and, of its own sequence s, rows own_begin[s] ..
+ * own_begin[s] + own_len[s] - 1 of k_own / v_own but for the last n - 1 - i, where it is token i
+ * of the sequence's n (the sequence's last token sees them all).  The tokens of sequence s are
+ * q_begin[s] .. q_begin[s+1] - 1 (ascending); without q_begin every token is a sequence.  Tokens
+ * outside all sequences are left as they are in out and lse.  A token that sees no key gets zeros
+ * and lse -inf; lse is the natural logarithm of the sum of exp(scale * q . k).  own_begin /
+ * own_len entries that reach outside 0 .. own_rows are clamped to it.
+ * The prefix is read once for all tokens.  workspace: 16-byte aligned scratch of
+ * annc_prefix_attention_workspace_bytes(tokens, heads, head_dim) bytes (for at most so many tokens),
+ * one call at a time. */
+typedef struct annc_prefix_attention_desc {
+  int32_t dtype;                 /* ANNC_BF16 or ANNC_F16: q, keys, values, out */
+  int32_t heads, kv_heads, head_dim; /* head_dim 1 .. 256 */
+  int64_t tokens, sequences, prefix_len, own_rows;
+  float scale;
+  int32_t reserved;
+  const void* q;                 /* [tokens, heads, head_dim] */
+  int64_t q_row, q_head;
+  const void* k_prefix;          /* [prefix_len, kv_heads, head_dim] */
+  int64_t k_prefix_row, k_prefix_head;
+  const void* v_prefix;
+  int64_t v_prefix_row, v_prefix_head;
+  const void* k_own;             /* [own_rows, kv_heads, head_dim] */
+  int64_t k_own_row, k_own_head;
+  const void* v_own;
+  int64_t v_own_row, v_own_head;
+  const int64_t* own_begin;      /* device [sequences] */
+  const int32_t* own_len;        /* device [sequences]; NULL = no own keys */
+  const int32_t* q_begin;        /* device [sequences + 1] or NULL */
+  void* out;                     /* [tokens, heads, head_dim] */
+  int64_t out_row, out_head;
+  float* lse;                    /* [tokens, heads] or NULL */
+  void* workspace;
+  size_t workspace_bytes;
+} annc_prefix_attention_desc;
+
+size_t annc_prefix_attention_workspace_bytes(int64_t tokens, int32_t heads, int32_t head_dim);
+int annc_prefix_attention_dev(const annc_prefix_attention_desc* desc, void* stream);
 
 /* ---------------------------------------------------------------- reference symbols
  * XLA custom-call targets (annc/service/cpu/kdnn_rewriter.h:140-155).  `in` holds the
