@@ -22,6 +22,15 @@ struct Params {
   int c_dtype, act;
 };
 
+// How a product is run: on CUDA cores, by the split kernel (tokens per tile, CTAs per tile), or by the pair kernel.
+enum RouteKind { ROUTE_SIMT = 0, ROUTE_SPLIT = 1, ROUTE_PAIR = 2 };
+struct Route {
+  RouteKind kind;
+  int tokens, split;
+};
+Route route_of(const Params& p);
+int run_tc(const Params& p, const Route& r, cudaStream_t s);
+
 #ifdef __CUDACC__
 // act(sum * scale_a * scale_b + bias).  The sum of products is exact (32-bit integers); it is rounded to fp32 once
 // (sums above 2^24), and the two scalings, the addition and C's type round once each.

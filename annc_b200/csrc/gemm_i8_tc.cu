@@ -1,0 +1,533 @@
+// 8-bit integer products on the 5th-generation tensor cores (tcgen05, kind::i8, 32-bit integer sums).
+//
+//   C[m,n] = act(sum_k A[m,k] B[n,k] * scale_a[m] * scale_b[n] + bias[n])
+//
+// Both kernels put the output channels (rows of B) on the 128 accumulator rows and the tokens (rows of A) on its
+// columns: a tile of few tokens then wastes no rows, and since tensor memory is read with a lane per accumulator
+// row, a warp's 32 values of one token are adjacent in C and are stored as they come, without a turn in shared
+// memory.  Operands come by TMA in k-steps of 128 bytes (128-byte swizzle, out-of-range bytes read as zero).
+//
+//   split kernel  one CTA takes 128 channels x 16 to 256 tokens; the CTAs of a cluster share a tile and split its k-steps,
+//                 leave their integer sums in shared memory and add them over distributed shared memory (integers:
+//                 any order gives the same).  For products whose tiles do not fill the chip, down to one token,
+//                 where the weight's bytes are all there is to do.
+//   pair kernel   persistent, a cluster of two CTAs takes 256 channels x 256 tokens (cta_group::2, each loads its own
+//                 half of both operands), accumulators double-buffered in tensor memory.
+//
+// Every wait is bounded; a role that gives up raises the error word that annc_gemm_check reads.
+#include <cuda.h>
+
+#include <cstdint>
+#include <cstring>
+
+#include "common.h"
+#include "gemm_i8.h"
+#include "pdl.cuh"
+#include "tc_host.h"
+#include "tc_ptx.cuh"
+
+namespace annc {
+namespace gemm {
+int* gemm_error_word();  // device address of the tcgen05 GEMM error word (gemm_tc.cu)
+}
+namespace gemm_i8 {
+
+namespace {
+
+using namespace annc::tc;
+
+constexpr int KB = 128;  // bytes (values) of k per stage
+
+__device__ __forceinline__ void umma_i8(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void umma_pair_i8(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void tma_prefetch_2d(const CUtensorMap* map, int x, int y) {
+  asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global [%0, {%1, %2}];" ::"l"(map), "r"(x), "r"(y) : "memory");
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
+// D s32; A and B signed 8-bit, both K-major.
+__host__ __device__ constexpr uint32_t i8_idesc(int m, int n) {
+  return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+}
+
+// ---------------------------------------------------------------- split kernel
+
+constexpr int kSplitThreads = 192;  // producer, MMA issuer, four epilogue warps
+constexpr int kChannels = 128;
+
+template <int TN>
+struct SplitShape {
+  static constexpr int kStage = (kChannels + TN) * KB;
+  static constexpr int kStages = TN <= 64 ? 8 : TN <= 128 ? 6 : 4;
+  static constexpr int kCols = TN < 32 ? 32 : TN;
+  // The sums of a tile lie where the stages were: kChannels * TN words fit there for every TN.
+  static_assert(kStages * kStage >= kChannels * TN * 4, "");
+  static constexpr size_t kSmem = 1024 + (size_t)kStages * kStage + 256;
+};
+
+template <int TN>
+__global__ void __launch_bounds__(kSplitThreads, 1)
+gemm_i8_split_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_t, Params p, int split,
+                     int* error_word) {
+  using S = SplitShape<TN>;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw);
+  const uint32_t base = (raw + 1023u) & ~1023u;
+  uint8_t* gen_base = smem_raw + (base - raw);
+  const uint32_t bars = base + S::kStages * S::kStage;
+  const uint32_t bar_full = bars, bar_empty = bars + 8 * S::kStages, bar_done = bars + 16 * S::kStages;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gen_base + S::kStages * S::kStage + 16 * S::kStages + 8);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int channel_tiles = (p.n + kChannels - 1) / kChannels, tile = blockIdx.x / split;
+  const int n0 = tile % channel_tiles * kChannels, m0 = tile / channel_tiles * TN;
+  const int rank = split > 1 ? (int)cluster_ctarank() : 0;
+  const int KT_all = (p.k + KB - 1) / KB;
+  const int kt0 = (int)((long long)KT_all * rank / split), KT = (int)((long long)KT_all * (rank + 1) / split) - kt0;
+
+  if (threadIdx.x == 0) {
+    prefetch_tensormap(&tmap_w);
+    prefetch_tensormap(&tmap_t);
+    for (int s = 0; s < S::kStages; ++s) {
+      mbar_init(bar_full + 8 * s, 1);
+      mbar_init(bar_empty + 8 * s, 1);
+    }
+    mbar_init(bar_done, 1);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    // The weight's bytes are on their way to L2 while the kernel before this one (which quantises the tokens)
+    // drains; L2 is where all its writes would be seen, so that nothing stale is read later.
+    for (int kt = 0; kt < KT && kt < S::kStages; ++kt) tma_prefetch_2d(&tmap_w, (kt0 + kt) * KB, n0);
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                 "r"((uint32_t)S::kCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  pdl_trigger();
+  pdl_wait();
+  const bool poisoned = *reinterpret_cast<volatile int*>(error_word) != 0;  // an earlier launch gave up
+  bool ok = !poisoned;
+
+  if (ok && warp == 0) {
+    if (lane == 0) {
+      for (int kt = 0; kt < KT && ok; ++kt) {
+        const int s = kt % S::kStages;
+        ok = mbar_wait(bar_empty + 8 * s, ((kt / S::kStages) & 1u) ^ 1u, abort_flag, error_word);
+        if (!ok) break;
+        const uint32_t sw = base + s * S::kStage;
+        mbar_expect_tx(bar_full + 8 * s, S::kStage);
+        tma_load_2d(sw, &tmap_w, (kt0 + kt) * KB, n0, bar_full + 8 * s);
+        tma_load_2d(sw + kChannels * KB, &tmap_t, (kt0 + kt) * KB, m0, bar_full + 8 * s);
+      }
+    }
+  } else if (ok && warp == 1) {
+    if (lane == 0) {
+      for (int kt = 0; kt < KT && ok; ++kt) {
+        const int s = kt % S::kStages;
+        ok = mbar_wait(bar_full + 8 * s, (kt / S::kStages) & 1u, abort_flag, error_word);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t sw = base + s * S::kStage, st = sw + kChannels * KB;
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk)
+          umma_i8(tmem_base, smem_desc(sw + kk * 32, 16, 1024, 2), smem_desc(st + kk * 32, 16, 1024, 2), i8_idesc(kChannels, TN),
+                  (kt | kk) != 0 ? 1u : 0u);
+        umma_commit(bar_empty + 8 * s);
+      }
+      if (ok) umma_commit(bar_done);
+    }
+  }
+
+  const int q = warp & 3;  // TMEM lanes 32 q ..
+  const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16);
+  const int tokens = min(TN, p.m - m0);
+  if (warp >= 2 && ok) ok = KT == 0 || mbar_wait(bar_done, 0, abort_flag, error_word);
+  if (warp >= 2) {
+    ok = __all_sync(0xffffffffu, ok) != 0;
+    tc_fence_after();
+  }
+  if (split == 1) {
+    if (warp >= 2 && ok) {
+      const int n = n0 + q * 32 + lane;
+      const bool in = n < p.n;
+      const float sb = in ? p.scale_b[n] : 0.0f, bias = in && p.bias ? p.bias[n] : 0.0f;
+#pragma unroll 1
+      for (int c0 = 0; c0 < tokens; c0 += 16) {
+        uint32_t r[16];
+        if (KT > 0) {
+          tmem_ld16(taddr + c0, r);
+          tmem_ld_wait();
+        }
+        const float sa_lane = lane < 16 && c0 + lane < tokens ? p.scale_a[m0 + c0 + lane] : 0.0f;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const float sa = __shfl_sync(0xffffffffu, sa_lane, j);
+          if (c0 + j < tokens && in) store_out(p, m0 + c0 + j, n, finish(p, KT > 0 ? (int)r[j] : 0, sa, sb, bias));
+        }
+      }
+    }
+  } else {
+    // Sums [token][channel] in shared memory, where the stages were: every MMA that read them is done.
+    int* part = reinterpret_cast<int*>(gen_base);
+    if (warp >= 2 && ok) {
+#pragma unroll 1
+      for (int c0 = 0; c0 < tokens; c0 += 16) {
+        uint32_t r[16];
+        if (KT > 0) {
+          tmem_ld16(taddr + c0, r);
+          tmem_ld_wait();
+        }
+#pragma unroll
+        for (int j = 0; j < 16; ++j) part[(c0 + j) * kChannels + q * 32 + lane] = KT > 0 ? (int)r[j] : 0;
+      }
+    }
+    cluster_sync_all();
+    if (warp >= 2 && ok) {
+      // rank takes tokens rank, rank + split, ...; a warp takes one token at a time, a lane four channels
+      const int n = n0 + 4 * lane;
+      float sb[4], bias[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        sb[e] = n + e < p.n ? p.scale_b[n + e] : 0.0f;
+        bias[e] = n + e < p.n && p.bias ? p.bias[n + e] : 0.0f;
+      }
+      for (int t = rank + split * (warp - 2); t < tokens; t += 4 * split) {
+        const uint32_t at = base + (uint32_t)(t * kChannels + 4 * lane) * 4u;
+        int sum[4] = {0, 0, 0, 0};
+        for (int r = 0; r < split; ++r) {
+          int v[4];
+          asm volatile("ld.shared::cluster.v4.b32 {%0, %1, %2, %3}, [%4];"
+                       : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
+                       : "r"(mapa_u32(at, (uint32_t)r))
+                       : "memory");
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sum[e] += v[e];
+        }
+        const float sa = p.scale_a[m0 + t];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (n + e < p.n) store_out(p, m0 + t, n + e, finish(p, sum[e], sa, sb[e], bias[e]));
+      }
+    }
+    cluster_sync_all();  // a peer may still read this CTA's sums
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"((uint32_t)S::kCols) : "memory");
+  }
+}
+
+// ---------------------------------------------------------------- pair kernel
+
+constexpr int kPairStage = 32768;  // 128 channels and 128 tokens x 128 bytes per CTA
+constexpr int kPairStages = 6;
+constexpr int kPairThreads = 320;  // producer, MMA issuer, eight epilogue warps
+constexpr int kPairTokens = 256;
+constexpr int kPairScales = 8 * (kPairTokens / 2) * 4;  // every epilogue warp's 128 token scales
+constexpr size_t kPairSmem = 1024 + (size_t)kPairStages * kPairStage + kPairScales + 256;
+constexpr int kBand = 8;
+
+struct PairTiles {
+  int channels, tokens;  // tiles along each
+  int count;
+};
+// Bands of eight token tiles, inside a band the channel tile advances slowest: the tiles in flight share the
+// panels of both operands through L2.
+__device__ __forceinline__ void tile_coords(const PairTiles& t, int tile, int* channel0, int* token0) {
+  const int band = tile / (kBand * t.channels), rem = tile - band * (kBand * t.channels);
+  const int rows = min(kBand, t.tokens - band * kBand);
+  const int c = rem / rows;
+  *channel0 = c * (2 * kChannels);
+  *token0 = (band * kBand + rem - c * rows) * kPairTokens;
+}
+
+__global__ void __launch_bounds__(kPairThreads, 1)
+gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_t, Params p, PairTiles tiles,
+                    int* error_word) {
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw);
+  const uint32_t base = (raw + 1023u) & ~1023u;
+  uint8_t* gen_base = smem_raw + (base - raw);
+  float* scales = reinterpret_cast<float*>(gen_base + kPairStages * kPairStage);
+  constexpr int kBars = kPairStages * kPairStage + kPairScales;
+  const uint32_t bars = base + kBars;
+  const uint32_t bar_full = bars, bar_empty = bars + 8 * kPairStages;
+  const uint32_t bar_tfull = bars + 16 * kPairStages, bar_tempty = bar_tfull + 16;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gen_base + kBars + 16 * kPairStages + 32);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  const bool leader = rank == 0;
+  const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+  const int KT = (p.k + KB - 1) / KB;
+
+  if (threadIdx.x == 0) {
+    prefetch_tensormap(&tmap_w);
+    prefetch_tensormap(&tmap_t);
+    for (int s = 0; s < kPairStages; ++s) {
+      mbar_init(bar_full + 8 * s, 1);   // the leader's expect_tx arrival; bytes come from both CTAs
+      mbar_init(bar_empty + 8 * s, 1);  // one commit
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(bar_tfull + 8 * a, 1);
+      mbar_init(bar_tempty + 8 * a, 16);  // the epilogue warps of both CTAs
+    }
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) tmem_alloc_pair(smem_u32(tmem_slot), 512);
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();  // both CTAs' barriers exist before anything signals across the pair
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  pdl_trigger();
+  pdl_wait();
+  const bool poisoned = *reinterpret_cast<volatile int*>(error_word) != 0;  // an earlier launch gave up
+
+  if (!poisoned) {
+    if (warp == 0) {
+      if (lane == 0) {
+        uint32_t kit = 0;
+        bool ok = true;
+        for (int tile = pair; tile < tiles.count && ok; tile += pairs) {
+          int n0, m0;
+          tile_coords(tiles, tile, &n0, &m0);
+          n0 += (int)rank * kChannels;
+          m0 += (int)rank * (kPairTokens / 2);
+          for (int kt = 0; kt < KT; ++kt, ++kit) {
+            const int s = kit % kPairStages;
+            ok = mbar_wait(bar_empty + 8 * s, ((kit / kPairStages) & 1u) ^ 1u, abort_flag, error_word);
+            if (!ok) break;
+            const uint32_t sw = base + s * kPairStage;
+            const uint32_t full_leader = mapa_u32(bar_full + 8 * s, 0);
+            if (leader) mbar_expect_tx(bar_full + 8 * s, 2 * kPairStage);
+            tma_load_2d_pair(sw, &tmap_w, kt * KB, n0, full_leader);
+            tma_load_2d_pair(sw + kChannels * KB, &tmap_t, kt * KB, m0, full_leader);
+          }
+        }
+      }
+    } else if (warp == 1) {
+      if (leader && lane == 0) {
+        uint32_t kit = 0, count = 0;
+        bool ok = true;
+        for (int tile = pair; tile < tiles.count && ok; tile += pairs, ++count) {
+          const uint32_t acc = count & 1u;
+          ok = mbar_wait(bar_tempty + 8 * acc, ((count >> 1) & 1u) ^ 1u, abort_flag, error_word);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t tmem_d = tmem_base + acc * (uint32_t)kPairTokens;
+          for (int kt = 0; kt < KT; ++kt, ++kit) {
+            const int s = kit % kPairStages;
+            ok = mbar_wait(bar_full + 8 * s, (kit / kPairStages) & 1u, abort_flag, error_word);
+            if (!ok) break;
+            tc_fence_after();
+            const uint32_t sw = base + s * kPairStage, st = sw + kChannels * KB;
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk)
+              umma_pair_i8(tmem_d, smem_desc(sw + kk * 32, 16, 1024, 2), smem_desc(st + kk * 32, 16, 1024, 2),
+                           i8_idesc(2 * kChannels, kPairTokens), (kt | kk) != 0 ? 1u : 0u);
+            umma_commit_pair(bar_empty + 8 * s);
+          }
+          if (ok) umma_commit_pair(bar_tfull + 8 * acc);
+        }
+      }
+    } else {
+      // warp (q, half): accumulator rows 32 q .., token columns 128 half ..
+      const int q = warp & 3, half = (warp - 2) >> 2;
+      uint32_t count = 0;
+      bool ok = true;
+      for (int tile = pair; tile < tiles.count && ok; tile += pairs, ++count) {
+        int n0, m0;
+        tile_coords(tiles, tile, &n0, &m0);
+        const uint32_t acc = count & 1u;
+        const int n = n0 + (int)rank * kChannels + q * 32 + lane;
+        const bool in = n < p.n;
+        const float sb = in ? p.scale_b[n] : 0.0f, bias = in && p.bias ? p.bias[n] : 0.0f;
+        m0 += half * (kPairTokens / 2);
+        float* const sa = scales + (warp - 2) * (kPairTokens / 2);  // (each warp its own: no warp waits for another)
+        for (int j = lane; j < kPairTokens / 2; j += 32) sa[j] = m0 + j < p.m ? p.scale_a[m0 + j] : 0.0f;
+        __syncwarp();
+        ok = __all_sync(0xffffffffu, mbar_wait(bar_tfull + 8 * acc, (count >> 1) & 1u, abort_flag, error_word)) != 0;
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16) + acc * (uint32_t)kPairTokens + half * (kPairTokens / 2);
+        const int tokens = min(kPairTokens / 2, p.m - m0);
+#pragma unroll 1
+        for (int c0 = 0; c0 < tokens; c0 += 32) {
+          uint32_t r[32];
+          tmem_ld32(taddr + c0, r);
+          tmem_ld_wait();
+          if (in) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (c0 + j < tokens) store_out(p, m0 + c0 + j, n, finish(p, (int)r[j], sa[c0 + j], sb, bias));
+          }
+          __syncwarp();
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(mapa_u32(bar_tempty + 8 * acc, 0));
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();  // the peer may read this CTA's shared memory until its last MMA is done
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem_base, 512);
+  }
+}
+
+// ---------------------------------------------------------------- host
+
+int make_map(CUtensorMap* map, const int8_t* ptr, long long rows, long long cols, long long ld, int box_rows) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return fail(ANNC_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
+  const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)ld};
+  const cuuint32_t box[2] = {KB, (cuuint32_t)box_rows};
+  const cuuint32_t estr[2] = {1, 1};
+  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<int8_t*>(ptr), dims, strides, box, estr,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(ANNC_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
+  return ANNC_OK;
+}
+
+template <int TN>
+int launch_split(const Params& p, int split, int* error_word, cudaStream_t s) {
+  static bool attr_done[kMaxDevices] = {};
+  const int dev = device_slot();
+  if (!attr_done[dev]) {
+    ANNC_CUDA(cudaFuncSetAttribute(gemm_i8_split_kernel<TN>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                   (int)SplitShape<TN>::kSmem));
+    attr_done[dev] = true;
+  }
+  CUtensorMap tw, tt;
+  ANNC_TRY(make_map(&tw, p.b, p.n, p.k, p.ldb, kChannels));
+  ANNC_TRY(make_map(&tt, p.a, p.m, p.k, p.lda, TN));
+  cudaLaunchConfig_t cfg;
+  memset(&cfg, 0, sizeof(cfg));
+  cudaLaunchAttribute attr[2];
+  attr[0] = pdl_attribute();
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)split;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.gridDim = dim3((unsigned)split * (unsigned)((p.n + kChannels - 1) / kChannels) * (unsigned)((p.m + TN - 1) / TN), 1, 1);
+  cfg.blockDim = dim3(kSplitThreads, 1, 1);
+  cfg.dynamicSmemBytes = SplitShape<TN>::kSmem;
+  cfg.stream = s;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  ANNC_CUDA(cudaLaunchKernelEx(&cfg, gemm_i8_split_kernel<TN>, tw, tt, p, split, error_word));
+  return ANNC_OK;
+}
+
+int launch_pair(const Params& p, int* error_word, cudaStream_t s) {
+  static int max_pairs_dev[kMaxDevices] = {};
+  int& max_pairs = max_pairs_dev[device_slot()];
+  cudaLaunchConfig_t cfg;
+  memset(&cfg, 0, sizeof(cfg));
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1] = pdl_attribute();
+  cfg.gridDim = dim3(2, 1, 1);
+  cfg.blockDim = dim3(kPairThreads, 1, 1);
+  cfg.dynamicSmemBytes = kPairSmem;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (max_pairs == 0) {
+    ANNC_CUDA(cudaFuncSetAttribute(gemm_i8_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kPairSmem));
+    int n = 0;
+    ANNC_CUDA(cudaOccupancyMaxActiveClusters(&n, gemm_i8_pair_kernel, &cfg));
+    if (n < 1) return fail(ANNC_ERR_CUDA, "no CTA pair fits this device");
+    max_pairs = n;
+  }
+  CUtensorMap tw, tt;
+  ANNC_TRY(make_map(&tw, p.b, p.n, p.k, p.ldb, kChannels));
+  ANNC_TRY(make_map(&tt, p.a, p.m, p.k, p.lda, kPairTokens / 2));
+  PairTiles t;
+  t.channels = (p.n + 2 * kChannels - 1) / (2 * kChannels);
+  t.tokens = (p.m + kPairTokens - 1) / kPairTokens;
+  t.count = t.channels * t.tokens;
+  cfg.gridDim.x = 2u * (unsigned)(t.count < max_pairs ? t.count : max_pairs);
+  cfg.stream = s;
+  cfg.numAttrs = 2;
+  ANNC_CUDA(cudaLaunchKernelEx(&cfg, gemm_i8_pair_kernel, tw, tt, p, t, error_word));
+  return ANNC_OK;
+}
+
+}  // namespace
+
+Route route_of(const Params& p) {
+  Route r = {ROUTE_SIMT, 0, 0};
+  // TMA wants rows on 16 bytes
+  if (p.k < 1 || ((reinterpret_cast<uintptr_t>(p.a) | reinterpret_cast<uintptr_t>(p.b)) & 15) || p.lda % 16 || p.ldb % 16) return r;
+  const long long tiles_m = (p.m + 255LL) / 256, pair_tiles = tiles_m * ((p.n + 255LL) / 256);
+  if (pair_tiles > (1LL << 30)) return r;
+  if (p.m > 128 && p.n > 128 && pair_tiles >= 37) {
+    r.kind = ROUTE_PAIR;
+    return r;
+  }
+  int tn = 16;
+  while (tn < 256 && tn < p.m) tn *= 2;
+  const long long tiles = ((p.n + 127LL) / 128) * ((p.m + tn - 1LL) / tn);
+  const int kt = (p.k + KB - 1) / KB;
+  int split = 1;
+  while (split < 8 && tiles * split * 2 <= 148 && kt >= 2 * split) split *= 2;
+  if (tiles * split > 0x7fffffffLL) return r;
+  r.kind = ROUTE_SPLIT;
+  r.tokens = tn;
+  r.split = split;
+  return r;
+}
+
+int run_tc(const Params& p, const Route& r, cudaStream_t s) {
+  int* word = gemm::gemm_error_word();
+  if (!word) return fail(ANNC_ERR_CUDA, "gemm error word is not addressable");
+  if (r.kind == ROUTE_PAIR) return launch_pair(p, word, s);
+  switch (r.tokens) {
+    case 16: return launch_split<16>(p, r.split, word, s);
+    case 32: return launch_split<32>(p, r.split, word, s);
+    case 64: return launch_split<64>(p, r.split, word, s);
+    case 128: return launch_split<128>(p, r.split, word, s);
+    default: return launch_split<256>(p, r.split, word, s);
+  }
+}
+
+}  // namespace gemm_i8
+}  // namespace annc

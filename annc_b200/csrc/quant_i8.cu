@@ -7,6 +7,7 @@
 
 #include "common.h"
 #include "gemm_i8.h"
+#include "pdl.cuh"
 
 namespace annc {
 namespace gemm_i8 {
@@ -67,6 +68,8 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(QuantParams p) {
   constexpr int NV = VEC ? 8 : 16;
   const int t = threadIdx.x % TPR, lane = threadIdx.x & 31;
   const long long row = (long long)blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
+  pdl_trigger();
+  pdl_wait();
   if (row >= p.rows) return;  // (whole warps, and with TPR = 256 whole blocks)
   const T* x = static_cast<const T*>(p.x) + row * p.ld;
   int8_t* q = p.q + row * p.ldq;
@@ -224,16 +227,14 @@ int launch_quantize(const QuantParams& p, cudaStream_t s) {
   const long long blocks = warp ? (p.rows + 7) / 8 : p.rows;
   ANNC_REQUIRE(blocks <= 0x7fffffffLL, ANNC_ERR_UNSUPPORTED, "quantize rows: too many rows");
   const unsigned g = (unsigned)blocks;
-  if (vec && warp) quantize_rows_kernel<T, 32, true><<<g, 256, 0, s>>>(p);
-  else if (vec) quantize_rows_kernel<T, 256, true><<<g, 256, 0, s>>>(p);
-  else if (warp) quantize_rows_kernel<T, 32, false><<<g, 256, 0, s>>>(p);
-  else quantize_rows_kernel<T, 256, false><<<g, 256, 0, s>>>(p);
-  ANNC_CUDA(cudaGetLastError());
+  void (*const kernel)(QuantParams) = vec ? (warp ? quantize_rows_kernel<T, 32, true> : quantize_rows_kernel<T, 256, true>)
+                                          : (warp ? quantize_rows_kernel<T, 32, false> : quantize_rows_kernel<T, 256, false>);
+  ANNC_CUDA(launch_pdl(kernel, dim3(g), dim3(256), 0, s, p));
   return ANNC_OK;
 }
 
 int validate(const annc_gemm_i8_desc& d) {
-  ANNC_REQUIRE(d.m >= 0 && d.n >= 0 && d.k >= 0 && d.m < (1LL << 31) && d.n < (1LL << 31), ANNC_ERR_INVALID_ARGUMENT,
+  ANNC_REQUIRE(d.m >= 0 && d.n >= 0 && d.k >= 0 && d.m <= (1LL << 30) && d.n <= (1LL << 30), ANNC_ERR_INVALID_ARGUMENT,
                "gemm i8: bad extents");
   // 131071 * 128 * 128 is below 2^31: no sum of so many products leaves 32 bits
   ANNC_REQUIRE(d.k <= 131071, ANNC_ERR_UNSUPPORTED, "gemm i8: k above 131071 (the sums are kept in 32 bits)");
@@ -252,7 +253,9 @@ int validate(const annc_gemm_i8_desc& d) {
 }
 
 Params params_of(const annc_gemm_i8_desc& d) {
-  return Params{d.a, d.b, d.scale_a, d.scale_b, d.bias, d.c, d.lda, d.ldb, d.ldc, (int)d.m, (int)d.n, (int)d.k,
+  // the pitch of a single row does not matter: one that the tensor-core kernels take
+  const long long whole = (d.k + 15) / 16 * 16;
+  return Params{d.a, d.b, d.scale_a, d.scale_b, d.bias, d.c, d.m == 1 ? whole : d.lda, d.n == 1 ? whole : d.ldb, d.ldc, (int)d.m, (int)d.n, (int)d.k,
                 d.c_dtype, d.activation};
 }
 
@@ -268,12 +271,19 @@ int annc_gemm_i8_run(const annc_gemm_i8_desc* desc, void* stream) {
   ANNC_REQUIRE(desc, ANNC_ERR_INVALID_ARGUMENT, "gemm i8: null descriptor");
   ANNC_TRY(gemm_i8::validate(*desc));
   if (desc->m == 0 || desc->n == 0) return ANNC_OK;
-  return gemm_i8::run_simt(gemm_i8::params_of(*desc), static_cast<cudaStream_t>(stream));
+  const gemm_i8::Params p = gemm_i8::params_of(*desc);
+  const gemm_i8::Route r = gemm_i8::route_of(p);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return r.kind == gemm_i8::ROUTE_SIMT ? gemm_i8::run_simt(p, s) : gemm_i8::run_tc(p, r, s);
 }
 
 const char* annc_gemm_i8_kernel_name(const annc_gemm_i8_desc* desc) {
   if (!desc) return "";
-  return "simt_i8";
+  switch (gemm_i8::route_of(gemm_i8::params_of(*desc)).kind) {
+    case gemm_i8::ROUTE_PAIR: return "tcgen05_pair_i8";
+    case gemm_i8::ROUTE_SPLIT: return "tcgen05_i8";
+    default: return "simt_i8";
+  }
 }
 
 int annc_quantize_rows_dev(const void* x, int32_t dtype, int64_t rows, int64_t cols, int64_t ld, int8_t* q,

@@ -27,7 +27,7 @@ def gemm_desc(**kw):
 
 
 @pytest.mark.parametrize("kw,code,text", [
-    (dict(m=-1), INVALID, "extents"), (dict(n=1 << 31), INVALID, "extents"),
+    (dict(m=-1), INVALID, "extents"), (dict(n=(1 << 30) + 1), INVALID, "extents"),
     (dict(k=131072, lda=131072, ldb=131072), UNSUPPORTED, "131071"),
     (dict(lda=31), INVALID, "leading"), (dict(ldb=31), INVALID, "leading"), (dict(ldc=15), INVALID, "leading"),
     (dict(activation=3), INVALID, "activation"), (dict(activation=-1), INVALID, "activation"),
