@@ -5,6 +5,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 
 _PKG = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_PKG, "lib", "libannc_b200.so")
@@ -80,6 +81,13 @@ class PrefixAttentionDesc(C.Structure):
          ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
 
 
+# The same layouts as bytes: the calls of device.py fill a descriptor in 0.5 us this way, a Structure takes 1.5 us.
+PACK_GEMM_I8 = struct.Struct("@6q6P2i")
+PACK_ROTARY = struct.Struct("@6iq2Pfi" + "2P5q" * 2)
+PACK_PREFIX_ATTENTION = struct.Struct("@4i4qfi" + "P2q" * 5 + "3PP2q2PN")
+for _pack, _desc in ((PACK_GEMM_I8, GemmI8Desc), (PACK_ROTARY, RotaryDesc), (PACK_PREFIX_ATTENTION, PrefixAttentionDesc)):
+    assert _pack.size == C.sizeof(_desc)
+
 ALLOC_FN = C.CFUNCTYPE(C.c_void_p, C.c_void_p, C.c_int, C.c_int32, C.c_int32, C.POINTER(C.c_int64))
 
 
@@ -98,19 +106,19 @@ def _load() -> C.CDLL:
     lib.annc_select_gemm_target.restype = C.c_char_p
     lib.annc_gemm_kernel_name.restype = C.c_char_p
     lib.annc_gemm_run.argtypes = [C.POINTER(GemmDesc), C.c_void_p]
-    lib.annc_gemm_i8_run.argtypes = [C.POINTER(GemmI8Desc), C.c_void_p]
+    lib.annc_gemm_i8_run.argtypes = [C.c_void_p, C.c_void_p]  # (a descriptor by reference, or its bytes)
     lib.annc_gemm_i8_kernel_name.restype = C.c_char_p
-    lib.annc_gemm_i8_kernel_name.argtypes = [C.POINTER(GemmI8Desc)]
+    lib.annc_gemm_i8_kernel_name.argtypes = [C.c_void_p]
     lib.annc_quantize_rows_dev.argtypes = [C.c_void_p, C.c_int32, C.c_int64, C.c_int64, C.c_int64, C.c_void_p,
                                            C.c_int64, C.c_void_p, C.c_void_p]
     lib.annc_i8_weight_dev.argtypes = [C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_int64,
                                        C.c_int64, C.c_void_p]
     lib.annc_rotary_frequencies.argtypes = [C.c_int32, C.c_double, C.c_int32, C.c_double, C.c_int64, C.c_double,
                                             C.c_double, C.POINTER(C.c_double), C.POINTER(C.c_float)]
-    lib.annc_rotary_dev.argtypes = [C.POINTER(RotaryDesc), C.c_void_p]
+    lib.annc_rotary_dev.argtypes = [C.c_void_p, C.c_void_p]
     lib.annc_prefix_attention_workspace_bytes.restype = C.c_size_t
     lib.annc_prefix_attention_workspace_bytes.argtypes = [C.c_int64, C.c_int32, C.c_int32]
-    lib.annc_prefix_attention_dev.argtypes = [C.POINTER(PrefixAttentionDesc), C.c_void_p]
+    lib.annc_prefix_attention_dev.argtypes = [C.c_void_p, C.c_void_p]
     lib.annc_embed_bag_workspace_bytes.restype = C.c_size_t
     lib.annc_embed_bag_workspace_bytes.argtypes = [C.c_int, C.c_int64]
     lib.annc_kn4_offset.restype = C.c_int64

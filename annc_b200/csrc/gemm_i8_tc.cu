@@ -68,9 +68,42 @@ __host__ __device__ constexpr uint32_t i8_idesc(int m, int n) {
   return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
 
+template <int BYTES>
+struct Vector4;  // four values of so many bytes
+template <>
+struct Vector4<4> { using type = uint4; };
+template <>
+struct Vector4<2> { using type = uint2; };
+
+// N accumulator columns (tokens) of this lane's channel: finished, and stored N times one value of 32 adjacent
+// channels per warp.  `out` is the place of the first token, `count` how many tokens there are.
+template <typename T, int N>
+__device__ __forceinline__ void finish_columns(const Params& p, const uint32_t (&r)[N], const float* scale_a, float scale_b,
+                                               float bias, T* out, int count, bool in) {
+  float v[N];
+#pragma unroll
+  for (int j = 0; j < N; j += 4) {
+    const float4 sa = *reinterpret_cast<const float4*>(scale_a + j);
+    v[j] = scaled((int)r[j], sa.x, scale_b, bias);
+    v[j + 1] = scaled((int)r[j + 1], sa.y, scale_b, bias);
+    v[j + 2] = scaled((int)r[j + 2], sa.z, scale_b, bias);
+    v[j + 3] = scaled((int)r[j + 3], sa.w, scale_b, bias);
+  }
+  activate(p.act, v);
+  if (!in) return;
+  if (count >= N) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) out[j * p.ldc] = to_type<T>(v[j]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      if (j < count) out[j * p.ldc] = to_type<T>(v[j]);
+  }
+}
+
 // ---------------------------------------------------------------- split kernel
 
-constexpr int kSplitThreads = 192;  // producer, MMA issuer, four epilogue warps
+constexpr int kSplitThreads = 320;  // producer, MMA issuer, eight epilogue warps
 constexpr int kChannels = 128;
 
 template <int TN>
@@ -80,26 +113,32 @@ struct SplitShape {
   static constexpr int kCols = TN < 32 ? 32 : TN;
   // The sums of a tile lie where the stages were: kChannels * TN words fit there for every TN.
   static_assert(kStages * kStage >= kChannels * TN * 4, "");
-  static constexpr size_t kSmem = 1024 + (size_t)kStages * kStage + 256;
+  static constexpr int kScales = TN * 4;  // of the tile's tokens
+  static constexpr size_t kSmem = 1024 + (size_t)kStages * kStage + kScales + 256;
 };
 
-template <int TN>
+// A tile is `ch` channels (32, 64 or 128) x TN tokens.  With fewer than 128 channels the accumulator rows behind
+// them are products of whatever lies in shared memory there, and nobody reads them: narrow tiles bring the
+// weight of a small batch into more SMs at once without another cut through K.
+template <int TN, typename T>
 __global__ void __launch_bounds__(kSplitThreads, 1)
 gemm_i8_split_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_t, Params p, int split,
-                     int* error_word) {
+                     int ch, int* error_word) {
   using S = SplitShape<TN>;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
   const uint32_t base = (raw + 1023u) & ~1023u;
   uint8_t* gen_base = smem_raw + (base - raw);
-  const uint32_t bars = base + S::kStages * S::kStage;
+  float* const scales = reinterpret_cast<float*>(gen_base + S::kStages * S::kStage);
+  constexpr int kBars = S::kStages * S::kStage + S::kScales;
+  const uint32_t bars = base + kBars;
   const uint32_t bar_full = bars, bar_empty = bars + 8 * S::kStages, bar_done = bars + 16 * S::kStages;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gen_base + S::kStages * S::kStage + 16 * S::kStages + 8);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gen_base + kBars + 16 * S::kStages + 8);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int channel_tiles = (p.n + kChannels - 1) / kChannels, tile = blockIdx.x / split;
-  const int n0 = tile % channel_tiles * kChannels, m0 = tile / channel_tiles * TN;
+  const int channel_tiles = (p.n + ch - 1) / ch, tile = blockIdx.x / split;
+  const int n0 = tile % channel_tiles * ch, m0 = tile / channel_tiles * TN;
   const int rank = split > 1 ? (int)cluster_ctarank() : 0;
   const int KT_all = (p.k + KB - 1) / KB;
   const int kt0 = (int)((long long)KT_all * rank / split), KT = (int)((long long)KT_all * (rank + 1) / split) - kt0;
@@ -140,7 +179,7 @@ gemm_i8_split_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
         ok = mbar_wait(bar_empty + 8 * s, ((kt / S::kStages) & 1u) ^ 1u, abort_flag, error_word);
         if (!ok) break;
         const uint32_t sw = base + s * S::kStage;
-        mbar_expect_tx(bar_full + 8 * s, S::kStage);
+        mbar_expect_tx(bar_full + 8 * s, (uint32_t)((ch + TN) * KB));
         tma_load_2d(sw, &tmap_w, (kt0 + kt) * KB, n0, bar_full + 8 * s);
         tma_load_2d(sw + kChannels * KB, &tmap_t, (kt0 + kt) * KB, m0, bar_full + 8 * s);
       }
@@ -163,75 +202,89 @@ gemm_i8_split_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
     }
   }
 
-  const int q = warp & 3;  // TMEM lanes 32 q ..
-  const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16);
+  __syncwarp();
   const int tokens = min(TN, p.m - m0);
-  if (warp >= 2 && ok) ok = KT == 0 || mbar_wait(bar_done, 0, abort_flag, error_word);
-  if (warp >= 2) {
-    ok = __all_sync(0xffffffffu, ok) != 0;
+  if (warp >= 2 && ok) {  // while the MMAs run
+    for (int j = threadIdx.x - 64; j < TN; j += kSplitThreads - 64) scales[j] = j < tokens ? p.scale_a[m0 + j] : 0.0f;
+  }
+  // warp (q, half): channels 32 q .., every other piece of 16 tokens
+  const int q = warp & 3, half = (warp - 2) >> 2;
+  const bool reads = warp >= 2 && ok && q * 32 < ch;
+  bool done = false;
+  if (reads) {
+    done = __all_sync(0xffffffffu, mbar_wait(bar_done, 0, abort_flag, error_word)) != 0;
     tc_fence_after();
   }
+  const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16);
+  T* const c = static_cast<T*>(p.c);
   if (split == 1) {
-    if (warp >= 2 && ok) {
+    if (warp >= 2) asm volatile("bar.sync 1, 256;" ::: "memory");  // the scales are there
+    if (done) {
       const int n = n0 + q * 32 + lane;
       const bool in = n < p.n;
       const float sb = in ? p.scale_b[n] : 0.0f, bias = in && p.bias ? p.bias[n] : 0.0f;
 #pragma unroll 1
-      for (int c0 = 0; c0 < tokens; c0 += 16) {
+      for (int c0 = 16 * half; c0 < tokens; c0 += 32) {
         uint32_t r[16];
-        if (KT > 0) {
-          tmem_ld16(taddr + c0, r);
-          tmem_ld_wait();
-        }
-        const float sa_lane = lane < 16 && c0 + lane < tokens ? p.scale_a[m0 + c0 + lane] : 0.0f;
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          const float sa = __shfl_sync(0xffffffffu, sa_lane, j);
-          if (c0 + j < tokens && in) store_out(p, m0 + c0 + j, n, finish(p, KT > 0 ? (int)r[j] : 0, sa, sb, bias));
-        }
+        tmem_ld16(taddr + c0, r);
+        tmem_ld_wait();
+        finish_columns<T, 16>(p, r, scales + c0, sb, bias, c + (m0 + c0) * p.ldc + n, tokens - c0, in);
       }
     }
   } else {
     // Sums [token][channel] in shared memory, where the stages were: every MMA that read them is done.
     int* part = reinterpret_cast<int*>(gen_base);
-    if (warp >= 2 && ok) {
+    if (done) {
 #pragma unroll 1
-      for (int c0 = 0; c0 < tokens; c0 += 16) {
+      for (int c0 = 16 * half; c0 < tokens; c0 += 32) {
         uint32_t r[16];
-        if (KT > 0) {
-          tmem_ld16(taddr + c0, r);
-          tmem_ld_wait();
-        }
+        tmem_ld16(taddr + c0, r);
+        tmem_ld_wait();
 #pragma unroll
-        for (int j = 0; j < 16; ++j) part[(c0 + j) * kChannels + q * 32 + lane] = KT > 0 ? (int)r[j] : 0;
+        for (int j = 0; j < 16; ++j) part[(c0 + j) * kChannels + q * 32 + lane] = (int)r[j];
       }
     }
     cluster_sync_all();
-    if (warp >= 2 && ok) {
-      // rank takes tokens rank, rank + split, ...; a warp takes one token at a time, a lane four channels
-      const int n = n0 + 4 * lane;
-      float sb[4], bias[4];
+    if (ok) {
+      // A piece of work is four adjacent channels of a token; the ranks take tokens in turn.
+      const int per_token = ch / 4;
+      const int pieces = (tokens - rank + split - 1) / split * per_token;
+      for (int i = threadIdx.x; i < pieces; i += kSplitThreads) {
+        const int t = rank + i / per_token * split, n = n0 + i % per_token * 4;
+        if (n >= p.n) continue;
+        const uint32_t at = base + (uint32_t)(t * kChannels + i % per_token * 4) * 4u;
+        int sum[8][4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        sb[e] = n + e < p.n ? p.scale_b[n + e] : 0.0f;
-        bias[e] = n + e < p.n && p.bias ? p.bias[n + e] : 0.0f;
-      }
-      for (int t = rank + split * (warp - 2); t < tokens; t += 4 * split) {
-        const uint32_t at = base + (uint32_t)(t * kChannels + 4 * lane) * 4u;
-        int sum[4] = {0, 0, 0, 0};
-        for (int r = 0; r < split; ++r) {
-          int v[4];
-          asm volatile("ld.shared::cluster.v4.b32 {%0, %1, %2, %3}, [%4];"
-                       : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
-                       : "r"(mapa_u32(at, (uint32_t)r))
-                       : "memory");
-#pragma unroll
-          for (int e = 0; e < 4; ++e) sum[e] += v[e];
-        }
+        for (int r = 0; r < 8; ++r)
+          if (r < split)
+            asm volatile("ld.shared::cluster.v4.b32 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(sum[r][0]), "=r"(sum[r][1]), "=r"(sum[r][2]), "=r"(sum[r][3])
+                         : "r"(mapa_u32(at, (uint32_t)r)));
         const float sa = p.scale_a[m0 + t];
+        const int more = min(4, p.n - n);
+        float v[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (n + e < p.n) store_out(p, m0 + t, n + e, finish(p, sum[e], sa, sb[e], bias[e]));
+        for (int e = 0; e < 4; ++e) {
+#pragma unroll
+          for (int r = 1; r < 8; ++r)
+            if (r < split) sum[0][e] += sum[r][e];
+          v[e] = e < more ? scaled(sum[0][e], sa, p.scale_b[n + e], p.bias ? p.bias[n + e] : 0.0f) : 0.0f;
+        }
+        activate(p.act, v);
+        T* const out = c + (m0 + t) * p.ldc + n;
+        T o[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = to_type<T>(v[e]);
+        if (more == 4 && (reinterpret_cast<uintptr_t>(out) & (4 * sizeof(T) - 1)) == 0) {
+          using V = typename Vector4<sizeof(T)>::type;
+          V w;
+          memcpy(&w, o, sizeof(w));
+          *reinterpret_cast<V*>(out) = w;
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (e < more) out[e] = o[e];
+        }
       }
     }
     cluster_sync_all();  // a peer may still read this CTA's sums
@@ -268,6 +321,7 @@ __device__ __forceinline__ void tile_coords(const PairTiles& t, int tile, int* c
   *token0 = (band * kBand + rem - c * rows) * kPairTokens;
 }
 
+template <typename T>
 __global__ void __launch_bounds__(kPairThreads, 1)
 gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_t, Params p, PairTiles tiles,
                     int* error_word) {
@@ -386,11 +440,7 @@ gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
           uint32_t r[32];
           tmem_ld32(taddr + c0, r);
           tmem_ld_wait();
-          if (in) {
-#pragma unroll
-            for (int j = 0; j < 32; ++j)
-              if (c0 + j < tokens) store_out(p, m0 + c0 + j, n, finish(p, (int)r[j], sa[c0 + j], sb, bias));
-          }
+          finish_columns<T, 32>(p, r, sa + c0, sb, bias, static_cast<T*>(p.c) + (m0 + c0) * p.ldc + n, tokens - c0, in);
           __syncwarp();
         }
         tc_fence_before();
@@ -424,17 +474,18 @@ int make_map(CUtensorMap* map, const int8_t* ptr, long long rows, long long cols
   return ANNC_OK;
 }
 
-template <int TN>
-int launch_split(const Params& p, int split, int* error_word, cudaStream_t s) {
+template <int TN, typename T>
+int launch_split(const Params& p, int split, int ch, int* error_word, cudaStream_t s) {
+  void (*const kernel)(CUtensorMap, CUtensorMap, Params, int, int, int*) = gemm_i8_split_kernel<TN, T>;
   static bool attr_done[kMaxDevices] = {};
   const int dev = device_slot();
   if (!attr_done[dev]) {
-    ANNC_CUDA(cudaFuncSetAttribute(gemm_i8_split_kernel<TN>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    ANNC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                    (int)SplitShape<TN>::kSmem));
     attr_done[dev] = true;
   }
   CUtensorMap tw, tt;
-  ANNC_TRY(make_map(&tw, p.b, p.n, p.k, p.ldb, kChannels));
+  ANNC_TRY(make_map(&tw, p.b, p.n, p.k, p.ldb, ch));
   ANNC_TRY(make_map(&tt, p.a, p.m, p.k, p.lda, TN));
   cudaLaunchConfig_t cfg;
   memset(&cfg, 0, sizeof(cfg));
@@ -444,17 +495,19 @@ int launch_split(const Params& p, int split, int* error_word, cudaStream_t s) {
   attr[1].val.clusterDim.x = (unsigned)split;
   attr[1].val.clusterDim.y = 1;
   attr[1].val.clusterDim.z = 1;
-  cfg.gridDim = dim3((unsigned)split * (unsigned)((p.n + kChannels - 1) / kChannels) * (unsigned)((p.m + TN - 1) / TN), 1, 1);
+  cfg.gridDim = dim3((unsigned)split * (unsigned)((p.n + ch - 1) / ch) * (unsigned)((p.m + TN - 1) / TN), 1, 1);
   cfg.blockDim = dim3(kSplitThreads, 1, 1);
   cfg.dynamicSmemBytes = SplitShape<TN>::kSmem;
   cfg.stream = s;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  ANNC_CUDA(cudaLaunchKernelEx(&cfg, gemm_i8_split_kernel<TN>, tw, tt, p, split, error_word));
+  ANNC_CUDA(cudaLaunchKernelEx(&cfg, kernel, tw, tt, p, split, ch, error_word));
   return ANNC_OK;
 }
 
+template <typename T>
 int launch_pair(const Params& p, int* error_word, cudaStream_t s) {
+  void (*const kernel)(CUtensorMap, CUtensorMap, Params, PairTiles, int*) = gemm_i8_pair_kernel<T>;
   static int max_pairs_dev[kMaxDevices] = {};
   int& max_pairs = max_pairs_dev[device_slot()];
   cudaLaunchConfig_t cfg;
@@ -471,9 +524,9 @@ int launch_pair(const Params& p, int* error_word, cudaStream_t s) {
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   if (max_pairs == 0) {
-    ANNC_CUDA(cudaFuncSetAttribute(gemm_i8_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kPairSmem));
+    ANNC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kPairSmem));
     int n = 0;
-    ANNC_CUDA(cudaOccupancyMaxActiveClusters(&n, gemm_i8_pair_kernel, &cfg));
+    ANNC_CUDA(cudaOccupancyMaxActiveClusters(&n, kernel, &cfg));
     if (n < 1) return fail(ANNC_ERR_CUDA, "no CTA pair fits this device");
     max_pairs = n;
   }
@@ -487,14 +540,14 @@ int launch_pair(const Params& p, int* error_word, cudaStream_t s) {
   cfg.gridDim.x = 2u * (unsigned)(t.count < max_pairs ? t.count : max_pairs);
   cfg.stream = s;
   cfg.numAttrs = 2;
-  ANNC_CUDA(cudaLaunchKernelEx(&cfg, gemm_i8_pair_kernel, tw, tt, p, t, error_word));
+  ANNC_CUDA(cudaLaunchKernelEx(&cfg, kernel, tw, tt, p, t, error_word));
   return ANNC_OK;
 }
 
 }  // namespace
 
 Route route_of(const Params& p) {
-  Route r = {ROUTE_SIMT, 0, 0};
+  Route r = {ROUTE_SIMT, 0, 0, 0};
   // TMA wants rows on 16 bytes
   if (p.k < 1 || ((reinterpret_cast<uintptr_t>(p.a) | reinterpret_cast<uintptr_t>(p.b)) & 15) || p.lda % 16 || p.ldb % 16) return r;
   const long long tiles_m = (p.m + 255LL) / 256, pair_tiles = tiles_m * ((p.n + 255LL) / 256);
@@ -513,20 +566,30 @@ Route route_of(const Params& p) {
   r.kind = ROUTE_SPLIT;
   r.tokens = tn;
   r.split = split;
+  r.channels = 128;
   return r;
 }
 
-int run_tc(const Params& p, const Route& r, cudaStream_t s) {
+namespace {
+template <typename T>
+int run_as(const Params& p, const Route& r, cudaStream_t s) {
   int* word = gemm::gemm_error_word();
   if (!word) return fail(ANNC_ERR_CUDA, "gemm error word is not addressable");
-  if (r.kind == ROUTE_PAIR) return launch_pair(p, word, s);
+  if (r.kind == ROUTE_PAIR) return launch_pair<T>(p, word, s);
   switch (r.tokens) {
-    case 16: return launch_split<16>(p, r.split, word, s);
-    case 32: return launch_split<32>(p, r.split, word, s);
-    case 64: return launch_split<64>(p, r.split, word, s);
-    case 128: return launch_split<128>(p, r.split, word, s);
-    default: return launch_split<256>(p, r.split, word, s);
+    case 16: return launch_split<16, T>(p, r.split, r.channels, word, s);
+    case 32: return launch_split<32, T>(p, r.split, r.channels, word, s);
+    case 64: return launch_split<64, T>(p, r.split, r.channels, word, s);
+    case 128: return launch_split<128, T>(p, r.split, r.channels, word, s);
+    default: return launch_split<256, T>(p, r.split, r.channels, word, s);
   }
+}
+}  // namespace
+
+int run_tc(const Params& p, const Route& r, cudaStream_t s) {
+  if (p.c_dtype == ANNC_F32) return run_as<float>(p, r, s);
+  if (p.c_dtype == ANNC_BF16) return run_as<__nv_bfloat16>(p, r, s);
+  return run_as<__half>(p, r, s);
 }
 
 }  // namespace gemm_i8

@@ -169,6 +169,7 @@ i8_weight_kernel(const float* __restrict__ src, long long ldb, int8_t* __restric
 // 4 x 4 sums.  For operands whose rows are not at 16-byte addresses, which the tensor-core kernels do not take.
 constexpr int ST = 64;
 
+template <typename T>
 __global__ void __launch_bounds__(256) gemm_i8_simt_kernel(Params p) {
   __shared__ __align__(16) int8_t sa[ST][ST + 4], sb[ST][ST + 4];  // rows of 17 words: no bank twice
   const int m0 = blockIdx.y * ST, n0 = blockIdx.x * ST;
@@ -202,18 +203,25 @@ __global__ void __launch_bounds__(256) gemm_i8_simt_kernel(Params p) {
     const int r = m0 + ty + 16 * i;
     if (r >= p.m) continue;
     const float s = p.scale_a[r];
+    float v[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int c = n0 + tx + 16 * j;
-      if (c < p.n) store_out(p, r, c, finish(p, acc[i][j], s, p.scale_b[c], p.bias ? p.bias[c] : 0.0f));
+      v[j] = c < p.n ? scaled(acc[i][j], s, p.scale_b[c], p.bias ? p.bias[c] : 0.0f) : 0.0f;
     }
+    activate(p.act, v);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (n0 + tx + 16 * j < p.n) static_cast<T*>(p.c)[r * p.ldc + n0 + tx + 16 * j] = to_type<T>(v[j]);
   }
 }
 
 int run_simt(const Params& p, cudaStream_t s) {
   const dim3 grid((unsigned)((p.n + ST - 1) / ST), (unsigned)((p.m + ST - 1) / ST));
   ANNC_REQUIRE(grid.y <= 65535, ANNC_ERR_UNSUPPORTED, "gemm i8: more rows than this layout of the operands allows");
-  gemm_i8_simt_kernel<<<grid, 256, 0, s>>>(p);
+  if (p.c_dtype == ANNC_F32) gemm_i8_simt_kernel<float><<<grid, 256, 0, s>>>(p);
+  else if (p.c_dtype == ANNC_BF16) gemm_i8_simt_kernel<__nv_bfloat16><<<grid, 256, 0, s>>>(p);
+  else gemm_i8_simt_kernel<__half><<<grid, 256, 0, s>>>(p);
   ANNC_CUDA(cudaGetLastError());
   return ANNC_OK;
 }

@@ -12,7 +12,7 @@ import torch
 
 from ._lib import (ACT_NONE, ANNC_BF16, ANNC_F16, ANNC_F32, ANNC_I32, ANNC_I64, B_PLAIN, ERR_INVALID_ARGUMENT, MATH_AUTO,
                    ROTARY_HALF, ROTARY_INTERLEAVED, ROTARY_LINEAR, ROTARY_NTK, ROTARY_UNSCALED, ROTARY_YARN, AnncError,
-                   BagTable, GemmDesc, GemmI8Desc, PrefixAttentionDesc, RotaryDesc, check, lib)
+                   BagTable, GemmDesc, PACK_GEMM_I8, PACK_PREFIX_ATTENTION, PACK_ROTARY, check, lib)
 
 
 def raw_stream() -> int:
@@ -334,24 +334,53 @@ class BagPrepass:
 _DTYPES = {torch.float32: ANNC_F32, torch.bfloat16: ANNC_BF16, torch.float16: ANNC_F16}
 
 
-def _require(cond: bool, message: str) -> None:
-    if not cond:
-        raise AnncError(ERR_INVALID_ARGUMENT, message)
+def _refuse(message: str) -> None:
+    raise AnncError(ERR_INVALID_ARGUMENT, message)
 
 
-def _operand(name: str, t: torch.Tensor, dtypes, shape) -> None:
-    """A tensor of the current device with one of the types and the shape (None: any extent), the values of its
-    last dimension adjacent."""
-    _require(t.is_cuda and t.device.index == torch.cuda.current_device(), f"{name}: not on the current CUDA device")
-    _require(t.dtype in dtypes, f"{name}: bad type {t.dtype}")
-    _require(t.dim() == len(shape) and all(w is None or w == g for w, g in zip(shape, t.shape)),
-             f"{name}: bad shape {tuple(t.shape)}")
-    _require(t.shape[-1] <= 1 or t.stride(-1) == 1, f"{name}: the values of the last dimension are not adjacent")
+def _current(name: str, t: torch.Tensor) -> int:
+    """The current device, which is the tensor's."""
+    dev = t.get_device()
+    if dev < 0 or dev != torch._C._cuda_getDevice():
+        _refuse(f"{name}: not on the current CUDA device")
+    return dev
 
 
-def _pitch(t: torch.Tensor) -> int:
+# The checks of an operand (some 0.7 us each: they are a good part of what a small call costs).  All operands are on
+# the current device `dev`.
+
+def _dense(name: str, t: torch.Tensor, dev: int, dtypes, dims: int):
+    """(shape, strides) of a tensor of so many dimensions, the values of the last one adjacent."""
+    if t.get_device() != dev:
+        _refuse(f"{name}: not on the current CUDA device")
+    if t.dtype not in dtypes:
+        _refuse(f"{name}: bad type {t.dtype}")
+    shape, strides = t.shape, t.stride()
+    if len(shape) != dims:
+        _refuse(f"{name}: bad shape {tuple(shape)}")
+    if strides[-1] != 1 and shape[-1] > 1:
+        _refuse(f"{name}: the values of the last dimension are not adjacent")
+    return shape, strides
+
+
+def _vector(name: str, t: torch.Tensor, dev: int, dtype, length: int) -> int:
+    """Address of a vector of that length."""
+    if t.get_device() != dev or t.dtype is not dtype or t.shape != (length,) or not t.is_contiguous():
+        _refuse(f"{name}: has to be a vector of {length} {dtype} on the current CUDA device")
+    return t.data_ptr()
+
+
+def _alike(name: str, shape, want) -> None:
+    if shape != want:
+        _refuse(f"{name}: bad shape {tuple(shape)}, wanted {tuple(want)}")
+
+
+def _pitch(shape, strides) -> int:
     """Elements from row to row; a single row has any."""
-    return max(t.stride(0), t.shape[1]) if t.shape[0] <= 1 else t.stride(0)
+    return strides[0] if shape[0] > 1 else max(strides[0], shape[1])
+
+
+_I8, _FLOATS = (torch.int8,), tuple(_DTYPES)
 
 
 def i8_rows(rows: int, cols: int, device=None) -> torch.Tensor:
@@ -361,53 +390,57 @@ def i8_rows(rows: int, cols: int, device=None) -> torch.Tensor:
 
 def quantize_rows(x: torch.Tensor, q: torch.Tensor, scale: torch.Tensor) -> None:
     """annc_quantize_rows_dev: x f32 / bf16 / f16 [rows, cols] -> q i8[rows, cols] (i8_rows), scale f32[rows]."""
-    _operand("x", x, _DTYPES, (None, None))
-    _operand("q", q, (torch.int8,), x.shape)
-    _operand("scale", scale, (torch.float32,), (x.shape[0],))
-    rc = lib.annc_quantize_rows_dev(x.data_ptr(), _DTYPES[x.dtype], x.shape[0], x.shape[1], _pitch(x), q.data_ptr(),
-                                    _pitch(q), scale.data_ptr(), raw_stream())
+    dev = _current("x", x)
+    shape, strides = _dense("x", x, dev, _FLOATS, 2)
+    q_shape, q_strides = _dense("q", q, dev, _I8, 2)
+    _alike("q", q_shape, shape)
+    rc = lib.annc_quantize_rows_dev(x.data_ptr(), _DTYPES[x.dtype], shape[0], shape[1], _pitch(shape, strides), q.data_ptr(),
+                                    _pitch(q_shape, q_strides), _vector("scale", scale, dev, torch.float32, shape[0]),
+                                    torch._C._cuda_getCurrentRawStream(dev))
     if rc:
         check(rc)
 
 
 def i8_weight(b_kn: torch.Tensor):
     """f32 [K,N] -> (i8 [N,K] with rows on 16 bytes, f32 scale [N]) for gemm_i8 (annc_i8_weight_dev)."""
-    _operand("b_kn", b_kn, (torch.float32,), (None, None))
-    k, n = b_kn.shape
+    shape, strides = _dense("b_kn", b_kn, _current("b_kn", b_kn), (torch.float32,), 2)
+    k, n = shape
     q = i8_rows(n, k, b_kn.device)
     scale = torch.empty(n, dtype=torch.float32, device=b_kn.device)
-    check(lib.annc_i8_weight_dev(b_kn.data_ptr(), _pitch(b_kn), q.data_ptr(), q.stride(0), scale.data_ptr(), k, n,
+    check(lib.annc_i8_weight_dev(b_kn.data_ptr(), _pitch(shape, strides), q.data_ptr(), q.stride(0), scale.data_ptr(), k, n,
                                  raw_stream()))
     return q, scale
 
 
-def gemm_i8_desc(a, scale_a, b, scale_b, c, bias=None, activation: int = ACT_NONE) -> GemmI8Desc:
-    """The checked descriptor of gemm_i8."""
-    m, n, k = a.shape[0], b.shape[0], a.shape[-1]
-    _operand("a", a, (torch.int8,), (None, None))
-    _operand("b", b, (torch.int8,), (None, k))
-    _operand("scale_a", scale_a, (torch.float32,), (m,))
-    _operand("scale_b", scale_b, (torch.float32,), (n,))
-    _operand("c", c, _DTYPES, (m, n))
-    if bias is not None:
-        _operand("bias", bias, (torch.float32,), (n,))
-    return GemmI8Desc(m, n, k, _pitch(a), _pitch(b), _pitch(c), a.data_ptr(), b.data_ptr(), scale_a.data_ptr(),
-                      scale_b.data_ptr(), None if bias is None else bias.data_ptr(), c.data_ptr(), _DTYPES[c.dtype],
-                      activation)
+def _gemm_i8_desc(dev, a, scale_a, b, scale_b, c, bias, activation) -> bytes:
+    a_shape, a_strides = _dense("a", a, dev, _I8, 2)
+    b_shape, b_strides = _dense("b", b, dev, _I8, 2)
+    c_shape, c_strides = _dense("c", c, dev, _FLOATS, 2)
+    m, k = a_shape
+    n = b_shape[0]
+    if b_shape[1] != k or c_shape != (m, n):
+        _refuse(f"gemm_i8: a {tuple(a_shape)}, b {tuple(b_shape)} and c {tuple(c_shape)} do not belong together")
+    return PACK_GEMM_I8.pack(m, n, k, _pitch(a_shape, a_strides), _pitch(b_shape, b_strides), _pitch(c_shape, c_strides),
+                             a.data_ptr(), b.data_ptr(), _vector("scale_a", scale_a, dev, torch.float32, m),
+                             _vector("scale_b", scale_b, dev, torch.float32, n),
+                             0 if bias is None else _vector("bias", bias, dev, torch.float32, n), c.data_ptr(),
+                             _DTYPES[c.dtype], activation)
 
 
 def gemm_i8(a: torch.Tensor, scale_a: torch.Tensor, b: torch.Tensor, scale_b: torch.Tensor, c: torch.Tensor, *,
             bias: Optional[torch.Tensor] = None, activation: int = ACT_NONE) -> None:
     """annc_gemm_i8_run on the current stream: c = act(a b^T * scale_a[:, None] * scale_b + bias); a i8[m,k], b
     i8[n,k], c f32 / bf16 / f16 [m,n]."""
-    rc = lib.annc_gemm_i8_run(C.byref(gemm_i8_desc(a, scale_a, b, scale_b, c, bias, activation)), raw_stream())
+    dev = _current("a", a)
+    rc = lib.annc_gemm_i8_run(_gemm_i8_desc(dev, a, scale_a, b, scale_b, c, bias, activation),
+                              torch._C._cuda_getCurrentRawStream(dev))
     if rc:
         check(rc)
 
 
 def gemm_i8_kernel_name(a, scale_a, b, scale_b, c, bias=None, activation: int = ACT_NONE) -> str:
     """Name of the kernel family that gemm_i8 takes for these operands."""
-    return lib.annc_gemm_i8_kernel_name(C.byref(gemm_i8_desc(a, scale_a, b, scale_b, c, bias, activation))).decode()
+    return lib.annc_gemm_i8_kernel_name(_gemm_i8_desc(_current("a", a), a, scale_a, b, scale_b, c, bias, activation)).decode()
 
 
 class Rotary:
@@ -419,8 +452,8 @@ class Rotary:
                  device=None):
         layouts = {"half": ROTARY_HALF, "interleaved": ROTARY_INTERLEAVED}
         scalings = {"none": ROTARY_UNSCALED, "linear": ROTARY_LINEAR, "ntk": ROTARY_NTK, "yarn": ROTARY_YARN}
-        _require(layout in layouts, f"rotary: unknown layout {layout!r}")
-        _require(scaling in scalings, f"rotary: unknown scaling {scaling!r}")
+        if layout not in layouts or scaling not in scalings:
+            _refuse(f"rotary: unknown layout {layout!r} or scaling {scaling!r}")
         self.rot_dim, self.layout = int(rot_dim), layouts[layout]
         host = (C.c_double * max(self.rot_dim // 2, 1))()
         size = C.c_float(0)
@@ -433,22 +466,34 @@ class Rotary:
             out_k: Optional[torch.Tensor] = None, *, transposed: bool = False) -> None:
         """q [tokens, heads, head_dim] -> out_q (q itself: in place), and k likewise in the same launch; positions
         i32 / i64 [tokens]."""
-        _operand("q", q, _DTYPES, (None, None, None))
-        tokens, _, dim = q.shape
-        _operand("out_q", out_q, (q.dtype,), q.shape)
-        _operand("positions", positions, (torch.int32, torch.int64), (tokens,))
-        _require(self.freq.device == q.device, "q: not on the device of the frequencies")
-        _require((k is None) == (out_k is None), "rotary: k and out_k go together")
-        d = RotaryDesc(_DTYPES[q.dtype], dim, self.rot_dim, self.layout,
-                       ANNC_I64 if positions.dtype == torch.int64 else ANNC_I32, int(transposed), tokens,
-                       positions.data_ptr(), self.freq.data_ptr(), self.size)
-        d.x[0] = (q.data_ptr(), out_q.data_ptr(), q.shape[1], q.stride(0), q.stride(1), out_q.stride(0), out_q.stride(1))
+        dev = _current("q", q)
+        dtypes = (q.dtype,)
+        shape, s = _dense("q", q, dev, _FLOATS, 3)
+        out_shape, so = _dense("out_q", out_q, dev, dtypes, 3)
+        _alike("out_q", out_shape, shape)
+        tokens, heads, dim = shape
+        if self.freq.get_device() != dev:
+            _refuse("q: not on the device of the frequencies")
+        if positions.dtype is torch.int64:
+            pos, pos_type = _vector("positions", positions, dev, torch.int64, tokens), ANNC_I64
+        else:
+            pos, pos_type = _vector("positions", positions, dev, torch.int32, tokens), ANNC_I32
+        second = (0, 0, 0, 0, 0, 0, 0)
         if k is not None:
-            _operand("k", k, (q.dtype,), (tokens, None, dim))
-            _operand("out_k", out_k, (q.dtype,), k.shape)
-            d.x[1] = (k.data_ptr(), out_k.data_ptr(), k.shape[1], k.stride(0), k.stride(1), out_k.stride(0),
-                      out_k.stride(1))
-        rc = lib.annc_rotary_dev(C.byref(d), raw_stream())
+            if out_k is None:
+                _refuse("rotary: k and out_k go together")
+            k_shape, sk = _dense("k", k, dev, dtypes, 3)
+            out_shape, sko = _dense("out_k", out_k, dev, dtypes, 3)
+            _alike("k", k_shape, (tokens, k_shape[1], dim))
+            _alike("out_k", out_shape, k_shape)
+            second = (k.data_ptr(), out_k.data_ptr(), k_shape[1], sk[0], sk[1], sko[0], sko[1])
+        elif out_k is not None:
+            _refuse("rotary: k and out_k go together")
+        rc = lib.annc_rotary_dev(
+            PACK_ROTARY.pack(_DTYPES[q.dtype], dim, self.rot_dim, self.layout, pos_type, 1 if transposed else 0, tokens, pos,
+                             self.freq.data_ptr(), self.size, 0, q.data_ptr(), out_q.data_ptr(), heads, s[0], s[1], so[0],
+                             so[1], *second),
+            torch._C._cuda_getCurrentRawStream(dev))
         if rc:
             check(rc)
 
@@ -458,11 +503,12 @@ class PrefixAttention:
     One run() at a time: runs on different streams that may overlap, captured graphs among them, need a plan each."""
 
     def __init__(self, heads: int, kv_heads: int, head_dim: int, max_tokens: int, *, dtype=torch.bfloat16, device=None):
-        _require(dtype in (torch.bfloat16, torch.float16), f"prefix attention: bad type {dtype}")
+        if dtype not in (torch.bfloat16, torch.float16):
+            _refuse(f"prefix attention: bad type {dtype}")
         self.heads, self.kv_heads, self.head_dim = int(heads), int(kv_heads), int(head_dim)
         self.max_tokens, self.dtype = int(max_tokens), dtype
         self.ws_bytes = int(lib.annc_prefix_attention_workspace_bytes(self.max_tokens, self.heads, self.head_dim))
-        self.ws = torch.empty(self.ws_bytes, dtype=torch.uint8, device=device or "cuda")
+        self.ws = torch.empty(max(self.ws_bytes, 16), dtype=torch.uint8, device=device or "cuda")
 
     def run(self, q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: torch.Tensor, out: torch.Tensor, *,
             k_own: Optional[torch.Tensor] = None, v_own: Optional[torch.Tensor] = None,
@@ -472,41 +518,53 @@ class PrefixAttention:
         """q, out [tokens, heads, head_dim]; k_prefix, v_prefix [prefix, kv_heads, head_dim]; k_own, v_own [rows,
         kv_heads, head_dim] with own_begin i64[sequences] and own_len i32[sequences]; q_begin i32[sequences + 1],
         without it a token is a sequence; scale head_dim ** -0.5 unless given; lse f32[tokens, heads]."""
-        heads, kv, dim = self.heads, self.kv_heads, self.head_dim
-        dt = (self.dtype,)
-        _operand("q", q, dt, (None, heads, dim))
-        tokens = q.shape[0]
-        _require(tokens <= self.max_tokens, f"q: more than the plan's {self.max_tokens} tokens")
-        _require(self.ws.device == q.device, "q: not on the plan's device")
-        _operand("out", out, dt, q.shape)
-        _operand("k_prefix", k_prefix, dt, (None, kv, dim))
-        _operand("v_prefix", v_prefix, dt, k_prefix.shape)
-        d = PrefixAttentionDesc(_DTYPES[self.dtype], heads, kv, dim, tokens, tokens, k_prefix.shape[0], 0,
-                                dim ** -0.5 if scale is None else scale, 0,
-                                q.data_ptr(), q.stride(0), q.stride(1),
-                                k_prefix.data_ptr(), k_prefix.stride(0), k_prefix.stride(1),
-                                v_prefix.data_ptr(), v_prefix.stride(0), v_prefix.stride(1))
+        heads, kv, dim, dtypes = self.heads, self.kv_heads, self.head_dim, (self.dtype,)
+        dev = _current("q", q)
+        shape, sq = _dense("q", q, dev, dtypes, 3)
+        tokens = shape[0]
+        _alike("q", shape, (tokens, heads, dim))
+        if tokens > self.max_tokens:
+            _refuse(f"q: more than the plan's {self.max_tokens} tokens")
+        if self.ws.get_device() != dev:
+            _refuse("q: not on the plan's device")
+        out_shape, so = _dense("out", out, dev, dtypes, 3)
+        _alike("out", out_shape, shape)
+        k_shape, sk = _dense("k_prefix", k_prefix, dev, dtypes, 3)
+        v_shape, sv = _dense("v_prefix", v_prefix, dev, dtypes, 3)
+        prefix = k_shape[0]
+        _alike("k_prefix", k_shape, (prefix, kv, dim))
+        _alike("v_prefix", v_shape, k_shape)
+        sequences, q_ptr = tokens, 0
         if q_begin is not None:
-            _operand("q_begin", q_begin, (torch.int32,), (None,))
-            _require(q_begin.shape[0] >= 1, "q_begin: has one entry more than there are sequences")
-            d.sequences, d.q_begin = q_begin.shape[0] - 1, q_begin.data_ptr()
-        given = [x is not None for x in (k_own, v_own, own_begin, own_len)]
-        _require(all(given) or not any(given), "prefix attention: own keys need k_own, v_own, own_begin and own_len")
+            sequences = q_begin.shape[0] - 1 if q_begin.dim() == 1 else -1
+            if sequences < 0:
+                _refuse("q_begin: a vector with one entry more than there are sequences")
+            q_ptr = _vector("q_begin", q_begin, dev, torch.int32, sequences + 1)
+        rows, own, lists = 0, (0, 0, 0, 0, 0, 0), (0, 0)
         if k_own is not None:
-            _operand("k_own", k_own, dt, (None, kv, dim))
-            _operand("v_own", v_own, dt, k_own.shape)
-            _operand("own_begin", own_begin, (torch.int64,), (d.sequences,))
-            _operand("own_len", own_len, (torch.int32,), (d.sequences,))
-            d.own_rows = k_own.shape[0]
-            d.k_own, d.k_own_row, d.k_own_head = k_own.data_ptr(), k_own.stride(0), k_own.stride(1)
-            d.v_own, d.v_own_row, d.v_own_head = v_own.data_ptr(), v_own.stride(0), v_own.stride(1)
-            d.own_begin, d.own_len = own_begin.data_ptr(), own_len.data_ptr()
-        d.out, d.out_row, d.out_head = out.data_ptr(), out.stride(0), out.stride(1)
+            if v_own is None or own_begin is None or own_len is None:
+                _refuse("prefix attention: own keys need k_own, v_own, own_begin and own_len")
+            k_shape, sko = _dense("k_own", k_own, dev, dtypes, 3)
+            v_shape, svo = _dense("v_own", v_own, dev, dtypes, 3)
+            rows = k_shape[0]
+            _alike("k_own", k_shape, (rows, kv, dim))
+            _alike("v_own", v_shape, k_shape)
+            own = (k_own.data_ptr(), sko[0], sko[1], v_own.data_ptr(), svo[0], svo[1])
+            lists = (_vector("own_begin", own_begin, dev, torch.int64, sequences),
+                     _vector("own_len", own_len, dev, torch.int32, sequences))
+        elif v_own is not None or own_begin is not None or own_len is not None:
+            _refuse("prefix attention: own keys need k_own, v_own, own_begin and own_len")
+        lse_ptr = 0
         if lse is not None:
-            _operand("lse", lse, (torch.float32,), (tokens, heads))
-            _require(lse.is_contiguous(), "lse: not contiguous")
-            d.lse = lse.data_ptr()
-        d.workspace, d.workspace_bytes = self.ws.data_ptr(), self.ws_bytes
-        rc = lib.annc_prefix_attention_dev(C.byref(d), raw_stream())
+            _alike("lse", _dense("lse", lse, dev, (torch.float32,), 2)[0], (tokens, heads))
+            if not lse.is_contiguous():
+                _refuse("lse: not contiguous")
+            lse_ptr = lse.data_ptr()
+        rc = lib.annc_prefix_attention_dev(
+            PACK_PREFIX_ATTENTION.pack(_DTYPES[self.dtype], heads, kv, dim, tokens, sequences, prefix, rows,
+                                       dim ** -0.5 if scale is None else scale, 0, q.data_ptr(), sq[0], sq[1],
+                                       k_prefix.data_ptr(), sk[0], sk[1], v_prefix.data_ptr(), sv[0], sv[1], *own, *lists,
+                                       q_ptr, out.data_ptr(), so[0], so[1], lse_ptr, self.ws.data_ptr(), self.ws_bytes),
+            torch._C._cuda_getCurrentRawStream(dev))
         if rc:
             check(rc)
