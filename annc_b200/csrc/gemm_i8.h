@@ -22,11 +22,12 @@ struct Params {
   int c_dtype, act;
 };
 
-// How a product is run: on CUDA cores, by the split kernel (tokens and channels per tile, CTAs per tile), or by the pair kernel.
+// How a product is run: on CUDA cores, by the split kernel (tokens per tile, CTAs per tile), or
+// by the pair kernel.
 enum RouteKind { ROUTE_SIMT = 0, ROUTE_SPLIT = 1, ROUTE_PAIR = 2 };
 struct Route {
   RouteKind kind;
-  int tokens, split, channels;
+  int tokens, split;
 };
 Route route_of(const Params& p);
 int run_tc(const Params& p, const Route& r, cudaStream_t s);

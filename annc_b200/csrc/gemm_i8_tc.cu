@@ -2,17 +2,21 @@
 //
 //   C[m,n] = act(sum_k A[m,k] B[n,k] * scale_a[m] * scale_b[n] + bias[n])
 //
-// Both kernels put the output channels (rows of B) on the 128 accumulator rows and the tokens (rows of A) on its
-// columns: a tile of few tokens then wastes no rows, and since tensor memory is read with a lane per accumulator
-// row, a warp's 32 values of one token are adjacent in C and are stored as they come, without a turn in shared
-// memory.  Operands come by TMA in k-steps of 128 bytes (128-byte swizzle, out-of-range bytes read as zero).
+// Operands come by TMA in k-steps of 128 bytes (128-byte swizzle, out-of-range bytes read as zero).
 //
-//   split kernel  one CTA takes 128 channels x 16 to 256 tokens; the CTAs of a cluster share a tile and split its k-steps,
-//                 leave their integer sums in shared memory and add them over distributed shared memory (integers:
-//                 any order gives the same).  For products whose tiles do not fill the chip, down to one token,
-//                 where the weight's bytes are all there is to do.
-//   pair kernel   persistent, a cluster of two CTAs takes 256 channels x 256 tokens (cta_group::2, each loads its own
-//                 half of both operands), accumulators double-buffered in tensor memory.
+//   split kernel  one CTA takes 128 channels x 16 to 256 tokens.  The channels (rows of B) lie on the 128 accumulator
+//                 rows, so that a tile of few tokens wastes none, and since tensor memory is read with a lane per
+//                 accumulator row, a warp's 32 values of one token are adjacent in C and are stored as they come.
+//                 The CTAs of a cluster share a tile and split its k-steps, leave their integer sums in shared
+//                 memory and add them over distributed shared memory (integers: any order gives the same).  For
+//                 products whose tiles do not fill the chip, down to one token, where the weight's bytes are all
+//                 there is to do.
+//   pair kernel   persistent, a cluster of two CTAs takes 256 tokens x 256 channels (cta_group::2, each loads its own
+//                 half of both operands), accumulators double-buffered in tensor memory, so that a tile is written
+//                 under the next one's products.  Here tokens lie on the rows: a lane then holds adjacent channels, which
+//                 leave through shared memory in whole lines by TMA.  (With a store of 32 channels per token and
+//                 warp, as in the split kernel, the epilogue took 3.7 us a tile and bounded every product with k
+//                 below 1024: 16384 x 8192 x 256 103 us.)
 //
 // Every wait is bounded; a role that gives up raises the error word that annc_gemm_check reads.
 #include <cuda.h>
@@ -75,6 +79,14 @@ struct Vector4<4> { using type = uint4; };
 template <>
 struct Vector4<2> { using type = uint2; };
 
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  const T v[2] = {to_type<T>(lo), to_type<T>(hi)};
+  uint32_t w = 0;
+  memcpy(&w, v, sizeof(v) < 4 ? sizeof(v) : 4);
+  return w;
+}
+
 // N accumulator columns (tokens) of this lane's channel: finished, and stored N times one value of 32 adjacent
 // channels per warp.  `out` is the place of the first token, `count` how many tokens there are.
 template <typename T, int N>
@@ -117,13 +129,10 @@ struct SplitShape {
   static constexpr size_t kSmem = 1024 + (size_t)kStages * kStage + kScales + 256;
 };
 
-// A tile is `ch` channels (32, 64 or 128) x TN tokens.  With fewer than 128 channels the accumulator rows behind
-// them are products of whatever lies in shared memory there, and nobody reads them: narrow tiles bring the
-// weight of a small batch into more SMs at once without another cut through K.
 template <int TN, typename T>
 __global__ void __launch_bounds__(kSplitThreads, 1)
 gemm_i8_split_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_t, Params p, int split,
-                     int ch, int* error_word) {
+                     int* error_word) {
   using S = SplitShape<TN>;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
@@ -137,8 +146,8 @@ gemm_i8_split_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int channel_tiles = (p.n + ch - 1) / ch, tile = blockIdx.x / split;
-  const int n0 = tile % channel_tiles * ch, m0 = tile / channel_tiles * TN;
+  const int channel_tiles = (p.n + kChannels - 1) / kChannels, tile = blockIdx.x / split;
+  const int n0 = tile % channel_tiles * kChannels, m0 = tile / channel_tiles * TN;
   const int rank = split > 1 ? (int)cluster_ctarank() : 0;
   const int KT_all = (p.k + KB - 1) / KB;
   const int kt0 = (int)((long long)KT_all * rank / split), KT = (int)((long long)KT_all * (rank + 1) / split) - kt0;
@@ -179,7 +188,7 @@ gemm_i8_split_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
         ok = mbar_wait(bar_empty + 8 * s, ((kt / S::kStages) & 1u) ^ 1u, abort_flag, error_word);
         if (!ok) break;
         const uint32_t sw = base + s * S::kStage;
-        mbar_expect_tx(bar_full + 8 * s, (uint32_t)((ch + TN) * KB));
+        mbar_expect_tx(bar_full + 8 * s, S::kStage);
         tma_load_2d(sw, &tmap_w, (kt0 + kt) * KB, n0, bar_full + 8 * s);
         tma_load_2d(sw + kChannels * KB, &tmap_t, (kt0 + kt) * KB, m0, bar_full + 8 * s);
       }
@@ -209,9 +218,8 @@ gemm_i8_split_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
   }
   // warp (q, half): channels 32 q .., every other piece of 16 tokens
   const int q = warp & 3, half = (warp - 2) >> 2;
-  const bool reads = warp >= 2 && ok && q * 32 < ch;
   bool done = false;
-  if (reads) {
+  if (warp >= 2 && ok) {
     done = __all_sync(0xffffffffu, mbar_wait(bar_done, 0, abort_flag, error_word)) != 0;
     tc_fence_after();
   }
@@ -247,7 +255,7 @@ gemm_i8_split_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
     cluster_sync_all();
     if (ok) {
       // A piece of work is four adjacent channels of a token; the ranks take tokens in turn.
-      const int per_token = ch / 4;
+      constexpr int per_token = kChannels / 4;
       const int pieces = (tokens - rank + split - 1) / split * per_token;
       for (int i = threadIdx.x; i < pieces; i += kSplitThreads) {
         const int t = rank + i / per_token * split, n = n0 + i % per_token * 4;
@@ -299,12 +307,12 @@ gemm_i8_split_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
 
 // ---------------------------------------------------------------- pair kernel
 
-constexpr int kPairStage = 32768;  // 128 channels and 128 tokens x 128 bytes per CTA
+constexpr int kPairStage = 32768;  // 128 tokens and 128 channels x 128 bytes per CTA
 constexpr int kPairStages = 6;
 constexpr int kPairThreads = 320;  // producer, MMA issuer, eight epilogue warps
-constexpr int kPairTokens = 256;
-constexpr int kPairScales = 8 * (kPairTokens / 2) * 4;  // every epilogue warp's 128 token scales
-constexpr size_t kPairSmem = 1024 + (size_t)kPairStages * kPairStage + kPairScales + 256;
+constexpr int kPairTile = 256;     // tokens and channels
+constexpr int kPairStaging = 8 * 4096;  // per epilogue warp 32 tokens x 128 bytes of C, swizzled
+constexpr size_t kPairSmem = 1024 + (size_t)kPairStages * kPairStage + kPairStaging + 256;
 constexpr int kBand = 8;
 
 struct PairTiles {
@@ -313,24 +321,25 @@ struct PairTiles {
 };
 // Bands of eight token tiles, inside a band the channel tile advances slowest: the tiles in flight share the
 // panels of both operands through L2.
-__device__ __forceinline__ void tile_coords(const PairTiles& t, int tile, int* channel0, int* token0) {
+__device__ __forceinline__ void tile_coords(const PairTiles& t, int tile, int* token0, int* channel0) {
   const int band = tile / (kBand * t.channels), rem = tile - band * (kBand * t.channels);
   const int rows = min(kBand, t.tokens - band * kBand);
   const int c = rem / rows;
-  *channel0 = c * (2 * kChannels);
-  *token0 = (band * kBand + rem - c * rows) * kPairTokens;
+  *channel0 = c * kPairTile;
+  *token0 = (band * kBand + rem - c * rows) * kPairTile;
 }
 
-template <typename T>
+// TMA_STORE: C goes out by TMA from the staging tiles (rows of whole 16-byte pieces at 16-byte addresses); else a
+// warp writes its staging tile row by row, one or two values a lane.
+template <typename T, bool TMA_STORE>
 __global__ void __launch_bounds__(kPairThreads, 1)
-gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_t, Params p, PairTiles tiles,
-                    int* error_word) {
+gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
+                    const __grid_constant__ CUtensorMap tmap_c, Params p, PairTiles tiles, int* error_word) {
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
   const uint32_t base = (raw + 1023u) & ~1023u;
   uint8_t* gen_base = smem_raw + (base - raw);
-  float* scales = reinterpret_cast<float*>(gen_base + kPairStages * kPairStage);
-  constexpr int kBars = kPairStages * kPairStage + kPairScales;
+  constexpr int kBars = kPairStages * kPairStage + kPairStaging;
   const uint32_t bars = base + kBars;
   const uint32_t bar_full = bars, bar_empty = bars + 8 * kPairStages;
   const uint32_t bar_tfull = bars + 16 * kPairStages, bar_tempty = bar_tfull + 16;
@@ -344,8 +353,9 @@ gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
   const int KT = (p.k + KB - 1) / KB;
 
   if (threadIdx.x == 0) {
-    prefetch_tensormap(&tmap_w);
-    prefetch_tensormap(&tmap_t);
+    prefetch_tensormap(&tmap_a);
+    prefetch_tensormap(&tmap_b);
+    if (TMA_STORE) prefetch_tensormap(&tmap_c);
     for (int s = 0; s < kPairStages; ++s) {
       mbar_init(bar_full + 8 * s, 1);   // the leader's expect_tx arrival; bytes come from both CTAs
       mbar_init(bar_empty + 8 * s, 1);  // one commit
@@ -373,19 +383,19 @@ gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
         uint32_t kit = 0;
         bool ok = true;
         for (int tile = pair; tile < tiles.count && ok; tile += pairs) {
-          int n0, m0;
-          tile_coords(tiles, tile, &n0, &m0);
-          n0 += (int)rank * kChannels;
-          m0 += (int)rank * (kPairTokens / 2);
+          int m0, n0;
+          tile_coords(tiles, tile, &m0, &n0);
+          m0 += (int)rank * (kPairTile / 2);
+          n0 += (int)rank * (kPairTile / 2);
           for (int kt = 0; kt < KT; ++kt, ++kit) {
             const int s = kit % kPairStages;
             ok = mbar_wait(bar_empty + 8 * s, ((kit / kPairStages) & 1u) ^ 1u, abort_flag, error_word);
             if (!ok) break;
-            const uint32_t sw = base + s * kPairStage;
+            const uint32_t sa = base + s * kPairStage;
             const uint32_t full_leader = mapa_u32(bar_full + 8 * s, 0);
             if (leader) mbar_expect_tx(bar_full + 8 * s, 2 * kPairStage);
-            tma_load_2d_pair(sw, &tmap_w, kt * KB, n0, full_leader);
-            tma_load_2d_pair(sw + kChannels * KB, &tmap_t, kt * KB, m0, full_leader);
+            tma_load_2d_pair(sa, &tmap_a, kt * KB, m0, full_leader);
+            tma_load_2d_pair(sa + kPairStage / 2, &tmap_b, kt * KB, n0, full_leader);
           }
         }
       }
@@ -398,57 +408,114 @@ gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
           ok = mbar_wait(bar_tempty + 8 * acc, ((count >> 1) & 1u) ^ 1u, abort_flag, error_word);
           if (!ok) break;
           tc_fence_after();
-          const uint32_t tmem_d = tmem_base + acc * (uint32_t)kPairTokens;
+          const uint32_t tmem_d = tmem_base + acc * (uint32_t)kPairTile;
           for (int kt = 0; kt < KT; ++kt, ++kit) {
             const int s = kit % kPairStages;
             ok = mbar_wait(bar_full + 8 * s, (kit / kPairStages) & 1u, abort_flag, error_word);
             if (!ok) break;
             tc_fence_after();
-            const uint32_t sw = base + s * kPairStage, st = sw + kChannels * KB;
+            const uint32_t sa = base + s * kPairStage, sb = sa + kPairStage / 2;
 #pragma unroll
             for (int kk = 0; kk < 4; ++kk)
-              umma_pair_i8(tmem_d, smem_desc(sw + kk * 32, 16, 1024, 2), smem_desc(st + kk * 32, 16, 1024, 2),
-                           i8_idesc(2 * kChannels, kPairTokens), (kt | kk) != 0 ? 1u : 0u);
+              umma_pair_i8(tmem_d, smem_desc(sa + kk * 32, 16, 1024, 2), smem_desc(sb + kk * 32, 16, 1024, 2),
+                           i8_idesc(kPairTile, kPairTile), (kt | kk) != 0 ? 1u : 0u);
             umma_commit_pair(bar_empty + 8 * s);
           }
           if (ok) umma_commit_pair(bar_tfull + 8 * acc);
         }
       }
     } else {
-      // warp (q, half): accumulator rows 32 q .., token columns 128 half ..
+      // warp (q, half): tokens 32 q .. of this CTA's 128, channels 128 half ..; a lane is a token
+      constexpr int COLS = 128 / (int)sizeof(T);  // channels of a chunk: 128 bytes of C
       const int q = warp & 3, half = (warp - 2) >> 2;
+      uint8_t* const stg = gen_base + kPairStages * kPairStage + (warp - 2) * 4096;
       uint32_t count = 0;
       bool ok = true;
       for (int tile = pair; tile < tiles.count && ok; tile += pairs, ++count) {
-        int n0, m0;
-        tile_coords(tiles, tile, &n0, &m0);
+        int m0, n0;
+        tile_coords(tiles, tile, &m0, &n0);
+        m0 += (int)rank * (kPairTile / 2) + q * 32;
+        n0 += half * (kPairTile / 2);
         const uint32_t acc = count & 1u;
-        const int n = n0 + (int)rank * kChannels + q * 32 + lane;
-        const bool in = n < p.n;
-        const float sb = in ? p.scale_b[n] : 0.0f, bias = in && p.bias ? p.bias[n] : 0.0f;
-        m0 += half * (kPairTokens / 2);
-        float* const sa = scales + (warp - 2) * (kPairTokens / 2);  // (each warp its own: no warp waits for another)
-        for (int j = lane; j < kPairTokens / 2; j += 32) sa[j] = m0 + j < p.m ? p.scale_a[m0 + j] : 0.0f;
-        __syncwarp();
+        // four channels a lane of the warp's 128, handed round by shuffles below
+        float sb[4], bias[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int n = n0 + 4 * lane + e;
+          sb[e] = n < p.n ? p.scale_b[n] : 0.0f;
+          bias[e] = n < p.n && p.bias ? p.bias[n] : 0.0f;
+        }
+        const float sa = m0 + lane < p.m ? p.scale_a[m0 + lane] : 0.0f;
         ok = __all_sync(0xffffffffu, mbar_wait(bar_tfull + 8 * acc, (count >> 1) & 1u, abort_flag, error_word)) != 0;
         if (!ok) break;
         tc_fence_after();
-        const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16) + acc * (uint32_t)kPairTokens + half * (kPairTokens / 2);
-        const int tokens = min(kPairTokens / 2, p.m - m0);
+        const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16) + acc * (uint32_t)kPairTile + half * (kPairTile / 2);
+        uint32_t r[32];
+        if (m0 < p.m && n0 < p.n) tmem_ld32(taddr, r);
 #pragma unroll 1
-        for (int c0 = 0; c0 < tokens; c0 += 32) {
-          uint32_t r[32];
-          tmem_ld32(taddr + c0, r);
-          tmem_ld_wait();
-          finish_columns<T, 32>(p, r, sa + c0, sb, bias, static_cast<T*>(p.c) + (m0 + c0) * p.ldc + n, tokens - c0, in);
-          __syncwarp();
+        for (int c0 = 0; c0 < kPairTile / 2; c0 += COLS) {
+          if (m0 >= p.m || n0 + c0 >= p.n) break;  // warp-uniform
+          uint32_t words[32];  // the lane's 128 bytes
+#pragma unroll
+          for (int h = 0; h < COLS / 32; ++h) {
+            float v[32];
+            const int first = (c0 + 32 * h) / 4;
+            tmem_ld_wait();
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              v[j] = scaled((int)r[j], sa, __shfl_sync(0xffffffffu, sb[j & 3], first + (j >> 2)),
+                            __shfl_sync(0xffffffffu, bias[j & 3], first + (j >> 2)));
+            // (channels behind n are products of zeros with a scale of zero)
+            if (c0 + 32 * h + 32 < kPairTile / 2) tmem_ld32(taddr + c0 + 32 * h + 32, r);
+            activate(p.act, v);
+            if (sizeof(T) == 4) {
+#pragma unroll
+              for (int j = 0; j < 32; ++j) words[j] = __float_as_uint(v[j]);
+            } else {
+#pragma unroll
+              for (int j = 0; j < 16; ++j) words[16 * h + j] = pack2<T>(v[2 * j], v[2 * j + 1]);
+            }
+          }
+          if (TMA_STORE) {
+            if (lane == 0) bulk_wait_read<0>();  // the chunk before has left the staging tile
+            __syncwarp();
+          }
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            *reinterpret_cast<uint4*>(stg + lane * 128 + ((j ^ (lane & 7)) << 4)) =
+                make_uint4(words[4 * j], words[4 * j + 1], words[4 * j + 2], words[4 * j + 3]);
+          if (TMA_STORE) {
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) {
+              tma_store_2d(&tmap_c, n0 + c0, m0, smem_u32(stg));
+              bulk_commit();
+            }
+          } else {
+            __syncwarp();
+            constexpr int PER = COLS / 32;  // values a lane
+            const int n = n0 + c0 + lane * PER;
+#pragma unroll 4
+            for (int t = 0; t < 32; ++t) {
+              if (m0 + t >= p.m) break;
+              const T* from = reinterpret_cast<const T*>(stg + t * 128 + (((lane >> 2) ^ (t & 7)) << 4) + (lane & 3) * 4);
+              T* const out = static_cast<T*>(p.c) + (m0 + t) * p.ldc + n;
+#pragma unroll
+              for (int e = 0; e < PER; ++e)
+                if (n + e < p.n) out[e] = from[e];
+            }
+            __syncwarp();
+          }
         }
+        tmem_ld_wait();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive_cluster(mapa_u32(bar_tempty + 8 * acc, 0));
       }
+      if (TMA_STORE && lane == 0) bulk_wait_all();  // the stores read this CTA's shared memory
     }
   }
+  __syncwarp();
   tc_fence_before();
   __syncthreads();
   cluster_sync_all();  // the peer may read this CTA's shared memory until its last MMA is done
@@ -460,23 +527,26 @@ gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
 
 // ---------------------------------------------------------------- host
 
-int make_map(CUtensorMap* map, const int8_t* ptr, long long rows, long long cols, long long ld, int box_rows) {
+int make_map(CUtensorMap* map, CUtensorMapDataType type, int bytes, const void* ptr, long long rows, long long cols, long long ld,
+             int box_cols, int box_rows) {
   EncodeTiledFn fn = encode_fn();
   if (!fn) return fail(ANNC_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
   const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
-  const cuuint64_t strides[1] = {(cuuint64_t)ld};
-  const cuuint32_t box[2] = {KB, (cuuint32_t)box_rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)ld * bytes};
+  const cuuint32_t box[2] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows};
   const cuuint32_t estr[2] = {1, 1};
-  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<int8_t*>(ptr), dims, strides, box, estr,
-                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  CUresult r = fn(map, type, 2, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return fail(ANNC_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
   return ANNC_OK;
 }
+int operand_map(CUtensorMap* map, const int8_t* ptr, long long rows, long long k, long long ld, int box_rows) {
+  return make_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, ptr, rows, k, ld, KB, box_rows);
+}
 
 template <int TN, typename T>
-int launch_split(const Params& p, int split, int ch, int* error_word, cudaStream_t s) {
-  void (*const kernel)(CUtensorMap, CUtensorMap, Params, int, int, int*) = gemm_i8_split_kernel<TN, T>;
+int launch_split(const Params& p, int split, int* error_word, cudaStream_t s) {
+  void (*const kernel)(CUtensorMap, CUtensorMap, Params, int, int*) = gemm_i8_split_kernel<TN, T>;
   static bool attr_done[kMaxDevices] = {};
   const int dev = device_slot();
   if (!attr_done[dev]) {
@@ -485,8 +555,8 @@ int launch_split(const Params& p, int split, int ch, int* error_word, cudaStream
     attr_done[dev] = true;
   }
   CUtensorMap tw, tt;
-  ANNC_TRY(make_map(&tw, p.b, p.n, p.k, p.ldb, ch));
-  ANNC_TRY(make_map(&tt, p.a, p.m, p.k, p.lda, TN));
+  ANNC_TRY(operand_map(&tw, p.b, p.n, p.k, p.ldb, kChannels));
+  ANNC_TRY(operand_map(&tt, p.a, p.m, p.k, p.lda, TN));
   cudaLaunchConfig_t cfg;
   memset(&cfg, 0, sizeof(cfg));
   cudaLaunchAttribute attr[2];
@@ -495,19 +565,19 @@ int launch_split(const Params& p, int split, int ch, int* error_word, cudaStream
   attr[1].val.clusterDim.x = (unsigned)split;
   attr[1].val.clusterDim.y = 1;
   attr[1].val.clusterDim.z = 1;
-  cfg.gridDim = dim3((unsigned)split * (unsigned)((p.n + ch - 1) / ch) * (unsigned)((p.m + TN - 1) / TN), 1, 1);
+  cfg.gridDim = dim3((unsigned)split * (unsigned)((p.n + kChannels - 1) / kChannels) * (unsigned)((p.m + TN - 1) / TN), 1, 1);
   cfg.blockDim = dim3(kSplitThreads, 1, 1);
   cfg.dynamicSmemBytes = SplitShape<TN>::kSmem;
   cfg.stream = s;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  ANNC_CUDA(cudaLaunchKernelEx(&cfg, kernel, tw, tt, p, split, ch, error_word));
+  ANNC_CUDA(cudaLaunchKernelEx(&cfg, kernel, tw, tt, p, split, error_word));
   return ANNC_OK;
 }
 
-template <typename T>
-int launch_pair(const Params& p, int* error_word, cudaStream_t s) {
-  void (*const kernel)(CUtensorMap, CUtensorMap, Params, PairTiles, int*) = gemm_i8_pair_kernel<T>;
+template <typename T, bool TMA_STORE>
+int launch_pair_as(const Params& p, int* error_word, cudaStream_t s) {
+  void (*const kernel)(CUtensorMap, CUtensorMap, CUtensorMap, Params, PairTiles, int*) = gemm_i8_pair_kernel<T, TMA_STORE>;
   static int max_pairs_dev[kMaxDevices] = {};
   int& max_pairs = max_pairs_dev[device_slot()];
   cudaLaunchConfig_t cfg;
@@ -530,44 +600,71 @@ int launch_pair(const Params& p, int* error_word, cudaStream_t s) {
     if (n < 1) return fail(ANNC_ERR_CUDA, "no CTA pair fits this device");
     max_pairs = n;
   }
-  CUtensorMap tw, tt;
-  ANNC_TRY(make_map(&tw, p.b, p.n, p.k, p.ldb, kChannels));
-  ANNC_TRY(make_map(&tt, p.a, p.m, p.k, p.lda, kPairTokens / 2));
+  CUtensorMap ta, tb, tc;
+  ANNC_TRY(operand_map(&ta, p.a, p.m, p.k, p.lda, kPairTile / 2));
+  ANNC_TRY(operand_map(&tb, p.b, p.n, p.k, p.ldb, kPairTile / 2));
+  if (TMA_STORE)
+    ANNC_TRY(make_map(&tc, sizeof(T) == 4 ? CU_TENSOR_MAP_DATA_TYPE_UINT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, sizeof(T), p.c, p.m,
+                      p.n, p.ldc, 128 / (int)sizeof(T), 32));
+  else tc = ta;
   PairTiles t;
-  t.channels = (p.n + 2 * kChannels - 1) / (2 * kChannels);
-  t.tokens = (p.m + kPairTokens - 1) / kPairTokens;
+  t.channels = (p.n + kPairTile - 1) / kPairTile;
+  t.tokens = (p.m + kPairTile - 1) / kPairTile;
   t.count = t.channels * t.tokens;
   cfg.gridDim.x = 2u * (unsigned)(t.count < max_pairs ? t.count : max_pairs);
   cfg.stream = s;
   cfg.numAttrs = 2;
-  ANNC_CUDA(cudaLaunchKernelEx(&cfg, kernel, tw, tt, p, t, error_word));
+  ANNC_CUDA(cudaLaunchKernelEx(&cfg, kernel, ta, tb, tc, p, t, error_word));
   return ANNC_OK;
+}
+template <typename T>
+int launch_pair(const Params& p, int* error_word, cudaStream_t s) {
+  constexpr int kPiece = 16 / (int)sizeof(T);
+  // (a TMA store clips at the tensor's edge in pieces of 16 bytes)
+  const bool tma = (reinterpret_cast<uintptr_t>(p.c) & 15) == 0 && p.ldc % kPiece == 0 && p.n % kPiece == 0 &&
+                   p.ldc * (long long)sizeof(T) < (1LL << 40);
+  return tma ? launch_pair_as<T, true>(p, error_word, s) : launch_pair_as<T, false>(p, error_word, s);
 }
 
 }  // namespace
 
+// Which kernel and shape: the smallest of their times as these sums model them (us, bf16 output, figures fitted to
+// 40 products from 1 x 512 x 256 to 16384 x 8192 x 256; 148 SMs).
+//   split  2.7 for launch and prologue; per round of CTAs a k-step 0.21 + 0.00043 TN (latency: a CTA streams alone on
+//          its SM) and, unsplit, 0.0105 TN to write the tile; split, once 1.0 + 0.016 TN for the sums of the cluster
+//   pair   6.1 for launch, prologue and the last tile's epilogue; a k-step 0.33, a tile at least the 3.3 that the
+//          epilogue under it takes
+// Measured, split kernel's best / pair: 1024 x 1024 x 1024 5.5 / 7.9, 512 x 4096 x 2048 8.6 / 10.6, 1024 x 4096 x 2048 10.3 /
+// 11.6, 2048 x 1024 x 8192 19.6 / 24.7, 4096 x 1024 x 8192 25.0 / 26.1, 700 x 8192 x 4096 27.9 / 25.8, 2048 x 4096 x 2048
+// 20.1 / 17.3, 8192 x 4096 x 2048 80 / 53.
 Route route_of(const Params& p) {
-  Route r = {ROUTE_SIMT, 0, 0, 0};
+  Route best = {ROUTE_SIMT, 0, 0};
   // TMA wants rows on 16 bytes
-  if (p.k < 1 || ((reinterpret_cast<uintptr_t>(p.a) | reinterpret_cast<uintptr_t>(p.b)) & 15) || p.lda % 16 || p.ldb % 16) return r;
-  const long long tiles_m = (p.m + 255LL) / 256, pair_tiles = tiles_m * ((p.n + 255LL) / 256);
-  if (pair_tiles > (1LL << 30)) return r;
-  if (p.m > 128 && p.n > 128 && pair_tiles >= 37) {
-    r.kind = ROUTE_PAIR;
-    return r;
-  }
-  int tn = 16;
-  while (tn < 256 && tn < p.m) tn *= 2;
-  const long long tiles = ((p.n + 127LL) / 128) * ((p.m + tn - 1LL) / tn);
+  if (p.k < 1 || ((reinterpret_cast<uintptr_t>(p.a) | reinterpret_cast<uintptr_t>(p.b)) & 15) || p.lda % 16 || p.ldb % 16) return best;
   const int kt = (p.k + KB - 1) / KB;
-  int split = 1;
-  while (split < 8 && tiles * split * 2 <= 148 && kt >= 2 * split) split *= 2;
-  if (tiles * split > 0x7fffffffLL) return r;
-  r.kind = ROUTE_SPLIT;
-  r.tokens = tn;
-  r.split = split;
-  r.channels = 128;
-  return r;
+  const long long pair_tiles = ((p.m + 255LL) / 256) * ((p.n + 255LL) / 256);
+  if (pair_tiles > (1LL << 30)) return best;
+  const double main = 0.33 * kt;
+  const long long pair_rounds = (pair_tiles + 73) / 74;
+  double us = 6.1 + main + (double)(pair_rounds - 1) * (main > 3.3 ? main : 3.3);
+  best.kind = ROUTE_PAIR;
+  for (int tn = 16; tn <= 256; tn *= 2) {
+    const long long tiles = ((p.n + 127LL) / 128) * ((p.m + tn - 1LL) / tn);
+    if (tiles > (1LL << 20)) continue;
+    // (15 clusters of eight, 33 of four and 74 of two CTAs fit the chip at once)
+    for (int split = 1; split <= 8 && split <= kt; split *= 2) {
+      if (split > 1 && tiles > (split == 8 ? 15 : split == 4 ? 33 : 74)) break;
+      const long long rounds = (tiles * split + 147) / 148;
+      const double step = 0.21 + 0.00043 * tn;
+      const double t = 2.7 + (double)rounds * ((kt + split - 1) / split * step + (split == 1 ? 0.0105 * tn : 0.0)) +
+                       (split > 1 ? 1.0 + 0.016 * tn : 0.0);
+      if (t < us) {
+        us = t;
+        best = {ROUTE_SPLIT, tn, split};
+      }
+    }
+  }
+  return best;
 }
 
 namespace {
@@ -577,11 +674,11 @@ int run_as(const Params& p, const Route& r, cudaStream_t s) {
   if (!word) return fail(ANNC_ERR_CUDA, "gemm error word is not addressable");
   if (r.kind == ROUTE_PAIR) return launch_pair<T>(p, word, s);
   switch (r.tokens) {
-    case 16: return launch_split<16, T>(p, r.split, r.channels, word, s);
-    case 32: return launch_split<32, T>(p, r.split, r.channels, word, s);
-    case 64: return launch_split<64, T>(p, r.split, r.channels, word, s);
-    case 128: return launch_split<128, T>(p, r.split, r.channels, word, s);
-    default: return launch_split<256, T>(p, r.split, r.channels, word, s);
+    case 16: return launch_split<16, T>(p, r.split, word, s);
+    case 32: return launch_split<32, T>(p, r.split, word, s);
+    case 64: return launch_split<64, T>(p, r.split, word, s);
+    case 128: return launch_split<128, T>(p, r.split, word, s);
+    default: return launch_split<256, T>(p, r.split, word, s);
   }
 }
 }  // namespace
