@@ -117,7 +117,7 @@ def _load() -> C.CDLL:
                                             C.c_double, C.POINTER(C.c_double), C.POINTER(C.c_float)]
     lib.annc_rotary_dev.argtypes = [C.c_void_p, C.c_void_p]
     lib.annc_prefix_attention_workspace_bytes.restype = C.c_size_t
-    lib.annc_prefix_attention_workspace_bytes.argtypes = [C.c_int64, C.c_int32, C.c_int32]
+    lib.annc_prefix_attention_workspace_bytes.argtypes = [C.c_int64, C.c_int32, C.c_int32, C.c_int32]
     lib.annc_prefix_attention_dev.argtypes = [C.c_void_p, C.c_void_p]
     lib.annc_embed_bag_workspace_bytes.restype = C.c_size_t
     lib.annc_embed_bag_workspace_bytes.argtypes = [C.c_int, C.c_int64]

@@ -11,59 +11,17 @@
 #include <cstdint>
 
 #include "common.h"
+#include "prefix_attention.h"
 
 namespace annc {
 namespace attention {
 
 namespace {
 
-struct Rows {  // [rows, heads, head_dim] with strides in elements
-  const void* data;
-  long long row, head;
-};
-struct Params {
-  Rows q, kp, vp, ko, vo;
-  void* out;
-  long long out_row, out_head;
-  float* lse;
-  const int64_t* own_begin;
-  const int32_t* own_len;
-  const int32_t* q_begin;
-  long long tokens, sequences, prefix, own_rows;
-  int heads, group, dim;
-  float scale;
-};
-
 __device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
 __device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
 __device__ __forceinline__ void from_float(float x, __nv_bfloat16* y) { *y = __float2bfloat16_rn(x); }
 __device__ __forceinline__ void from_float(float x, __half* y) { *y = __float2half_rn(x); }
-
-// The keys of a token's own sequence that it sees: rows first .. first + count - 1 of the own keys.  False for a
-// token that belongs to no sequence.  Bounds are clamped, whatever the arrays hold: no row outside the buffer is read.
-__device__ __forceinline__ bool own_keys(const Params& p, long long token, long long* first, int* count) {
-  *first = 0;
-  *count = 0;
-  long long seq = token;
-  long long behind = 0;  // tokens of the sequence behind this one
-  if (p.q_begin) {
-    if (p.sequences == 0 || token < p.q_begin[0] || token >= p.q_begin[p.sequences]) return false;
-    long long lo = 0, hi = p.sequences;  // q_begin[lo] <= token < q_begin[hi]
-    while (hi - lo > 1) {
-      const long long mid = (lo + hi) >> 1;
-      if (p.q_begin[mid] <= token) lo = mid;
-      else hi = mid;
-    }
-    seq = lo;
-    behind = (long long)p.q_begin[seq + 1] - 1 - token;
-  }
-  if (!p.own_len) return true;
-  const long long begin = p.own_begin[seq], len = p.own_len[seq] - behind;
-  if (len <= 0 || begin < 0 || begin >= p.own_rows) return true;
-  *first = begin;
-  *count = (int)min(len, p.own_rows - begin);
-  return true;
-}
 
 constexpr int kMaxDim = 256;
 
@@ -168,6 +126,7 @@ Params params_of(const annc_prefix_attention_desc& d) {
   p.prefix = d.prefix_len;
   p.own_rows = d.own_rows;
   p.heads = d.heads;
+  p.kv_heads = d.kv_heads;
   p.group = d.heads / d.kv_heads;
   p.dim = d.head_dim;
   p.scale = d.scale;
@@ -182,13 +141,23 @@ using namespace annc;
 
 extern "C" {
 
-size_t annc_prefix_attention_workspace_bytes(int64_t tokens, int32_t heads, int32_t head_dim) { return 0; }
+size_t annc_prefix_attention_workspace_bytes(int64_t tokens, int32_t heads, int32_t kv_heads, int32_t head_dim) {
+  if (tokens < 1 || kv_heads < 1 || heads < kv_heads || heads % kv_heads || head_dim < 1) return 0;
+  return attention::tc_workspace_bytes(tokens, heads, kv_heads, head_dim);
+}
 
 int annc_prefix_attention_dev(const annc_prefix_attention_desc* desc, void* stream) {
   ANNC_REQUIRE(desc, ANNC_ERR_INVALID_ARGUMENT, "prefix attention: null descriptor");
   ANNC_TRY(attention::validate(*desc));
   if (desc->tokens == 0) return ANNC_OK;
-  return attention::run_rows(attention::params_of(*desc), desc->dtype, static_cast<cudaStream_t>(stream));
+  const size_t need = annc_prefix_attention_workspace_bytes(desc->tokens, desc->heads, desc->kv_heads, desc->head_dim);
+  ANNC_REQUIRE(need == 0 || (desc->workspace && (reinterpret_cast<uintptr_t>(desc->workspace) & 15) == 0 &&
+                             desc->workspace_bytes >= need), ANNC_ERR_INVALID_ARGUMENT,
+               "prefix attention: workspace missing, too small or not 16-byte aligned");
+  const attention::Params p = attention::params_of(*desc);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return attention::tc_supported(p, desc->dtype) ? attention::run_tc(p, desc->dtype, desc->workspace, s)
+                                                 : attention::run_rows(p, desc->dtype, s);
 }
 
 }  // extern "C"

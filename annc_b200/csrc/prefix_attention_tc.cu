@@ -1,0 +1,749 @@
+// Shared-prefix attention on the 5th-generation tensor cores: one kernel takes all rows against the prefix, a second
+// one adds the keys of each sequence and joins the parts.
+//
+// Prefix kernel.  A CTA walks through its share of key tiles (plan_of in prefix_attention.h).  Per key tile of 128 keys and
+// tile of 128 rows:  S = Q K^T (tcgen05, operands in shared memory, S in tensor memory), softmax numerators P in
+// registers (a thread per row), P back to tensor memory over S as the operand of  O += P V  (V as it lies, N-major).
+// Two such chains run side by side so that one's products cover the other's exponentials: with more than 128 rows
+// in the item the two are its two row tiles, sharing the key tiles; else they take the key tiles in turn and leave a
+// part each.  The running maximum of a row only moves when a score passes it by more than 2^8 in the
+// exponential: until then O keeps its scale, the numerators grow to at most 256, and O is rescaled hardly ever.
+//
+//   warps 0-3, 4-7   softmax of the two chains, rescaling of O, parts
+//   warp 8           TMA: rows, then keys and values through a ring of tiles
+//   warp 9           tensor memory, all products
+//
+// Join kernel.  Warps take (token, key head): its up to 16 heads at a time against the token's own keys with
+// mma.sync straight from global memory (each lane reads 16-byte pieces; the order of the head's values in the products is
+// permuted alike on both sides, so that no transposition is needed), then all parts are added.
+//
+// Sums, maxima and O are held in fp32; the numerators are rounded to the operands' type for the second product, as the
+// tensor cores want them, while their sum is of the unrounded ones.
+#include <cuda.h>
+
+#include <cmath>
+#include <cstdint>
+#include <cstring>
+#include <type_traits>
+
+#include "common.h"
+#include "pdl.cuh"
+#include "prefix_attention.h"
+#include "tc_host.h"
+#include "tc_ptx.cuh"
+
+namespace annc {
+namespace gemm {
+int* gemm_error_word();  // device address of the tensor-core kernels' error word (gemm_tc.cu)
+}
+namespace attention {
+
+namespace {
+
+using namespace annc::tc;
+
+constexpr int kThreads = 320;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr float kSlack = 8.0f;  // log2 of what a numerator may grow to before the maximum moves
+
+template <int DP>
+struct Shape {
+  static constexpr int kTile = kTileKeys * DP * 2;  // bytes of 128 rows: DP / 64 blocks of 128 bytes x 128
+  static constexpr int kSlots = DP == 128 ? 5 : 9;
+  static constexpr int kBars = 2 * kTile + kSlots * kTile;
+  static constexpr size_t kSmem = 1024 + kBars + 256;
+};
+
+struct PrefixParams {
+  Plan plan;
+  long long tokens;
+  int kv_heads, group, prefix;
+  float scale2;  // scale * log2(e)
+  float* parts;  // [part][256][DP]
+  float2* stats; // [part][256]: maximum (log2 units), sum
+  int* error_word;
+};
+
+// ---------------------------------------------------------------- PTX
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, int w, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
+      "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ void umma_f16_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void umma_f16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]),
+      "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]),
+      "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  uint32_t w;
+  memcpy(&w, &v, 4);
+  return w;
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  uint32_t w;
+  memcpy(&w, &v, 4);
+  return w;
+}
+
+// ---------------------------------------------------------------- prefix kernel
+
+// What a CTA does of one item: key tiles first .. first + count - 1.
+struct Segment {
+  int item, head, tile;  // key head, pair of row tiles
+  int first, count;
+  int part;
+  bool dual;  // two row tiles; else the chains take the key tiles in turn
+  __device__ __forceinline__ int steps(int chain) const { return dual ? count : (count - chain + 1) / 2; }
+  __device__ __forceinline__ int key_tile(int chain, int step) const { return first + (dual ? step : 2 * step + chain); }
+};
+__device__ __forceinline__ Segment segment_at(const PrefixParams& p, int at, int begin, int end) {
+  Segment s;
+  s.item = at / p.plan.kv_tiles;
+  s.first = at - s.item * p.plan.kv_tiles;
+  s.count = min(p.plan.kv_tiles - s.first, end - at);
+  s.head = s.item / p.plan.row_items;
+  s.tile = s.item - s.head * p.plan.row_items;
+  s.dual = p.tokens - (long long)s.tile * 2 * p.plan.tile_tokens > p.plan.tile_tokens;
+  const bool whole = s.count == p.plan.kv_tiles;
+  s.part = whole ? 2 * kMaxCtas + s.item : 2 * (int)blockIdx.x + (at == begin ? 0 : 1);
+  return s;
+}
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kThreads, 1)
+prefix_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
+              const __grid_constant__ CUtensorMap tmap_v, PrefixParams p) {
+  using S = Shape<DP>;
+  constexpr int kBlock = kTileKeys * 128;  // bytes of a block of 64 values x 128 rows
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw);
+  const uint32_t base = (raw + 1023u) & ~1023u;
+  const uint32_t q_smem = base, ring = base + 2 * S::kTile, bars = base + S::kBars;
+  const uint32_t bar_full = bars, bar_empty = bars + 8 * S::kSlots;
+  const uint32_t bar_q = bars + 16 * S::kSlots, bar_qfree = bar_q + 8;
+  const uint32_t bar_s = bar_q + 16, bar_p = bar_q + 32, bar_o = bar_q + 48, bar_ofree = bar_q + 64;  // per chain
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem_raw + (bar_q + 80 - raw));
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    prefetch_tensormap(&tmap_q);
+    prefetch_tensormap(&tmap_k);
+    prefetch_tensormap(&tmap_v);
+    for (int s = 0; s < S::kSlots; ++s) {
+      mbar_init(bar_full + 8 * s, 1);
+      mbar_init(bar_empty + 8 * s, 1);
+    }
+    mbar_init(bar_q, 1);
+    mbar_init(bar_qfree, 1);
+    for (int c = 0; c < 2; ++c) {
+      mbar_init(bar_s + 8 * c, 1);
+      mbar_init(bar_p + 8 * c, 4);
+      mbar_init(bar_o + 8 * c, 1);
+      mbar_init(bar_ofree + 8 * c, 4);
+    }
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 9) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512u) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;  // S and P of the chains at columns 0 and 128, O at 256 and 384
+  pdl_trigger();
+  pdl_wait();
+  const int total = p.plan.items * p.plan.kv_tiles;
+  const int begin = (int)blockIdx.x * p.plan.per_cta, end = min(total, begin + p.plan.per_cta);
+  const bool poisoned = *reinterpret_cast<volatile int*>(p.error_word) != 0;  // an earlier launch gave up
+  bool ok = !poisoned;
+
+  if (warp == 8) {
+    if (ok && lane == 0) {
+      uint32_t n = 0, segments = 0;
+      const uint32_t q_bytes = (uint32_t)(p.plan.tile_tokens * p.group) * 128u * (DP / 64);
+      auto load = [&](const CUtensorMap* map, int head, int tile) {
+        const int s = n % S::kSlots;
+        ok = mbar_wait(bar_empty + 8 * s, ((n / S::kSlots) & 1u) ^ 1u, abort_flag, p.error_word);
+        if (!ok) return;
+        mbar_expect_tx(bar_full + 8 * s, S::kTile);
+#pragma unroll
+        for (int b = 0; b < DP / 64; ++b)
+          tma_load_3d(ring + s * S::kTile + b * kBlock, map, 64 * b, head, tile * kTileKeys, bar_full + 8 * s);
+        ++n;
+      };
+      for (int at = begin; at < end && ok; ++segments) {
+        const Segment g = segment_at(p, at, begin, end);
+        at += g.count;
+        ok = mbar_wait(bar_qfree, (segments & 1u) ^ 1u, abort_flag, p.error_word);
+        if (!ok) break;
+        mbar_expect_tx(bar_q, g.dual ? 2 * q_bytes : q_bytes);
+        for (int c = 0; c < (g.dual ? 2 : 1); ++c)
+#pragma unroll
+          for (int b = 0; b < DP / 64; ++b)
+            tma_load_4d(q_smem + c * S::kTile + b * kBlock, &tmap_q, 64 * b, 0, g.head, (2 * g.tile + c) * p.plan.tile_tokens, bar_q);
+        for (int t = 0; t < g.count && ok; ++t) {
+          load(&tmap_k, g.head, g.first + t);
+          if (ok) load(&tmap_v, g.head, g.first + t);
+        }
+      }
+      if (!ok) {
+        // given up: the copies still in flight write this CTA's shared memory, so they are waited for (with a limit)
+        const uint32_t from = n > (uint32_t)S::kSlots ? n - S::kSlots : 0;
+        for (uint32_t i = from; i < n; ++i)
+          for (int k = 0; k < 1000000 && !mbar_try_wait(bar_full + 8 * (i % S::kSlots), (i / S::kSlots) & 1u); ++k) {
+          }
+      }
+    }
+  } else if (warp == 9) {
+    if (ok && lane == 0) {
+      constexpr uint32_t fmt = sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+      constexpr uint32_t idesc_s = (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)(kTileKeys >> 3) << 17) | ((uint32_t)(kTileRows >> 4) << 24);
+      constexpr uint32_t idesc_o =
+          (1u << 4) | (fmt << 7) | (fmt << 10) | (1u << 16) | ((uint32_t)(DP >> 3) << 17) | ((uint32_t)(kTileRows >> 4) << 24);
+      uint32_t n0 = 0, segments = 0;  // ring number of the segment's first key tile
+      uint32_t steps_done[2] = {0, 0};
+      for (int at = begin; at < end && ok; ++segments) {
+        const Segment g = segment_at(p, at, begin, end);
+        at += g.count;
+        ok = mbar_wait(bar_q, segments & 1u, abort_flag, p.error_word);
+        if (!ok) break;
+        const int most = g.steps(0);
+        for (int step = 0; step <= most && ok; ++step) {
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const int steps = g.steps(c);
+            const uint32_t t_s = tmem + 128 * c, t_o = tmem + 256 + 128 * c;
+            if (step > 0 && step <= steps) {  // O += P V of the step before
+              const uint32_t i = n0 + 2 * (uint32_t)(g.key_tile(c, step - 1) - g.first) + 1, s = i % S::kSlots;
+              ok = mbar_wait(bar_p + 8 * c, (steps_done[c] + step - 1) & 1u, abort_flag, p.error_word);
+              if (ok && step == 1) ok = mbar_wait(bar_ofree + 8 * c, (segments & 1u) ^ 1u, abort_flag, p.error_word);
+              if (ok) ok = mbar_wait(bar_full + 8 * s, (i / S::kSlots) & 1u, abort_flag, p.error_word);
+              if (!ok) break;
+              tc_fence_after();
+              const uint32_t v = ring + s * S::kTile;
+#pragma unroll
+              for (int kk = 0; kk < kTileKeys / 16; ++kk)
+                umma_f16_ts(t_o, t_s + 8 * kk, smem_desc(v + kk * 2048, kBlock, 1024, 2), idesc_o, step > 1 || kk > 0 ? 1u : 0u);
+              if (!g.dual || c == 1) umma_commit(bar_empty + 8 * s);
+              if (step == steps) umma_commit(bar_o + 8 * c);
+            }
+            if (step < steps) {  // S = Q K^T
+              const uint32_t i = n0 + 2 * (uint32_t)(g.key_tile(c, step) - g.first), s = i % S::kSlots;
+              ok = mbar_wait(bar_full + 8 * s, (i / S::kSlots) & 1u, abort_flag, p.error_word);
+              if (!ok) break;
+              tc_fence_after();
+              const uint32_t k = ring + s * S::kTile, q = q_smem + (g.dual ? c : 0) * S::kTile;
+#pragma unroll
+              for (int kk = 0; kk < DP / 16; ++kk) {
+                const uint32_t off = (kk / 4) * kBlock + (kk % 4) * 32;
+                umma_f16_ss(t_s, smem_desc(q + off, 16, 1024, 2), smem_desc(k + off, 16, 1024, 2), idesc_s, kk > 0 ? 1u : 0u);
+              }
+              if (!g.dual || c == 1) umma_commit(bar_empty + 8 * s);
+              umma_commit(bar_s + 8 * c);
+            }
+          }
+          if (step == most - 1 && ok) umma_commit(bar_qfree);  // the segment's last use of its rows
+        }
+        steps_done[0] += g.steps(0);
+        steps_done[1] += g.steps(1);
+        n0 += 2 * g.count;
+      }
+    }
+  } else if (ok) {
+    const int c = warp >> 2, q = warp & 3;
+    const int row = q * 32 + lane;  // of the tile
+    const uint32_t lanes = (uint32_t)(q * 32) << 16;
+    const uint32_t t_s = tmem + 128 * c + lanes, t_o = tmem + 256 + 128 * c + lanes;
+    const float scale = p.scale2;
+    uint32_t parts = 0, done = 0;  // parts with key tiles, steps: of this chain so far
+    for (int at = begin; at < end && ok;) {
+      const Segment g = segment_at(p, at, begin, end);
+      at += g.count;
+      const int steps = g.steps(c);
+      // rows of the tile that there are
+      const long long token0 = (long long)(2 * g.tile + (g.dual ? c : 0)) * p.plan.tile_tokens;
+      const int rows = (int)min((long long)p.plan.tile_tokens, p.tokens - token0) * p.group;
+      const bool any = q * 32 < rows;  // of this warp's
+      float top = -INFINITY, sum = 0.0f;  // top in units of log2: scale * score
+      for (int step = 0; step < steps; ++step, ++done) {
+        ok = __all_sync(0xffffffffu, mbar_wait(bar_s + 8 * c, done & 1u, abort_flag, p.error_word)) != 0;
+        if (!ok) break;
+        if (any) {
+          tc_fence_after();
+          float s[128];
+#pragma unroll
+          for (int b = 0; b < 4; ++b) tmem_ld32(t_s + 32 * b, *reinterpret_cast<uint32_t(*)[32]>(&s[32 * b]));
+          tmem_ld_wait();
+          const int valid = p.prefix - g.key_tile(c, step) * kTileKeys;
+          if (valid < kTileKeys) {
+#pragma unroll
+            for (int j = 0; j < 128; ++j)
+              if (j >= valid) s[j] = -INFINITY;
+          }
+          float m4[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+          for (int j = 4; j < 128; ++j) m4[j & 3] = fmaxf(m4[j & 3], s[j]);
+          const float now = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * scale;
+          const bool moves = now > top + kSlack || step == 0;
+          if (step == 0) {
+            top = now;
+          } else if (__any_sync(0xffffffffu, moves)) {
+            // (every product before this S is complete, O among them)
+            const float keep = moves ? exp2_approx(top - now) : 1.0f;
+            if (moves) top = now;
+            sum *= keep;
+#pragma unroll
+            for (int b = 0; b < DP / 32; ++b) {
+              uint32_t o[32];
+              tmem_ld32(t_o + 32 * b, o);
+              tmem_ld_wait();
+#pragma unroll
+              for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * keep);
+              tmem_st32(t_o + 32 * b, o);
+            }
+          }
+          float sum4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+          for (int b = 0; b < 2; ++b) {
+            uint32_t w[32];
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+              const int e = 64 * b + 2 * j;
+              float lo = exp2_approx(fmaf(s[e], scale, -top)), hi = exp2_approx(fmaf(s[e + 1], scale, -top));
+              if (valid < kTileKeys) {  // (0 * -inf is no zero where the scale is)
+                if (e >= valid) lo = 0.0f;
+                if (e + 1 >= valid) hi = 0.0f;
+              }
+              sum4[2 * (j & 1)] += lo;
+              sum4[2 * (j & 1) + 1] += hi;
+              w[j] = pack2<T>(lo, hi);
+            }
+            tmem_st32(t_s + 32 * b, w);
+          }
+          sum += (sum4[0] + sum4[1]) + (sum4[2] + sum4[3]);
+          tmem_st_wait();
+          tc_fence_before();
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar_p + 8 * c);
+      }
+      if (!ok) break;
+      // the part: rows of this chain at 128 c
+      const long long at_row = (long long)g.part * kPartRows + c * kTileRows + row;
+      if (steps > 0) {
+        ok = __all_sync(0xffffffffu, mbar_wait(bar_o + 8 * c, parts & 1u, abort_flag, p.error_word)) != 0;
+        if (!ok) break;
+        ++parts;
+      }
+      if (row < rows) p.stats[at_row] = make_float2(top, sum);
+      if (steps > 0 && any) {
+        tc_fence_after();
+#pragma unroll
+        for (int b = 0; b < DP / 32; ++b) {
+          uint32_t o[32];
+          tmem_ld32(t_o + 32 * b, o);
+          tmem_ld_wait();
+          if (row < rows) {
+            uint4* out = reinterpret_cast<uint4*>(p.parts + at_row * DP + 32 * b);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) out[j] = make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+          }
+        }
+        tc_fence_before();
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar_ofree + 8 * c);
+    }
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 9) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+  }
+}
+
+// ---------------------------------------------------------------- join kernel
+
+template <typename T>
+__device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
+template <>
+__device__ __forceinline__ void mma_16816<__nv_bfloat16>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <>
+__device__ __forceinline__ void mma_16816<__half>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+struct JoinParams {
+  Params a;
+  Plan plan;
+  float scale2;
+  const float* parts;
+  const float2* stats;
+};
+
+// WPU warps work on a (token, key head).  Rows of the products: 16 heads of the group.  In the first product the
+// four words of a lane's 16-byte piece of Q and K take the places of the k indices that the fragment layout gives the
+// lane; in the second one a lane holds values dn * DP/8 .. of four keys, dn = lane / 4, and column dn of product t is
+// value dn * DP/8 + t, so that lane l ends with the 2 * DP/8 values from (l % 4) * DP/4 on, of rows l / 4 and l / 4 + 8.
+template <typename T, int DP, int WPU>
+__global__ void __launch_bounds__(128) join_kernel(JoinParams p) {
+  constexpr int NT = DP / 8;   // values a lane holds of a value row; products of the second kind
+  constexpr int LD = DP + 4;
+  extern __shared__ float join_smem[];  // per warp: 16 rows of LD, 16 x (maximum, sum)
+  pdl_trigger();
+  pdl_wait();
+  const Params& a = p.a;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, wi = warp % WPU;
+  float* const mine = join_smem + warp * (16 * LD + 32);
+  float* const unit0 = join_smem + (warp - wi) * (16 * LD + 32);  // of the unit's first warp
+  const long long unit = (long long)blockIdx.x * (4 / WPU) + warp / WPU;
+  const long long token = unit / a.kv_heads;
+  const int h = (int)(unit - token * a.kv_heads);
+  if (token >= a.tokens) return;
+  long long first;
+  int count;
+  if (!own_keys(a, token, &first, &count)) return;  // (the whole unit)
+  const int quad = lane & 3, dn = lane >> 2;
+
+  for (int g0 = 0; g0 < a.group; g0 += 16) {
+    const int rows = min(16, a.group - g0);
+    if (count > 0) {
+      uint32_t q[DP / 32][2][4];
+#pragma unroll
+      for (int b = 0; b < DP / 32; ++b)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          uint4 v = make_uint4(0, 0, 0, 0);
+          if (dn + 8 * r < rows && 32 * b + 8 * quad < a.dim)
+            v = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q.data) + token * a.q.row +
+                                                ((long long)h * a.group + g0 + dn + 8 * r) * a.q.head + 32 * b + 8 * quad);
+          q[b][r][0] = v.x; q[b][r][1] = v.y; q[b][r][2] = v.z; q[b][r][3] = v.w;
+        }
+      float o[NT][4];
+#pragma unroll
+      for (int t = 0; t < NT; ++t) o[t][0] = o[t][1] = o[t][2] = o[t][3] = 0.0f;
+      float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.0f, 0.0f};
+      const T* const keys = static_cast<const T*>(a.ko.data) + first * a.ko.row + h * a.ko.head;
+      const T* const values = static_cast<const T*>(a.vo.data) + first * a.vo.row + h * a.vo.head;
+      for (int k0 = 16 * wi; k0 < count; k0 += 16 * WPU) {
+        float s[2][4];
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          s[half][0] = s[half][1] = s[half][2] = s[half][3] = 0.0f;
+          const int key = k0 + 8 * half + dn;
+          uint4 w[DP / 32];
+#pragma unroll
+          for (int b = 0; b < DP / 32; ++b) {
+            w[b] = make_uint4(0, 0, 0, 0);
+            if (key < count && 32 * b + 8 * quad < a.dim)
+              w[b] = *reinterpret_cast<const uint4*>(keys + key * a.ko.row + 32 * b + 8 * quad);
+          }
+#pragma unroll
+          for (int b = 0; b < DP / 32; ++b) {
+            const uint32_t a0[4] = {q[b][0][0], q[b][1][0], q[b][0][1], q[b][1][1]};
+            const uint32_t a1[4] = {q[b][0][2], q[b][1][2], q[b][0][3], q[b][1][3]};
+            mma_16816<T>(s[half], a0, w[b].x, w[b].y);
+            mma_16816<T>(s[half], a1, w[b].z, w[b].w);
+          }
+        }
+        // values of keys 2 quad, 2 quad + 1, + 8, + 9 (on their way during the softmax)
+        uint32_t v[4][NT / 2];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int key = k0 + 2 * quad + (i & 1) + 8 * (i >> 1);
+#pragma unroll
+          for (int x = 0; x < NT / 8; ++x) {
+            uint4 w = make_uint4(0, 0, 0, 0);
+            if (key < count && dn * NT + 8 * x < a.dim)
+              w = *reinterpret_cast<const uint4*>(values + key * a.vo.row + dn * NT + 8 * x);
+            v[i][4 * x] = w.x; v[i][4 * x + 1] = w.y; v[i][4 * x + 2] = w.z; v[i][4 * x + 3] = w.w;
+          }
+        }
+        float pr[2][4];  // [row][key 2 quad, + 1, + 8, + 9]
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          float now = top[r];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const bool there = k0 + 2 * quad + (i & 1) + 8 * (i >> 1) < count;
+            pr[r][i] = there ? s[i >> 1][2 * r + (i & 1)] * p.scale2 : -INFINITY;
+            now = fmaxf(now, pr[r][i]);
+          }
+          now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, 1));
+          now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, 2));
+          const float keep = top[r] == -INFINITY ? 0.0f : exp2_approx(top[r] - now);
+          top[r] = now;
+          sum[r] *= keep;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const bool there = k0 + 2 * quad + (i & 1) + 8 * (i >> 1) < count;
+            pr[r][i] = there ? exp2_approx(pr[r][i] - now) : 0.0f;
+            sum[r] += pr[r][i];
+          }
+#pragma unroll
+          for (int t = 0; t < NT; ++t) {
+            o[t][2 * r] *= keep;
+            o[t][2 * r + 1] *= keep;
+          }
+        }
+        const uint32_t pa[4] = {pack2<T>(pr[0][0], pr[0][1]), pack2<T>(pr[1][0], pr[1][1]), pack2<T>(pr[0][2], pr[0][3]),
+                                pack2<T>(pr[1][2], pr[1][3])};
+#pragma unroll
+        for (int x = 0; x < NT / 2; ++x) {
+          mma_16816<T>(o[2 * x], pa, __byte_perm(v[0][x], v[1][x], 0x5410), __byte_perm(v[2][x], v[3][x], 0x5410));
+          mma_16816<T>(o[2 * x + 1], pa, __byte_perm(v[0][x], v[1][x], 0x7632), __byte_perm(v[2][x], v[3][x], 0x7632));
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 1);
+        sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 2);
+        if (dn + 8 * r < rows) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+#pragma unroll
+            for (int t = 0; t < NT; t += 4)
+              *reinterpret_cast<float4*>(mine + (dn + 8 * r) * LD + (2 * quad + e) * NT + t) =
+                  make_float4(o[t][2 * r + e], o[t + 1][2 * r + e], o[t + 2][2 * r + e], o[t + 3][2 * r + e]);
+          if (quad == 0) {
+            mine[16 * LD + 2 * (dn + 8 * r)] = top[r];
+            mine[16 * LD + 2 * (dn + 8 * r) + 1] = sum[r];
+          }
+        }
+      }
+    }
+    if (WPU == 1) __syncwarp();
+    else __syncthreads();
+
+    // Where the token's rows lie in the parts of the prefix.
+    int part0 = 0, parts = 0, chain_rows = 0, row0 = 0, item = 0;
+    bool whole = true;
+    if (p.plan.kv_tiles > 0) {
+      const long long tile = token / (2 * p.plan.tile_tokens);
+      const int within = (int)(token - tile * 2 * p.plan.tile_tokens);
+      const bool dual = a.tokens - tile * 2 * p.plan.tile_tokens > p.plan.tile_tokens;
+      item = h * p.plan.row_items + (int)tile;
+      const int from = item * p.plan.kv_tiles;
+      part0 = from / p.plan.per_cta;
+      parts = (from + p.plan.kv_tiles - 1) / p.plan.per_cta - part0 + 1;
+      whole = parts == 1;
+      const int chain = dual ? within / p.plan.tile_tokens : 0;
+      row0 = chain * kTileRows + (within - chain * p.plan.tile_tokens) * a.group + g0;
+      chain_rows = dual ? 0 : kTileRows;  // a part of the second chain behind the first one's
+    }
+    const int chains = chain_rows ? 2 : 1, all = parts * chains;
+    auto part_row = [&](int i) -> long long {
+      const int k = chains == 2 ? i >> 1 : i, cta = part0 + k;
+      const int slot = whole ? 2 * kMaxCtas + item : 2 * cta + (cta * p.plan.per_cta < item * p.plan.kv_tiles ? 1 : 0);
+      return (long long)slot * kPartRows + row0 + (chains == 2 && (i & 1) ? chain_rows : 0);
+    };
+    for (int e = wi * 32 + lane; e < rows * (DP / 4); e += WPU * 32) {
+      const int r = e / (DP / 4), d = e % (DP / 4) * 4;
+      float top = -INFINITY;
+      if (count > 0)
+#pragma unroll
+        for (int w = 0; w < WPU; ++w)
+          if (16 * w < count) top = fmaxf(top, unit0[w * (16 * LD + 32) + 16 * LD + 2 * r]);
+      for (int i = 0; i < all; ++i) {
+        const float2 st = p.stats[part_row(i) + r];
+        if (st.y != 0.0f) top = fmaxf(top, st.x);
+      }
+      float sum = 0.0f;
+      float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      if (count > 0)
+#pragma unroll
+        for (int w = 0; w < WPU; ++w)
+          if (16 * w < count) {
+            const float* from = unit0 + w * (16 * LD + 32);
+            const float weight = exp2_approx(from[16 * LD + 2 * r] - top);
+            const float4 v = *reinterpret_cast<const float4*>(from + r * LD + d);
+            sum += weight * from[16 * LD + 2 * r + 1];
+            acc.x += weight * v.x; acc.y += weight * v.y; acc.z += weight * v.z; acc.w += weight * v.w;
+          }
+      for (int i = 0; i < all; ++i) {
+        const long long at = part_row(i) + r;
+        const float2 st = p.stats[at];
+        if (st.y == 0.0f) continue;  // a chain that had no key tile: nothing was left there
+        const float weight = exp2_approx(st.x - top);
+        const float4 v = *reinterpret_cast<const float4*>(p.parts + at * DP + d);
+        sum += weight * st.y;
+        acc.x += weight * v.x; acc.y += weight * v.y; acc.z += weight * v.z; acc.w += weight * v.w;
+      }
+      const bool none = count == 0 && all == 0;
+      const float inv = none ? 0.0f : 1.0f / sum;
+      const long long head = (long long)h * a.group + g0 + r;
+      if (d < a.dim) {
+        uint2 w;
+        w.x = pack2<T>(acc.x * inv, acc.y * inv);
+        w.y = pack2<T>(acc.z * inv, acc.w * inv);
+        *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + token * a.out_row + head * a.out_head + d) = w;
+      }
+      if (d == 0 && a.lse) a.lse[token * a.heads + head] = none ? -INFINITY : (top + log2f(sum)) * kLn2;
+    }
+    if (WPU == 1) __syncwarp();
+    else __syncthreads();
+  }
+}
+
+// ---------------------------------------------------------------- host
+
+int heads_map(CUtensorMap* map, bool bf16, const void* ptr, int rank, const long long* dims, const long long* strides_elements,
+              const int* box) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return fail(ANNC_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
+  cuuint64_t d[4], st[3];
+  cuuint32_t b[4], one[4] = {1, 1, 1, 1};
+  for (int i = 0; i < rank; ++i) {
+    d[i] = (cuuint64_t)dims[i];
+    b[i] = (cuuint32_t)box[i];
+    // (the stride of a dimension of one does not matter, but has to be a multiple of 16 bytes)
+    if (i > 0) st[i - 1] = dims[i] == 1 ? 16 : (cuuint64_t)strides_elements[i - 1] * 2;
+  }
+  const CUresult r = fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, (cuuint32_t)rank,
+                        const_cast<void*>(ptr), d, st, b, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(ANNC_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
+  return ANNC_OK;
+}
+
+// 16-byte pieces of every row; TMA wants positive strides below 2^40 bytes.
+bool rows_ok(const Rows& r, long long rows, long long heads, bool tma) {
+  if (reinterpret_cast<uintptr_t>(r.data) & 15) return false;
+  auto stride_ok = [&](long long s, long long n) {
+    return n <= 1 || (s % 8 == 0 && (!tma || (s > 0 && s < (1LL << 39))));
+  };
+  return stride_ok(r.row, rows) && stride_ok(r.head, heads);
+}
+
+template <typename T, int DP>
+int launch_prefix(const Params& a, const PrefixParams& p, cudaStream_t s) {
+  void (*const kernel)(CUtensorMap, CUtensorMap, CUtensorMap, PrefixParams) = prefix_kernel<T, DP>;
+  static bool attr_done[kMaxDevices] = {};
+  const int dev = device_slot();
+  if (!attr_done[dev]) {
+    ANNC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Shape<DP>::kSmem));
+    attr_done[dev] = true;
+  }
+  const bool bf16 = std::is_same<T, __nv_bfloat16>::value;
+  CUtensorMap tq, tk, tv;
+  {
+    const long long dims[4] = {a.dim, a.group, a.kv_heads, a.tokens}, strides[3] = {a.q.head, a.q.head * a.group, a.q.row};
+    const int box[4] = {64, a.group, 1, p.plan.tile_tokens};
+    ANNC_TRY(heads_map(&tq, bf16, a.q.data, 4, dims, strides, box));
+  }
+  for (int v = 0; v < 2; ++v) {
+    const Rows& r = v ? a.vp : a.kp;
+    const long long dims[3] = {a.dim, a.kv_heads, a.prefix}, strides[2] = {r.head, r.row};
+    const int box[3] = {64, 1, kTileKeys};
+    ANNC_TRY(heads_map(v ? &tv : &tk, bf16, r.data, 3, dims, strides, box));
+  }
+  ANNC_CUDA(launch_pdl(kernel, dim3((unsigned)p.plan.ctas), dim3(kThreads), Shape<DP>::kSmem, s, tq, tk, tv, p));
+  return ANNC_OK;
+}
+
+template <typename T, int DP, int WPU>
+int launch_join(const JoinParams& p, cudaStream_t s) {
+  const long long blocks = (p.a.tokens * p.a.kv_heads + 4 / WPU - 1) / (4 / WPU);
+  ANNC_REQUIRE(blocks <= 0x7fffffffLL, ANNC_ERR_UNSUPPORTED, "prefix attention: too many tokens");
+  const size_t smem = 4 * (16 * (DP + 4) + 32) * sizeof(float);
+  ANNC_CUDA(launch_pdl(join_kernel<T, DP, WPU>, dim3((unsigned)blocks), dim3(128), smem, s, p));
+  return ANNC_OK;
+}
+
+template <typename T, int DP>
+int run_as(const Params& a, void* workspace, cudaStream_t s) {
+  PrefixParams p = {};
+  p.plan = plan_of(a.tokens, a.kv_heads, a.group, a.prefix);
+  p.tokens = a.tokens;
+  p.kv_heads = a.kv_heads;
+  p.group = a.group;
+  p.prefix = (int)a.prefix;
+  p.scale2 = a.scale * kLog2e;
+  const size_t slots = 2 * kMaxCtas + (size_t)p.plan.items;
+  p.parts = static_cast<float*>(workspace);
+  p.stats = reinterpret_cast<float2*>(p.parts + slots * kPartRows * DP);
+  p.error_word = gemm::gemm_error_word();
+  if (!p.error_word) return fail(ANNC_ERR_CUDA, "the tensor-core error word is not addressable");
+  if (a.prefix > 0) ANNC_TRY((launch_prefix<T, DP>(a, p, s)));
+  const JoinParams j{a, p.plan, p.scale2, p.parts, p.stats};
+  // a unit of work fills a warp; with few units (latency) four warps share one
+  return a.tokens * a.kv_heads >= 1184 ? launch_join<T, DP, 1>(j, s) : launch_join<T, DP, 4>(j, s);
+}
+
+}  // namespace
+
+size_t tc_workspace_bytes(long long tokens, int heads, int kv_heads, int dim) {
+  const int group = heads / kv_heads;
+  if (group > kTileRows || dim > 128) return 0;
+  const long long per_item = 2LL * (kTileRows / group);
+  const unsigned long long slots = 2ULL * kMaxCtas + (unsigned long long)((tokens + per_item - 1) / per_item) * kv_heads;
+  return (size_t)(slots * kPartRows * ((unsigned long long)part_width(dim) * 4 + 8));
+}
+
+bool tc_supported(const Params& p, int) {
+  if (p.dim % 8 || p.dim > 128 || p.group > kTileRows) return false;
+  if (p.prefix > 0 && !(p.scale >= 0.0f)) return false;  // (the prefix kernel takes the maximum of the unscaled scores)
+  const Plan plan = plan_of(p.tokens, p.kv_heads, p.group, p.prefix);
+  if ((long long)plan.row_items * p.kv_heads * (plan.kv_tiles > 0 ? plan.kv_tiles : 1) >= (1LL << 30)) return false;
+  if (!rows_ok(p.q, p.tokens, p.heads, true) || p.q.head * p.group >= (1LL << 39)) return false;
+  if (p.prefix > 0 && (!rows_ok(p.kp, p.prefix, p.kv_heads, true) || !rows_ok(p.vp, p.prefix, p.kv_heads, true))) return false;
+  if (p.own_len && (!rows_ok(p.ko, p.own_rows, p.kv_heads, false) || !rows_ok(p.vo, p.own_rows, p.kv_heads, false))) return false;
+  return (reinterpret_cast<uintptr_t>(p.out) & 7) == 0 && p.out_row % 4 == 0 && p.out_head % 4 == 0;
+}
+
+int run_tc(const Params& p, int dtype, void* workspace, cudaStream_t s) {
+  if (dtype == ANNC_BF16)
+    return p.dim <= 64 ? run_as<__nv_bfloat16, 64>(p, workspace, s) : run_as<__nv_bfloat16, 128>(p, workspace, s);
+  return p.dim <= 64 ? run_as<__half, 64>(p, workspace, s) : run_as<__half, 128>(p, workspace, s);
+}
+
+}  // namespace attention
+}  // namespace annc

@@ -507,7 +507,8 @@ class PrefixAttention:
             _refuse(f"prefix attention: bad type {dtype}")
         self.heads, self.kv_heads, self.head_dim = int(heads), int(kv_heads), int(head_dim)
         self.max_tokens, self.dtype = int(max_tokens), dtype
-        self.ws_bytes = int(lib.annc_prefix_attention_workspace_bytes(self.max_tokens, self.heads, self.head_dim))
+        self.ws_bytes = int(lib.annc_prefix_attention_workspace_bytes(self.max_tokens, self.heads, self.kv_heads,
+                                                                      self.head_dim))
         self.ws = torch.empty(max(self.ws_bytes, 16), dtype=torch.uint8, device=device or "cuda")
 
     def run(self, q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: torch.Tensor, out: torch.Tensor, *,

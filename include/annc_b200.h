@@ -706,8 +706,8 @@ int annc_rotary_dev(const annc_rotary_desc* desc, void* stream);
  * and lse -inf; lse is the natural logarithm of the sum of exp(scale * q . k).  own_begin /
  * own_len entries that reach outside 0 .. own_rows are clamped to it.
  * The prefix is read once for all tokens.  workspace: 16-byte aligned scratch of
- * annc_prefix_attention_workspace_bytes(tokens, heads, head_dim) bytes (for at most so many tokens),
- * one call at a time. */
+ * annc_prefix_attention_workspace_bytes(tokens, heads, kv_heads, head_dim) bytes (for at most so
+ * many tokens), one call at a time. */
 typedef struct annc_prefix_attention_desc {
   int32_t dtype;                 /* ANNC_BF16 or ANNC_F16: q, keys, values, out */
   int32_t heads, kv_heads, head_dim; /* head_dim 1 .. 256 */
@@ -734,7 +734,8 @@ typedef struct annc_prefix_attention_desc {
   size_t workspace_bytes;
 } annc_prefix_attention_desc;
 
-size_t annc_prefix_attention_workspace_bytes(int64_t tokens, int32_t heads, int32_t head_dim);
+size_t annc_prefix_attention_workspace_bytes(int64_t tokens, int32_t heads, int32_t kv_heads,
+                                             int32_t head_dim);
 int annc_prefix_attention_dev(const annc_prefix_attention_desc* desc, void* stream);
 
 /* ---------------------------------------------------------------- reference symbols

@@ -161,7 +161,8 @@ def attention_desc(**kw):
     (dict(scale=float("nan")), "scale"), (dict(scale=float("inf")), "scale"), (dict(q=None), "null"), (dict(out=None), "null"),
     (dict(k_prefix=None), "null"), (dict(v_prefix=None), "null"), (dict(k_own=None), "own"), (dict(own_begin=None), "own"),
     (dict(q=P + 1), "aligned"), (dict(v_own=P + 1), "aligned"), (dict(lse=P + 2), "aligned"), (dict(own_begin=P + 4), "aligned"),
-    (dict(q_begin=P + 2), "aligned"),
+    (dict(q_begin=P + 2), "aligned"), (dict(workspace=None), "workspace"), (dict(workspace=P + 8), "workspace"),
+    (dict(workspace_bytes=1000), "workspace"),
 ])
 def test_prefix_attention_refuses(kw, text):
     assert lib.annc_prefix_attention_dev(C.byref(attention_desc(**kw)), None) == INVALID
@@ -171,3 +172,12 @@ def test_prefix_attention_refuses(kw, text):
 def test_prefix_attention_no_tokens():
     assert lib.annc_prefix_attention_dev(None, None) == INVALID
     assert lib.annc_prefix_attention_dev(C.byref(attention_desc(tokens=0, sequences=0, q=None, out=None)), None) == 0
+
+
+def test_prefix_attention_workspace():
+    ws = lib.annc_prefix_attention_workspace_bytes
+    assert ws(0, 8, 2, 64) == 0 and ws(4, 7, 2, 64) == 0 and ws(4, 8, 0, 64) == 0
+    assert ws(4, 8, 2, 256) == 0  # taken row by row, without parts
+    for heads, kv, dim in ((8, 2, 64), (8, 8, 128), (96, 1, 40)):
+        sizes = [ws(t, heads, kv, dim) for t in (1, 2, 7, 100, 1000, 100000)]
+        assert sizes == sorted(sizes) and sizes[0] > 0  # what serves many tokens serves few
