@@ -42,7 +42,7 @@ namespace {
 
 using namespace annc::tc;
 
-constexpr int kThreads = 320;
+constexpr int kThreads = 384;  // eight softmax warps, loads, products, and two that complete the group of four
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kSlack = 8.0f;  // log2 of what a numerator may grow to before the maximum moves
 
@@ -85,21 +85,29 @@ __device__ __forceinline__ void umma_f16_ts(uint32_t d, uint32_t a, uint64_t b, 
       "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
       : "memory");
 }
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
-      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
       "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
-      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]),
-      "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]),
-      "r"(r[31])
+      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
       : "memory");
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
+// Registers of the calling group of four warps: a softmax thread holds the 128 scores of its row.  Launched with 168 each,
+// and 2 x 128 x 208 + 128 x 88 is what 384 x 168 makes.
+__device__ __forceinline__ void registers_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 208;"); }
+__device__ __forceinline__ void registers_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 88;"); }
 __device__ __forceinline__ float exp2_approx(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -146,6 +154,84 @@ __device__ __forceinline__ Segment segment_at(const PrefixParams& p, int at, int
   return s;
 }
 
+// A row's 128 scores of one key tile (in tensor memory, a lane each) -> numerators in the operands' type in their
+// place; the row's maximum `top` (log2 units: scale * score) and sum follow, and O where the maximum moves.  `half_ready` is
+// signalled when the first 64 keys' numerators are written.  TAIL: only the first `valid` keys are there.
+template <bool TAIL>
+__device__ __forceinline__ float max32(const uint32_t (&r)[32], int first, int valid, float top) {
+  float m[4] = {top, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+  for (int j = 0; j < 32; j += 8)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float x = TAIL && first + j + i >= valid ? -INFINITY : __uint_as_float(r[j + i]);
+      const float y = TAIL && first + j + 4 + i >= valid ? -INFINITY : __uint_as_float(r[j + 4 + i]);
+      m[i] = fmaxf(fmaxf(m[i], x), y);
+    }
+  return fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+}
+template <typename T, bool TAIL>
+__device__ __forceinline__ void exp32(const uint32_t (&r)[32], int first, int valid, float scale, float top, float (&sum)[4],
+                                      uint32_t (&w)[16]) {
+#pragma unroll
+  for (int j = 0; j < 32; j += 2) {
+    float lo = exp2_approx(fmaf(__uint_as_float(r[j]), scale, -top));
+    float hi = exp2_approx(fmaf(__uint_as_float(r[j + 1]), scale, -top));
+    if (TAIL) {
+      if (first + j >= valid) lo = 0.0f;
+      if (first + j + 1 >= valid) hi = 0.0f;
+    }
+    sum[j & 2] += lo;
+    sum[(j & 2) + 1] += hi;
+    w[j / 2] = pack2<T>(lo, hi);
+  }
+}
+template <typename T, int DP, bool TAIL>
+__device__ __forceinline__ void softmax_tile(uint32_t t_s, uint32_t t_o, float scale, bool first, int valid, float& top, float& sum,
+                                             uint32_t half_ready) {
+  uint32_t r0[32], r1[32], r2[32], r3[32];
+  tmem_ld32(t_s, r0);
+  tmem_ld32(t_s + 32, r1);
+  tmem_ld32(t_s + 64, r2);
+  tmem_ld32(t_s + 96, r3);
+  tmem_ld_wait();
+  const float now = fmaxf(fmaxf(max32<TAIL>(r0, 0, valid, -INFINITY), max32<TAIL>(r1, 32, valid, -INFINITY)),
+                          fmaxf(max32<TAIL>(r2, 64, valid, -INFINITY), max32<TAIL>(r3, 96, valid, -INFINITY))) * scale;
+  if (first) {
+    top = now;
+  } else if (__any_sync(0xffffffffu, now > top + kSlack)) {
+    // (every product before this S is complete, O among them)
+    const float keep = now > top + kSlack ? exp2_approx(top - now) : 1.0f;
+    if (now > top + kSlack) top = now;
+    sum *= keep;
+#pragma unroll 1
+    for (int b = 0; b < DP / 16; ++b) {
+      uint32_t o[16];
+      tmem_ld16(t_o + 16 * b, o);
+      tmem_ld_wait();
+#pragma unroll
+      for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * keep);
+      tmem_st16(t_o + 16 * b, o);
+    }
+  }
+  float sum4[4] = {sum, 0.0f, 0.0f, 0.0f};
+  uint32_t w[16];
+  exp32<T, TAIL>(r0, 0, valid, scale, top, sum4, w);
+  tmem_st16(t_s, w);
+  exp32<T, TAIL>(r1, 32, valid, scale, top, sum4, w);
+  tmem_st16(t_s + 16, w);
+  tmem_st_wait();
+  tc_fence_before();
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) mbar_arrive(half_ready);
+  exp32<T, TAIL>(r2, 64, valid, scale, top, sum4, w);
+  tmem_st16(t_s + 32, w);
+  exp32<T, TAIL>(r3, 96, valid, scale, top, sum4, w);
+  tmem_st16(t_s + 48, w);
+  sum = (sum4[0] + sum4[1]) + (sum4[2] + sum4[3]);
+  tmem_st_wait();
+}
+
 template <typename T, int DP>
 __global__ void __launch_bounds__(kThreads, 1)
 prefix_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
@@ -158,8 +244,8 @@ prefix_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
   const uint32_t q_smem = base, ring = base + 2 * S::kTile, bars = base + S::kBars;
   const uint32_t bar_full = bars, bar_empty = bars + 8 * S::kSlots;
   const uint32_t bar_q = bars + 16 * S::kSlots, bar_qfree = bar_q + 8;
-  const uint32_t bar_s = bar_q + 16, bar_p = bar_q + 32, bar_o = bar_q + 48, bar_ofree = bar_q + 64;  // per chain
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem_raw + (bar_q + 80 - raw));
+  const uint32_t bar_s = bar_q + 16, bar_p = bar_q + 32, bar_o = bar_q + 48, bar_ofree = bar_q + 64, bar_h = bar_q + 80;  // per chain
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem_raw + (bar_q + 96 - raw));
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -175,6 +261,7 @@ prefix_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
     mbar_init(bar_qfree, 1);
     for (int c = 0; c < 2; ++c) {
       mbar_init(bar_s + 8 * c, 1);
+      mbar_init(bar_h + 8 * c, 4);  // the first 64 numerators of every row, all of them
       mbar_init(bar_p + 8 * c, 4);
       mbar_init(bar_o + 8 * c, 1);
       mbar_init(bar_ofree + 8 * c, 4);
@@ -197,6 +284,8 @@ prefix_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
   const bool poisoned = *reinterpret_cast<volatile int*>(p.error_word) != 0;  // an earlier launch gave up
   bool ok = !poisoned;
 
+  if (warp >= 8) {
+  registers_down();
   if (warp == 8) {
     if (ok && lane == 0) {
       uint32_t n = 0, segments = 0;
@@ -255,15 +344,20 @@ prefix_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
             const uint32_t t_s = tmem + 128 * c, t_o = tmem + 256 + 128 * c;
             if (step > 0 && step <= steps) {  // O += P V of the step before
               const uint32_t i = n0 + 2 * (uint32_t)(g.key_tile(c, step - 1) - g.first) + 1, s = i % S::kSlots;
-              ok = mbar_wait(bar_p + 8 * c, (steps_done[c] + step - 1) & 1u, abort_flag, p.error_word);
+              const uint32_t phase = (steps_done[c] + step - 1) & 1u;
+              ok = mbar_wait(bar_full + 8 * s, (i / S::kSlots) & 1u, abort_flag, p.error_word);
               if (ok && step == 1) ok = mbar_wait(bar_ofree + 8 * c, (segments & 1u) ^ 1u, abort_flag, p.error_word);
-              if (ok) ok = mbar_wait(bar_full + 8 * s, (i / S::kSlots) & 1u, abort_flag, p.error_word);
-              if (!ok) break;
-              tc_fence_after();
               const uint32_t v = ring + s * S::kTile;
 #pragma unroll
-              for (int kk = 0; kk < kTileKeys / 16; ++kk)
-                umma_f16_ts(t_o, t_s + 8 * kk, smem_desc(v + kk * 2048, kBlock, 1024, 2), idesc_o, step > 1 || kk > 0 ? 1u : 0u);
+              for (int half = 0; half < 2; ++half) {
+                if (ok) ok = mbar_wait((half ? bar_p : bar_h) + 8 * c, phase, abort_flag, p.error_word);
+                if (!ok) break;
+                tc_fence_after();
+#pragma unroll
+                for (int kk = 4 * half; kk < 4 * half + 4; ++kk)
+                  umma_f16_ts(t_o, t_s + 8 * kk, smem_desc(v + kk * 2048, kBlock, 1024, 2), idesc_o, step > 1 || kk > 0 ? 1u : 0u);
+              }
+              if (!ok) break;
               if (!g.dual || c == 1) umma_commit(bar_empty + 8 * s);
               if (step == steps) umma_commit(bar_o + 8 * c);
             }
@@ -289,7 +383,10 @@ prefix_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
         n0 += 2 * g.count;
       }
     }
-  } else if (ok) {
+  }
+  } else {
+  registers_up();
+  if (ok) {
     const int c = warp >> 2, q = warp & 3;
     const int row = q * 32 + lane;  // of the tile
     const uint32_t lanes = (uint32_t)(q * 32) << 16;
@@ -310,59 +407,13 @@ prefix_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
         if (!ok) break;
         if (any) {
           tc_fence_after();
-          float s[128];
-#pragma unroll
-          for (int b = 0; b < 4; ++b) tmem_ld32(t_s + 32 * b, *reinterpret_cast<uint32_t(*)[32]>(&s[32 * b]));
-          tmem_ld_wait();
           const int valid = p.prefix - g.key_tile(c, step) * kTileKeys;
-          if (valid < kTileKeys) {
-#pragma unroll
-            for (int j = 0; j < 128; ++j)
-              if (j >= valid) s[j] = -INFINITY;
-          }
-          float m4[4] = {s[0], s[1], s[2], s[3]};
-#pragma unroll
-          for (int j = 4; j < 128; ++j) m4[j & 3] = fmaxf(m4[j & 3], s[j]);
-          const float now = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * scale;
-          const bool moves = now > top + kSlack || step == 0;
-          if (step == 0) {
-            top = now;
-          } else if (__any_sync(0xffffffffu, moves)) {
-            // (every product before this S is complete, O among them)
-            const float keep = moves ? exp2_approx(top - now) : 1.0f;
-            if (moves) top = now;
-            sum *= keep;
-#pragma unroll
-            for (int b = 0; b < DP / 32; ++b) {
-              uint32_t o[32];
-              tmem_ld32(t_o + 32 * b, o);
-              tmem_ld_wait();
-#pragma unroll
-              for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * keep);
-              tmem_st32(t_o + 32 * b, o);
-            }
-          }
-          float sum4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-          for (int b = 0; b < 2; ++b) {
-            uint32_t w[32];
-#pragma unroll
-            for (int j = 0; j < 32; ++j) {
-              const int e = 64 * b + 2 * j;
-              float lo = exp2_approx(fmaf(s[e], scale, -top)), hi = exp2_approx(fmaf(s[e + 1], scale, -top));
-              if (valid < kTileKeys) {  // (0 * -inf is no zero where the scale is)
-                if (e >= valid) lo = 0.0f;
-                if (e + 1 >= valid) hi = 0.0f;
-              }
-              sum4[2 * (j & 1)] += lo;
-              sum4[2 * (j & 1) + 1] += hi;
-              w[j] = pack2<T>(lo, hi);
-            }
-            tmem_st32(t_s + 32 * b, w);
-          }
-          sum += (sum4[0] + sum4[1]) + (sum4[2] + sum4[3]);
-          tmem_st_wait();
+          // (two copies of the code: selects for every value of every tile would be a third of its instructions)
+          if (valid >= kTileKeys) softmax_tile<T, DP, false>(t_s, t_o, scale, step == 0, valid, top, sum, bar_h + 8 * c);
+          else softmax_tile<T, DP, true>(t_s, t_o, scale, step == 0, valid, top, sum, bar_h + 8 * c);
           tc_fence_before();
+        } else if (lane == 0) {
+          mbar_arrive(bar_h + 8 * c);
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(bar_p + 8 * c);
@@ -394,6 +445,7 @@ prefix_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
       __syncwarp();
       if (lane == 0) mbar_arrive(bar_ofree + 8 * c);
     }
+  }
   }
   __syncwarp();
   tc_fence_before();
