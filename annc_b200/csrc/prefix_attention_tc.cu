@@ -71,18 +71,30 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map
       "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar)
       : "memory");
 }
+// Products and their commits are issued by a whole warp, of which one lane is elected in the instruction itself: its
+// operands then stay in uniform registers.  (From a branch that one lane takes, every product cost some 140 cycles to
+// issue, where 128 x 128 x 16 takes 64: 2048 tokens of 16 heads against 8192 keys 165 us.)
 __device__ __forceinline__ void umma_f16_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
+      "{\n\t.reg .pred p, q;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      "elect.sync _|q, 0xffffffff;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
       : "memory");
 }
 __device__ __forceinline__ void umma_f16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
+      "{\n\t.reg .pred p, q;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      "elect.sync _|q, 0xffffffff;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void umma_commit_elected(uint32_t bar) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "elect.sync _|q, 0xffffffff;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar)
       : "memory");
 }
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
@@ -101,6 +113,26 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
       : "memory");
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// As mbar_wait, but the clock is only looked at now and then: most waits here are as short as reading it.
+__device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* error_word) {
+  unsigned long long t0 = 0;
+  for (uint32_t i = 1;; ++i) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if ((i & 255u) == 0) {
+      if (*abort_flag) return false;
+      const unsigned long long now = global_ns();
+      if (t0 == 0) t0 = now;
+      if (now - t0 > 1000000000ull) {
+        *abort_flag = 1;
+        atomicExch(error_word, 1);
+        return false;
+      }
+    }
+  }
+}
+__device__ __forceinline__ bool all_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* error_word) {
+  return __all_sync(0xffffffffu, wait(bar, parity, abort_flag, error_word)) != 0;
+}
 __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
@@ -112,6 +144,25 @@ __device__ __forceinline__ float exp2_approx(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, c, d;\n\t"
+      "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+      "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, d;\n\t"
+      "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+      "add.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
 }
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi);
@@ -171,19 +222,18 @@ __device__ __forceinline__ float max32(const uint32_t (&r)[32], int first, int v
   return fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
 }
 template <typename T, bool TAIL>
-__device__ __forceinline__ void exp32(const uint32_t (&r)[32], int first, int valid, float scale, float top, float (&sum)[4],
+__device__ __forceinline__ void exp32(const uint32_t (&r)[32], int first, int valid, float2 scale, float2 minus_top, float2 (&sum)[2],
                                       uint32_t (&w)[16]) {
 #pragma unroll
   for (int j = 0; j < 32; j += 2) {
-    float lo = exp2_approx(fmaf(__uint_as_float(r[j]), scale, -top));
-    float hi = exp2_approx(fmaf(__uint_as_float(r[j + 1]), scale, -top));
+    const float2 x = fma2(make_float2(__uint_as_float(r[j]), __uint_as_float(r[j + 1])), scale, minus_top);
+    float2 e = make_float2(exp2_approx(x.x), exp2_approx(x.y));
     if (TAIL) {
-      if (first + j >= valid) lo = 0.0f;
-      if (first + j + 1 >= valid) hi = 0.0f;
+      if (first + j >= valid) e.x = 0.0f;
+      if (first + j + 1 >= valid) e.y = 0.0f;
     }
-    sum[j & 2] += lo;
-    sum[(j & 2) + 1] += hi;
-    w[j / 2] = pack2<T>(lo, hi);
+    sum[j / 2 & 1] = add2(sum[j / 2 & 1], e);
+    w[j / 2] = pack2<T>(e.x, e.y);
   }
 }
 template <typename T, int DP, bool TAIL>
@@ -214,21 +264,23 @@ __device__ __forceinline__ void softmax_tile(uint32_t t_s, uint32_t t_o, float s
       tmem_st16(t_o + 16 * b, o);
     }
   }
-  float sum4[4] = {sum, 0.0f, 0.0f, 0.0f};
+  float2 sums[2] = {make_float2(sum, 0.0f), make_float2(0.0f, 0.0f)};
+  const float2 scale2 = make_float2(scale, scale), minus_top = make_float2(-top, -top);
   uint32_t w[16];
-  exp32<T, TAIL>(r0, 0, valid, scale, top, sum4, w);
+  exp32<T, TAIL>(r0, 0, valid, scale2, minus_top, sums, w);
   tmem_st16(t_s, w);
-  exp32<T, TAIL>(r1, 32, valid, scale, top, sum4, w);
+  exp32<T, TAIL>(r1, 32, valid, scale2, minus_top, sums, w);
   tmem_st16(t_s + 16, w);
   tmem_st_wait();
   tc_fence_before();
   __syncwarp();
   if ((threadIdx.x & 31) == 0) mbar_arrive(half_ready);
-  exp32<T, TAIL>(r2, 64, valid, scale, top, sum4, w);
+  exp32<T, TAIL>(r2, 64, valid, scale2, minus_top, sums, w);
   tmem_st16(t_s + 32, w);
-  exp32<T, TAIL>(r3, 96, valid, scale, top, sum4, w);
+  exp32<T, TAIL>(r3, 96, valid, scale2, minus_top, sums, w);
   tmem_st16(t_s + 48, w);
-  sum = (sum4[0] + sum4[1]) + (sum4[2] + sum4[3]);
+  sums[0] = add2(sums[0], sums[1]);
+  sum = sums[0].x + sums[0].y;
   tmem_st_wait();
 }
 
@@ -248,7 +300,7 @@ prefix_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem_raw + (bar_q + 96 - raw));
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;  // (known to be uniform)
   if (threadIdx.x == 0) {
     prefetch_tensormap(&tmap_q);
     prefetch_tensormap(&tmap_k);
@@ -292,7 +344,7 @@ prefix_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
       const uint32_t q_bytes = (uint32_t)(p.plan.tile_tokens * p.group) * 128u * (DP / 64);
       auto load = [&](const CUtensorMap* map, int head, int tile) {
         const int s = n % S::kSlots;
-        ok = mbar_wait(bar_empty + 8 * s, ((n / S::kSlots) & 1u) ^ 1u, abort_flag, p.error_word);
+        ok = wait(bar_empty + 8 * s, ((n / S::kSlots) & 1u) ^ 1u, abort_flag, p.error_word);
         if (!ok) return;
         mbar_expect_tx(bar_full + 8 * s, S::kTile);
 #pragma unroll
@@ -303,7 +355,7 @@ prefix_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
       for (int at = begin; at < end && ok; ++segments) {
         const Segment g = segment_at(p, at, begin, end);
         at += g.count;
-        ok = mbar_wait(bar_qfree, (segments & 1u) ^ 1u, abort_flag, p.error_word);
+        ok = wait(bar_qfree, (segments & 1u) ^ 1u, abort_flag, p.error_word);
         if (!ok) break;
         mbar_expect_tx(bar_q, g.dual ? 2 * q_bytes : q_bytes);
         for (int c = 0; c < (g.dual ? 2 : 1); ++c)
@@ -324,17 +376,20 @@ prefix_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
       }
     }
   } else if (warp == 9) {
-    if (ok && lane == 0) {
+    if (ok) {
       constexpr uint32_t fmt = sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
       constexpr uint32_t idesc_s = (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)(kTileKeys >> 3) << 17) | ((uint32_t)(kTileRows >> 4) << 24);
       constexpr uint32_t idesc_o =
           (1u << 4) | (fmt << 7) | (fmt << 10) | (1u << 16) | ((uint32_t)(DP >> 3) << 17) | ((uint32_t)(kTileRows >> 4) << 24);
+      // (an address further on is a descriptor further on: the address field counts 16 bytes and cannot overflow)
+      const uint64_t q_desc = smem_desc(q_smem, 16, 1024, 2), k_desc = smem_desc(ring, 16, 1024, 2),
+                     v_desc = smem_desc(ring, kBlock, 1024, 2);
       uint32_t n0 = 0, segments = 0;  // ring number of the segment's first key tile
       uint32_t steps_done[2] = {0, 0};
       for (int at = begin; at < end && ok; ++segments) {
         const Segment g = segment_at(p, at, begin, end);
         at += g.count;
-        ok = mbar_wait(bar_q, segments & 1u, abort_flag, p.error_word);
+        ok = all_wait(bar_q, segments & 1u, abort_flag, p.error_word);
         if (!ok) break;
         const int most = g.steps(0);
         for (int step = 0; step <= most && ok; ++step) {
@@ -345,38 +400,38 @@ prefix_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
             if (step > 0 && step <= steps) {  // O += P V of the step before
               const uint32_t i = n0 + 2 * (uint32_t)(g.key_tile(c, step - 1) - g.first) + 1, s = i % S::kSlots;
               const uint32_t phase = (steps_done[c] + step - 1) & 1u;
-              ok = mbar_wait(bar_full + 8 * s, (i / S::kSlots) & 1u, abort_flag, p.error_word);
-              if (ok && step == 1) ok = mbar_wait(bar_ofree + 8 * c, (segments & 1u) ^ 1u, abort_flag, p.error_word);
-              const uint32_t v = ring + s * S::kTile;
+              ok = all_wait(bar_full + 8 * s, (i / S::kSlots) & 1u, abort_flag, p.error_word);
+              if (ok && step == 1) ok = all_wait(bar_ofree + 8 * c, (segments & 1u) ^ 1u, abort_flag, p.error_word);
+              const uint64_t v = v_desc + s * (S::kTile >> 4);
 #pragma unroll
               for (int half = 0; half < 2; ++half) {
-                if (ok) ok = mbar_wait((half ? bar_p : bar_h) + 8 * c, phase, abort_flag, p.error_word);
+                if (ok) ok = all_wait((half ? bar_p : bar_h) + 8 * c, phase, abort_flag, p.error_word);
                 if (!ok) break;
                 tc_fence_after();
 #pragma unroll
                 for (int kk = 4 * half; kk < 4 * half + 4; ++kk)
-                  umma_f16_ts(t_o, t_s + 8 * kk, smem_desc(v + kk * 2048, kBlock, 1024, 2), idesc_o, step > 1 || kk > 0 ? 1u : 0u);
+                  umma_f16_ts(t_o, t_s + 8 * kk, v + (kk * 2048 >> 4), idesc_o, step > 1 || kk > 0 ? 1u : 0u);
               }
               if (!ok) break;
-              if (!g.dual || c == 1) umma_commit(bar_empty + 8 * s);
-              if (step == steps) umma_commit(bar_o + 8 * c);
+              if (!g.dual || c == 1) umma_commit_elected(bar_empty + 8 * s);
+              if (step == steps) umma_commit_elected(bar_o + 8 * c);
             }
             if (step < steps) {  // S = Q K^T
               const uint32_t i = n0 + 2 * (uint32_t)(g.key_tile(c, step) - g.first), s = i % S::kSlots;
-              ok = mbar_wait(bar_full + 8 * s, (i / S::kSlots) & 1u, abort_flag, p.error_word);
+              ok = all_wait(bar_full + 8 * s, (i / S::kSlots) & 1u, abort_flag, p.error_word);
               if (!ok) break;
               tc_fence_after();
-              const uint32_t k = ring + s * S::kTile, q = q_smem + (g.dual ? c : 0) * S::kTile;
+              const uint64_t k = k_desc + s * (S::kTile >> 4), q = q_desc + (g.dual ? c : 0) * (S::kTile >> 4);
 #pragma unroll
               for (int kk = 0; kk < DP / 16; ++kk) {
-                const uint32_t off = (kk / 4) * kBlock + (kk % 4) * 32;
-                umma_f16_ss(t_s, smem_desc(q + off, 16, 1024, 2), smem_desc(k + off, 16, 1024, 2), idesc_s, kk > 0 ? 1u : 0u);
+                const uint32_t off = ((kk / 4) * kBlock + (kk % 4) * 32) >> 4;
+                umma_f16_ss(t_s, q + off, k + off, idesc_s, kk > 0 ? 1u : 0u);
               }
-              if (!g.dual || c == 1) umma_commit(bar_empty + 8 * s);
-              umma_commit(bar_s + 8 * c);
+              if (!g.dual || c == 1) umma_commit_elected(bar_empty + 8 * s);
+              umma_commit_elected(bar_s + 8 * c);
             }
           }
-          if (step == most - 1 && ok) umma_commit(bar_qfree);  // the segment's last use of its rows
+          if (step == most - 1 && ok) umma_commit_elected(bar_qfree);  // the segment's last use of its rows
         }
         steps_done[0] += g.steps(0);
         steps_done[1] += g.steps(1);
@@ -403,7 +458,7 @@ prefix_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
       const bool any = q * 32 < rows;  // of this warp's
       float top = -INFINITY, sum = 0.0f;  // top in units of log2: scale * score
       for (int step = 0; step < steps; ++step, ++done) {
-        ok = __all_sync(0xffffffffu, mbar_wait(bar_s + 8 * c, done & 1u, abort_flag, p.error_word)) != 0;
+        ok = all_wait(bar_s + 8 * c, done & 1u, abort_flag, p.error_word);
         if (!ok) break;
         if (any) {
           tc_fence_after();
@@ -422,7 +477,7 @@ prefix_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
       // the part: rows of this chain at 128 c
       const long long at_row = (long long)g.part * kPartRows + c * kTileRows + row;
       if (steps > 0) {
-        ok = __all_sync(0xffffffffu, mbar_wait(bar_o + 8 * c, parts & 1u, abort_flag, p.error_word)) != 0;
+        ok = all_wait(bar_o + 8 * c, parts & 1u, abort_flag, p.error_word);
         if (!ok) break;
         ++parts;
       }
