@@ -42,18 +42,41 @@ using namespace annc::tc;
 
 constexpr int KB = 128;  // bytes (values) of k per stage
 
+// Products and their commits are issued by a whole warp, of which one lane is elected in the instruction itself: its
+// operands then stay in uniform registers.  (From a branch that one lane takes, a product costs some 140 cycles to issue.)
+__device__ __forceinline__ void commit_elected(uint32_t bar) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "elect.sync _|q, 0xffffffff;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ void commit_pair_elected(uint32_t bar) {
+  const uint16_t mask = 3;
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "elect.sync _|q, 0xffffffff;\n\t"
+      "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n\t}" ::"r"(bar),
+      "h"(mask)
+      : "memory");
+}
+__device__ __forceinline__ bool all_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* error_word) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, error_word)) != 0;
+}
 __device__ __forceinline__ void umma_i8(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
+      "{\n\t.reg .pred p, q;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      "elect.sync _|q, 0xffffffff;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
 __device__ __forceinline__ void umma_pair_i8(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
+      "{\n\t.reg .pred p, q;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      "elect.sync _|q, 0xffffffff;\n\t"
+      "@q tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
 __device__ __forceinline__ void tma_prefetch_2d(const CUtensorMap* map, int x, int y) {
@@ -145,7 +168,7 @@ gemm_i8_split_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gen_base + kBars + 16 * S::kStages + 8);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;  // (known to be uniform)
   const int channel_tiles = (p.n + kChannels - 1) / kChannels, tile = blockIdx.x / split;
   const int n0 = tile % channel_tiles * kChannels, m0 = tile / channel_tiles * TN;
   const int rank = split > 1 ? (int)cluster_ctarank() : 0;
@@ -194,21 +217,20 @@ gemm_i8_split_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
       }
     }
   } else if (ok && warp == 1) {
-    if (lane == 0) {
-      for (int kt = 0; kt < KT && ok; ++kt) {
-        const int s = kt % S::kStages;
-        ok = mbar_wait(bar_full + 8 * s, (kt / S::kStages) & 1u, abort_flag, error_word);
-        if (!ok) break;
-        tc_fence_after();
-        const uint32_t sw = base + s * S::kStage, st = sw + kChannels * KB;
+    // (an address further on is a descriptor further on: the address field counts 16 bytes and cannot overflow)
+    const uint64_t w_desc = smem_desc(base, 16, 1024, 2), t_desc = smem_desc(base + kChannels * KB, 16, 1024, 2);
+    for (int kt = 0; kt < KT; ++kt) {
+      const int s = kt % S::kStages;
+      ok = all_wait(bar_full + 8 * s, (kt / S::kStages) & 1u, abort_flag, error_word);
+      if (!ok) break;
+      tc_fence_after();
+      const uint32_t off = s * (S::kStage >> 4);
 #pragma unroll
-        for (int kk = 0; kk < 4; ++kk)
-          umma_i8(tmem_base, smem_desc(sw + kk * 32, 16, 1024, 2), smem_desc(st + kk * 32, 16, 1024, 2), i8_idesc(kChannels, TN),
-                  (kt | kk) != 0 ? 1u : 0u);
-        umma_commit(bar_empty + 8 * s);
-      }
-      if (ok) umma_commit(bar_done);
+      for (int kk = 0; kk < 4; ++kk)
+        umma_i8(tmem_base, w_desc + off + 2 * kk, t_desc + off + 2 * kk, i8_idesc(kChannels, TN), (kt | kk) != 0 ? 1u : 0u);
+      commit_elected(bar_empty + 8 * s);
     }
+    if (ok) commit_elected(bar_done);
   }
 
   __syncwarp();
@@ -346,7 +368,7 @@ gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gen_base + kBars + 16 * kPairStages + 32);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;  // (known to be uniform)
   const uint32_t rank = cluster_ctarank();
   const bool leader = rank == 0;
   const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
@@ -400,28 +422,28 @@ gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
         }
       }
     } else if (warp == 1) {
-      if (leader && lane == 0) {
+      if (leader) {
+        const uint64_t a_desc = smem_desc(base, 16, 1024, 2), b_desc = smem_desc(base + kPairStage / 2, 16, 1024, 2);
         uint32_t kit = 0, count = 0;
         bool ok = true;
         for (int tile = pair; tile < tiles.count && ok; tile += pairs, ++count) {
           const uint32_t acc = count & 1u;
-          ok = mbar_wait(bar_tempty + 8 * acc, ((count >> 1) & 1u) ^ 1u, abort_flag, error_word);
+          ok = all_wait(bar_tempty + 8 * acc, ((count >> 1) & 1u) ^ 1u, abort_flag, error_word);
           if (!ok) break;
           tc_fence_after();
           const uint32_t tmem_d = tmem_base + acc * (uint32_t)kPairTile;
           for (int kt = 0; kt < KT; ++kt, ++kit) {
             const int s = kit % kPairStages;
-            ok = mbar_wait(bar_full + 8 * s, (kit / kPairStages) & 1u, abort_flag, error_word);
+            ok = all_wait(bar_full + 8 * s, (kit / kPairStages) & 1u, abort_flag, error_word);
             if (!ok) break;
             tc_fence_after();
-            const uint32_t sa = base + s * kPairStage, sb = sa + kPairStage / 2;
+            const uint32_t off = s * (kPairStage >> 4);
 #pragma unroll
             for (int kk = 0; kk < 4; ++kk)
-              umma_pair_i8(tmem_d, smem_desc(sa + kk * 32, 16, 1024, 2), smem_desc(sb + kk * 32, 16, 1024, 2),
-                           i8_idesc(kPairTile, kPairTile), (kt | kk) != 0 ? 1u : 0u);
-            umma_commit_pair(bar_empty + 8 * s);
+              umma_pair_i8(tmem_d, a_desc + off + 2 * kk, b_desc + off + 2 * kk, i8_idesc(kPairTile, kPairTile), (kt | kk) != 0 ? 1u : 0u);
+            commit_pair_elected(bar_empty + 8 * s);
           }
-          if (ok) umma_commit_pair(bar_tfull + 8 * acc);
+          if (ok) commit_pair_elected(bar_tfull + 8 * acc);
         }
       }
     } else {
@@ -629,14 +651,15 @@ int launch_pair(const Params& p, int* error_word, cudaStream_t s) {
 }  // namespace
 
 // Which kernel and shape: the smallest of their times as these sums model them (us, bf16 output, figures fitted to
-// 40 products from 1 x 512 x 256 to 16384 x 8192 x 256; 148 SMs).
-//   split  2.7 for launch and prologue; per round of CTAs a k-step 0.21 + 0.00043 TN (latency: a CTA streams alone on
-//          its SM) and, unsplit, 0.0105 TN to write the tile; split, once 1.0 + 0.016 TN for the sums of the cluster
-//   pair   6.1 for launch, prologue and the last tile's epilogue; a k-step 0.33, a tile at least the 3.3 that the
+// 45 products from 1 x 512 x 256 to 16384 x 8192 x 256; 148 SMs).
+//   split  2.4 for launch and prologue; per round of CTAs a k-step 0.165 + 0.00014 TN (latency: a CTA streams alone on
+//          its SM; 0.286 for 256 tokens, 48 KB) and, unsplit, 0.0098 TN to write the tile; split, once 0.6 + 0.022 TN
+//          for the sums of the cluster
+//   pair   6.1 for launch, prologue and the last tile's epilogue; a k-step 0.31, a tile at least the 3.3 that the
 //          epilogue under it takes
-// Measured, split kernel's best / pair: 1024 x 1024 x 1024 5.5 / 7.9, 512 x 4096 x 2048 8.6 / 10.6, 1024 x 4096 x 2048 10.3 /
-// 11.6, 2048 x 1024 x 8192 19.6 / 24.7, 4096 x 1024 x 8192 25.0 / 26.1, 700 x 8192 x 4096 27.9 / 25.8, 2048 x 4096 x 2048
-// 20.1 / 17.3, 8192 x 4096 x 2048 80 / 53.
+// Measured, split kernel's best / pair: 1024 x 1024 x 1024 4.8 / 8.3, 512 x 4096 x 2048 7.2 / 10.8, 1024 x 4096 x 2048 10.2 /
+// 11.5, 2048 x 1024 x 8192 16.1 / 24.3, 4096 x 1024 x 8192 24.8 / 25.1, 700 x 8192 x 4096 28.1 / 25.6, 2048 x 4096 x 2048
+// 19.9 / 16.7, 8192 x 4096 x 2048 73 / 49.
 Route route_of(const Params& p) {
   Route best = {ROUTE_SIMT, 0, 0};
   // TMA wants rows on 16 bytes
@@ -644,7 +667,7 @@ Route route_of(const Params& p) {
   const int kt = (p.k + KB - 1) / KB;
   const long long pair_tiles = ((p.m + 255LL) / 256) * ((p.n + 255LL) / 256);
   if (pair_tiles > (1LL << 30)) return best;
-  const double main = 0.33 * kt;
+  const double main = 0.31 * kt;
   const long long pair_rounds = (pair_tiles + 73) / 74;
   double us = 6.1 + main + (double)(pair_rounds - 1) * (main > 3.3 ? main : 3.3);
   best.kind = ROUTE_PAIR;
@@ -655,9 +678,9 @@ Route route_of(const Params& p) {
     for (int split = 1; split <= 8 && split <= kt; split *= 2) {
       if (split > 1 && tiles > (split == 8 ? 15 : split == 4 ? 33 : 74)) break;
       const long long rounds = (tiles * split + 147) / 148;
-      const double step = 0.21 + 0.00043 * tn;
-      const double t = 2.7 + (double)rounds * ((kt + split - 1) / split * step + (split == 1 ? 0.0105 * tn : 0.0)) +
-                       (split > 1 ? 1.0 + 0.016 * tn : 0.0);
+      const double step = tn == 256 ? 0.286 : 0.165 + 0.00014 * tn;
+      const double t = 2.4 + (double)rounds * ((kt + split - 1) / split * step + (split == 1 ? 0.0098 * tn : 0.0)) +
+                       (split > 1 ? 0.6 + 0.022 * tn : 0.0);
       if (t < us) {
         us = t;
         best = {ROUTE_SPLIT, tn, split};

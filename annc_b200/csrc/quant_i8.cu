@@ -4,6 +4,7 @@
 #include <cuda_fp16.h>
 
 #include <cstdint>
+#include <cstring>
 
 #include "common.h"
 #include "gemm_i8.h"
@@ -19,17 +20,28 @@ namespace {
 // that nothing below divides by zero), and q the whole number nearest to x / scale, halves to even.  A row with an
 // infinity or a NaN has the step NaN and q = 0: its products are NaN, as they would be in floating point.
 
-// The nearest whole number exactly, also where the quotient of two fp32 numbers lies next to a half: the first
-// guess may be one off, but the remainder x - q * scale has no more bits than fp32 holds (both are multiples of
-// the smaller one's last place and the difference is below one step), so that comparing it decides.
-__device__ __forceinline__ int quantize_one(float x, float scale, float inv) {
-  float q = rintf(x * inv);
-  const float rem = __fmaf_rn(-q, scale, x), twice = 2.0f * fabsf(rem);
-  if (twice >= scale) {  // beyond half a step: to the neighbour; just half: to the even one
-    const float other = q + (rem > 0.0f ? 1.0f : -1.0f);
-    if (twice > scale || ((int)q & 1)) q = other;
-  }
-  return (int)q;
+// The nearest whole number exactly, also where the quotient of two fp32 numbers lies next to a half.  The guess comes
+// from adding 1.5 * 2^23 (the sum's last place is one, its low byte the number) and may be one off there; the
+// remainder x - q * scale has no more bits than fp32 holds (both are multiples of the smaller one's last place and the
+// difference is little more than half a step), so that comparing it decides.
+constexpr float kRound = 12582912.0f;
+struct Guess {
+  float sum, rem;
+};
+__device__ __forceinline__ Guess guess_of(float x, float scale, float inv) {
+  Guess g;
+  g.sum = __fmaf_rn(x, inv, kRound);
+  g.rem = __fmaf_rn(kRound - g.sum, scale, x);
+  return g;
+}
+// Below half a step either way the guess stands; beyond, or just half and odd, it is the neighbour.
+__device__ __forceinline__ float settled(Guess g, float half) {
+  const bool odd = __float_as_int(g.sum) & 1;
+  if (fabsf(g.rem) > half || (fabsf(g.rem) == half && odd)) return g.sum + (g.rem > 0.0f ? 1.0f : -1.0f);
+  return g.sum;
+}
+__device__ __forceinline__ int8_t quantize_one(float x, float scale, float inv) {
+  return (int8_t)__float_as_int(settled(guess_of(x, scale, inv), 0.5f * scale));
 }
 // Largest |x| as the bits of a non-negative float, which order as the floats do, infinities and NaN on top.
 __device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
@@ -49,6 +61,35 @@ __device__ __forceinline__ float to_float(float x) { return x; }
 __device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
 __device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
 
+// The same over a piece of values: of two-byte types two at a time, as they lie.
+template <typename T, int V>
+__device__ __forceinline__ void top_of(const T (&v)[V], uint32_t& top) {
+  if (sizeof(T) == 4 || V == 1) {
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      uint32_t w = 0;
+      memcpy(&w, &v[e], sizeof(T));
+      top = max(top, w & (sizeof(T) == 4 ? 0x7fffffffu : 0x7fffu));
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e + 1 < V; e += 2) {
+      uint32_t w;
+      memcpy(&w, &v[e], 4);
+      top = __vmaxu2(top, w & 0x7fff7fffu);
+    }
+  }
+}
+// ... to the bits of a float.
+template <typename T>
+__device__ __forceinline__ uint32_t top_bits(uint32_t top) {
+  if (sizeof(T) == 4) return top;
+  const uint16_t most = (uint16_t)max(top & 0xffffu, top >> 16);
+  T v;
+  memcpy(&v, &most, 2);
+  return __float_as_uint(to_float(v));
+}
+
 struct QuantParams {
   const void* x;
   long long ld;
@@ -61,7 +102,9 @@ struct QuantParams {
 
 // TPR threads take a row (a warp or a block of 256); a thread keeps NV pieces of V values in registers between
 // the maximum and the rounding, so a row of up to TPR * NV * V values is read once; what is longer is read
-// again, from L2.  VEC: rows of whole 16-byte pieces at 16-byte addresses; else one value at a time.
+// again, from L2.  VEC: rows of whole 16-byte pieces at 16-byte addresses; else one value at a time.  Bound by memory
+// once the rounding takes few enough instructions: 8192 x 2048 bf16 31 us with rintf, a conversion and a branch for
+// every value.
 template <typename T, int TPR, bool VEC>
 __global__ void __launch_bounds__(256) quantize_rows_kernel(QuantParams p) {
   constexpr int V = VEC ? 16 / (int)sizeof(T) : 1;
@@ -77,7 +120,7 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(QuantParams p) {
 
   alignas(16) T keep[NV][V];
   auto load = [&](int piece, T (&to)[V]) {
-    if (VEC) *reinterpret_cast<uint4*>(to) = __ldg(reinterpret_cast<const uint4*>(x) + piece);
+    if (VEC) *reinterpret_cast<uint4*>(to) = *(reinterpret_cast<const uint4*>(x) + piece);
     else to[0] = x[piece];
   };
   uint32_t top = 0;
@@ -86,17 +129,13 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(QuantParams p) {
     if (t + i * TPR < pieces) load(t + i * TPR, keep[i]);
 #pragma unroll
   for (int i = 0; i < NV; ++i)
-    if (t + i * TPR < pieces) {
-#pragma unroll
-      for (int e = 0; e < V; ++e) top = max(top, abs_bits(to_float(keep[i][e])));
-    }
+    if (t + i * TPR < pieces) top_of(keep[i], top);
   for (int c = t + NV * TPR; c < pieces; c += TPR) {
     alignas(16) T v[V];
     load(c, v);
-#pragma unroll
-    for (int e = 0; e < V; ++e) top = max(top, abs_bits(to_float(v[e])));
+    top_of(v, top);
   }
-  top = __reduce_max_sync(0xffffffffu, top);
+  top = __reduce_max_sync(0xffffffffu, top_bits<T>(top));
   if (TPR > 32) {
     __shared__ uint32_t tops[8];
     if (lane == 0) tops[threadIdx.x >> 5] = top;
@@ -105,20 +144,31 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(QuantParams p) {
     for (int w = 0; w < 8; ++w) top = max(top, tops[w]);
   }
   const Step s = step_of(top);
+  const float half = 0.5f * s.scale;
   if (t == 0) p.scale[row] = s.scale;
 
   auto store = [&](int piece, const T (&v)[V]) {
-    int8_t o[V < 4 ? 4 : V];
+    Guess g[V];
+    bool doubt = false;
 #pragma unroll
-    for (int e = 0; e < V; ++e) o[e] = s.finite ? (int8_t)quantize_one(to_float(v[e]), s.scale, s.inv) : (int8_t)0;
+    for (int e = 0; e < V; ++e) {
+      g[e] = guess_of(to_float(v[e]), s.scale, s.inv);
+      doubt = doubt || !(fabsf(g[e].rem) < half);
+    }
+    if (doubt) {  // hardly ever: a quotient next to a half, or a row that is not finite
+#pragma unroll
+      for (int e = 0; e < V; ++e) g[e].sum = s.finite ? settled(g[e], half) : 0.0f;
+    }
     if (V == 1) {
-      q[piece] = o[0];
+      q[piece] = (int8_t)__float_as_int(g[0].sum);
     } else {
       uint32_t w[V < 4 ? 1 : V / 4];
 #pragma unroll
-      for (int j = 0; j < (V < 4 ? 1 : V / 4); ++j)
-        w[j] = (uint32_t)(uint8_t)o[4 * j] | (uint32_t)(uint8_t)o[4 * j + 1] << 8 | (uint32_t)(uint8_t)o[4 * j + 2] << 16 |
-               (uint32_t)(uint8_t)o[4 * j + 3] << 24;
+      for (int j = 0; j < V / 4; ++j) {
+        const uint32_t lo = __byte_perm(__float_as_uint(g[4 * j].sum), __float_as_uint(g[4 * j + 1].sum), 0x0040);
+        const uint32_t hi = __byte_perm(__float_as_uint(g[4 * j + 2].sum), __float_as_uint(g[4 * j + 3].sum), 0x0040);
+        w[j] = __byte_perm(lo, hi, 0x5410);
+      }
       if (V == 8) *(reinterpret_cast<uint2*>(q) + piece) = make_uint2(w[0], w[V / 4 - 1]);
       else *(reinterpret_cast<uint32_t*>(q) + piece) = w[0];
     }
@@ -154,7 +204,7 @@ i8_weight_kernel(const float* __restrict__ src, long long ldb, int8_t* __restric
   for (int k0 = 0; k0 < K; k0 += 128) {
     for (int r = ty; r < 128; r += 8)
       tile[tx][r] = n < N && k0 + r < K && s.finite
-                        ? (int8_t)quantize_one(src[(long long)(k0 + r) * ldb + n], s.scale, s.inv) : (int8_t)0;
+                        ? quantize_one(src[(long long)(k0 + r) * ldb + n], s.scale, s.inv) : (int8_t)0;
     __syncthreads();
     for (int c = ty; c < 32; c += 8)
       if (n0 + c < N)
