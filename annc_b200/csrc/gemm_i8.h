@@ -38,10 +38,11 @@ int run_tc(const Params& p, const Route& r, cudaStream_t s);
 __device__ __forceinline__ float scaled(int sum, float scale_a, float scale_b, float bias) {
   return fmaf((float)sum * scale_a, scale_b, bias);
 }
-// Out of line: the loops that hardly ever take it stay small.
+// Out of line: the loops that hardly ever take it stay small.  (The quotient within 2 ulp; correctly rounded it took a
+// third of what 1999 x 1003 x 1001 takes.)
 static __device__ __noinline__ float4 sigmoid4(float4 v) {
-  return make_float4(__fdiv_rn(1.0f, 1.0f + expf(-v.x)), __fdiv_rn(1.0f, 1.0f + expf(-v.y)), __fdiv_rn(1.0f, 1.0f + expf(-v.z)),
-                     __fdiv_rn(1.0f, 1.0f + expf(-v.w)));
+  return make_float4(__fdividef(1.0f, 1.0f + expf(-v.x)), __fdividef(1.0f, 1.0f + expf(-v.y)), __fdividef(1.0f, 1.0f + expf(-v.z)),
+                     __fdividef(1.0f, 1.0f + expf(-v.w)));
 }
 template <int N>
 __device__ __forceinline__ void activate(int act, float (&v)[N]) {

@@ -100,23 +100,24 @@ struct QuantParams {
   int cols;
 };
 
-// TPR threads take a row (a warp or a block of 256); a thread keeps NV pieces of V values in registers between
-// the maximum and the rounding, so a row of up to TPR * NV * V values is read once; what is longer is read
-// again, from L2.  VEC: rows of whole 16-byte pieces at 16-byte addresses; else one value at a time.  Bound by memory
-// once the rounding takes few enough instructions: 8192 x 2048 bf16 31 us with rintf, a conversion and a branch for
-// every value.
+// TPR threads take a row; a thread keeps NV pieces of V values in registers between the maximum and the rounding, so
+// that a row of up to TPR * NV * V values is read once; what is longer is read again, from L2.  VEC: rows of whole 16-byte
+// pieces at 16-byte addresses; else one value at a time.  Bound by memory once the rounding takes few enough
+// instructions (8192 x 2048 bf16 31 us with rintf, a conversion and a branch for every value) and a thread has several
+// pieces on their way (65536 x 256 bf16, a warp a row, one piece a lane, 27 us).
 template <typename T, int TPR, bool VEC>
 __global__ void __launch_bounds__(256) quantize_rows_kernel(QuantParams p) {
   constexpr int V = VEC ? 16 / (int)sizeof(T) : 1;
   constexpr int NV = VEC ? 8 : 16;
   const int t = threadIdx.x % TPR, lane = threadIdx.x & 31;
-  const long long row = (long long)blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
+  const long long at_row = (long long)blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
   pdl_trigger();
   pdl_wait();
-  if (row >= p.rows) return;  // (whole warps, and with TPR = 256 whole blocks)
+  const bool there = at_row < p.rows;
+  const long long row = there ? at_row : 0;
   const T* x = static_cast<const T*>(p.x) + row * p.ld;
   int8_t* q = p.q + row * p.ldq;
-  const int pieces = p.cols / V;
+  const int pieces = there ? p.cols / V : 0;
 
   alignas(16) T keep[NV][V];
   auto load = [&](int piece, T (&to)[V]) {
@@ -135,17 +136,20 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(QuantParams p) {
     load(c, v);
     top_of(v, top);
   }
-  top = __reduce_max_sync(0xffffffffu, top_bits<T>(top));
+  top = top_bits<T>(top);
+#pragma unroll
+  for (int d = 1; d < 32 && d < TPR; d <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
   if (TPR > 32) {
     __shared__ uint32_t tops[8];
-    if (lane == 0) tops[threadIdx.x >> 5] = top;
+    const int warp = threadIdx.x >> 5;
+    if (lane == 0) tops[warp] = top;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < 8; ++w) top = max(top, tops[w]);
+    for (int w = 0; w < TPR / 32; ++w) top = max(top, tops[warp / (TPR / 32) * (TPR / 32) + w]);
   }
   const Step s = step_of(top);
   const float half = 0.5f * s.scale;
-  if (t == 0) p.scale[row] = s.scale;
+  if (t == 0 && there) p.scale[row] = s.scale;
 
   auto store = [&](int piece, const T (&v)[V]) {
     Guess g[V];
@@ -281,13 +285,16 @@ int launch_quantize(const QuantParams& p, cudaStream_t s) {
   constexpr int V = 16 / (int)sizeof(T);
   const bool vec = p.cols % V == 0 && p.ld % V == 0 && (reinterpret_cast<uintptr_t>(p.x) & 15) == 0 && p.ldq % V == 0 &&
                    (reinterpret_cast<uintptr_t>(p.q) & (V - 1)) == 0;
-  const bool warp = p.rows >= 1024 && p.cols <= 32 * (vec ? 8 * V : 16);
-  const long long blocks = warp ? (p.rows + 7) / 8 : p.rows;
+  const int pieces = p.cols / (vec ? V : 1), kept = vec ? 8 : 16;
+  // as few threads a row as hold it in registers, but two blocks an SM if the rows give them
+  int tpr = 4;
+  while (tpr < 256 && (pieces > kept * tpr || p.rows * tpr < 2 * 148 * 256)) tpr *= 4;
+  const long long blocks = (p.rows + 256 / tpr - 1) / (256 / tpr);
   ANNC_REQUIRE(blocks <= 0x7fffffffLL, ANNC_ERR_UNSUPPORTED, "quantize rows: too many rows");
-  const unsigned g = (unsigned)blocks;
-  void (*const kernel)(QuantParams) = vec ? (warp ? quantize_rows_kernel<T, 32, true> : quantize_rows_kernel<T, 256, true>)
-                                          : (warp ? quantize_rows_kernel<T, 32, false> : quantize_rows_kernel<T, 256, false>);
-  ANNC_CUDA(launch_pdl(kernel, dim3(g), dim3(256), 0, s, p));
+  static void (*const kernels[2][4])(QuantParams) = {
+      {quantize_rows_kernel<T, 4, false>, quantize_rows_kernel<T, 16, false>, quantize_rows_kernel<T, 64, false>, quantize_rows_kernel<T, 256, false>},
+      {quantize_rows_kernel<T, 4, true>, quantize_rows_kernel<T, 16, true>, quantize_rows_kernel<T, 64, true>, quantize_rows_kernel<T, 256, true>}};
+  ANNC_CUDA(launch_pdl(kernels[vec][tpr == 4 ? 0 : tpr == 16 ? 1 : tpr == 64 ? 2 : 3], dim3((unsigned)blocks), dim3(256), 0, s, p));
   return ANNC_OK;
 }
 
