@@ -5,17 +5,18 @@
 // tile of 128 rows:  S = Q K^T (tcgen05, operands in shared memory, S in tensor memory), softmax numerators P in
 // registers (a thread per row), P back to tensor memory over S as the operand of  O += P V  (V as it lies, N-major).
 // Two such chains run side by side so that one's products cover the other's exponentials: with more than 128 rows
-// in the item the two are its two row tiles, sharing the key tiles; else they take the key tiles in turn and leave a
-// part each.  The running maximum of a row only moves when a score passes it by more than 2^8 in the
+// in the item the two are its two row tiles, sharing the key tiles; else they take the key tiles in turn and are added
+// at the end of the segment, each reading the other's O from tensor memory.  The running maximum of a row only moves when a score passes it by more than 2^8 in the
 // exponential: until then O keeps its scale, the numerators grow to at most 256, and O is rescaled hardly ever.
 //
 //   warps 0-3, 4-7   softmax of the two chains, rescaling of O, parts
 //   warp 8           TMA: rows, then keys and values through a ring of tiles
 //   warp 9           tensor memory, all products
 //
-// Join kernel.  Warps take (token, key head): its up to 16 heads at a time against the token's own keys with
-// mma.sync straight from global memory (each lane reads 16-byte pieces; the order of the head's values in the products is
-// permuted alike on both sides, so that no transposition is needed), then all parts are added.
+// Join kernel.  Warps take (token, key head): its heads against the token's own keys with mma.sync straight from global
+// memory (each lane reads 16-byte pieces; the order of the head's values in the products is permuted alike on both
+// sides), and the parts of the prefix are added in registers.  Without own keys, items that one CTA has all of are
+// written by the prefix kernel.
 //
 // Sums, maxima and O are held in fp32; the numerators are rounded to the operands' type for the second product, as the
 // tensor cores want them, while their sum is of the unrounded ones.
@@ -50,17 +51,23 @@ template <int DP>
 struct Shape {
   static constexpr int kTile = kTileKeys * DP * 2;  // bytes of 128 rows: DP / 64 blocks of 128 bytes x 128
   static constexpr int kSlots = DP == 128 ? 5 : 9;
-  static constexpr int kBars = 2 * kTile + kSlots * kTile;
+  static constexpr int kExchange = 2 * kTile + kSlots * kTile;  // the second chain's [128] (maximum, sum)
+  static constexpr int kBars = kExchange + kTileRows * 8;
   static constexpr size_t kSmem = 1024 + kBars + 256;
 };
 
 struct PrefixParams {
   Plan plan;
   long long tokens;
-  int kv_heads, group, prefix;
+  int kv_heads, group, prefix, dim;
   float scale2;  // scale * log2(e)
-  float* parts;  // [part][256][DP]
-  float2* stats; // [part][256]: maximum (log2 units), sum
+  float* parts;   // [part][256][DP]
+  float2* stats;  // [part][256]: maximum (log2 units), sum
+  // no own keys, every token a sequence: what a CTA has all of goes out at once
+  int direct;
+  void* out;
+  long long out_row, out_head;
+  float* lse;
   int* error_word;
 };
 
@@ -188,7 +195,8 @@ struct Segment {
   int item, head, tile;  // key head, pair of row tiles
   int first, count;
   int part;
-  bool dual;  // two row tiles; else the chains take the key tiles in turn
+  bool whole;  // all of the item
+  bool dual;   // two row tiles; else the chains take the key tiles in turn
   __device__ __forceinline__ int steps(int chain) const { return dual ? count : (count - chain + 1) / 2; }
   __device__ __forceinline__ int key_tile(int chain, int step) const { return first + (dual ? step : 2 * step + chain); }
 };
@@ -200,8 +208,8 @@ __device__ __forceinline__ Segment segment_at(const PrefixParams& p, int at, int
   s.head = s.item / p.plan.row_items;
   s.tile = s.item - s.head * p.plan.row_items;
   s.dual = p.tokens - (long long)s.tile * 2 * p.plan.tile_tokens > p.plan.tile_tokens;
-  const bool whole = s.count == p.plan.kv_tiles;
-  s.part = whole ? 2 * kMaxCtas + s.item : 2 * (int)blockIdx.x + (at == begin ? 0 : 1);
+  s.whole = s.count == p.plan.kv_tiles;
+  s.part = s.whole ? 2 * kMaxCtas + s.item : 2 * (int)blockIdx.x + (at == begin ? 0 : 1);
   return s;
 }
 
@@ -297,7 +305,8 @@ prefix_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
   const uint32_t bar_full = bars, bar_empty = bars + 8 * S::kSlots;
   const uint32_t bar_q = bars + 16 * S::kSlots, bar_qfree = bar_q + 8;
   const uint32_t bar_s = bar_q + 16, bar_p = bar_q + 32, bar_o = bar_q + 48, bar_ofree = bar_q + 64, bar_h = bar_q + 80;  // per chain
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem_raw + (bar_q + 96 - raw));
+  const uint32_t bar_x = bar_q + 96;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem_raw + (bar_q + 104 - raw));
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;  // (known to be uniform)
@@ -318,6 +327,7 @@ prefix_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
       mbar_init(bar_o + 8 * c, 1);
       mbar_init(bar_ofree + 8 * c, 4);
     }
+    mbar_init(bar_x, 4);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -447,7 +457,7 @@ prefix_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
     const uint32_t lanes = (uint32_t)(q * 32) << 16;
     const uint32_t t_s = tmem + 128 * c + lanes, t_o = tmem + 256 + 128 * c + lanes;
     const float scale = p.scale2;
-    uint32_t parts = 0, done = 0;  // parts with key tiles, steps: of this chain so far
+    uint32_t parts = 0, done = 0, joins = 0;  // segments with key tiles, steps, segments joined: of this chain so far
     for (int at = begin; at < end && ok;) {
       const Segment g = segment_at(p, at, begin, end);
       at += g.count;
@@ -474,31 +484,84 @@ prefix_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
         if (lane == 0) mbar_arrive(bar_p + 8 * c);
       }
       if (!ok) break;
-      // the part: rows of this chain at 128 c
-      const long long at_row = (long long)g.part * kPartRows + c * kTileRows + row;
+      // O and sums of the segment: of two row tiles each chain its own, else both add up to one
       if (steps > 0) {
         ok = all_wait(bar_o + 8 * c, parts & 1u, abort_flag, p.error_word);
         if (!ok) break;
         ++parts;
       }
-      if (row < rows) p.stats[at_row] = make_float2(top, sum);
-      if (steps > 0 && any) {
+      float weight = 1.0f, other = 0.0f;  // of this chain's O, of the other one's
+      if (!g.dual && g.steps(1) > 0) {
+        float2* const exchange = reinterpret_cast<float2*>(smem_raw + (base + S::kExchange - raw));
+        if (c == 1) {
+          exchange[row] = make_float2(top, sum);
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar_x);
+          continue;
+        }
+        ok = all_wait(bar_x, joins & 1u, abort_flag, p.error_word);
+        if (!ok) break;
+        ++joins;
+        const float2 o = exchange[row];
+        const float now = fmaxf(top, o.x);
+        weight = exp2_approx(top - now);
+        other = exp2_approx(o.x - now);
+        sum = sum * weight + o.y * other;
+        top = now;
+      } else if (!g.dual && c == 1) {
+        continue;
+      }
+      if (any) {
         tc_fence_after();
-#pragma unroll
+        const bool mine = row < rows;
+        const bool direct = p.direct && g.whole;
+        const long long part_row = (long long)g.part * kPartRows + (g.dual ? c : 0) * kTileRows + row;
+        const long long token = token0 + row / p.group;
+        const int head = g.head * p.group + row % p.group;
+        if (mine) {
+          if (!direct) p.stats[part_row] = make_float2(top, sum);
+          else if (p.lse) p.lse[token * p.kv_heads * p.group + head] = (top + log2f(sum)) * kLn2;
+        }
+        if (direct) {
+          const float inv = 1.0f / sum;
+          weight *= inv;
+          other *= inv;
+        }
+        const uint32_t t_o1 = tmem + 384 + lanes;
         for (int b = 0; b < DP / 32; ++b) {
           uint32_t o[32];
+          float v[32];
           tmem_ld32(t_o + 32 * b, o);
           tmem_ld_wait();
-          if (row < rows) {
-            uint4* out = reinterpret_cast<uint4*>(p.parts + at_row * DP + 32 * b);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) out[j] = make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+          for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(o[j]) * weight;
+          if (!g.dual && g.steps(1) > 0) {
+            tmem_ld32(t_o1 + 32 * b, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] = fmaf(__uint_as_float(o[j]), other, v[j]);
+          }
+          if (!mine) continue;
+          if (!direct) {
+            float4* out = reinterpret_cast<float4*>(p.parts + part_row * DP + 32 * b);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) out[j] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+          } else {
+            T* out = static_cast<T*>(p.out) + token * p.out_row + head * p.out_head + 32 * b;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if (32 * b + 8 * j < p.dim)
+                *reinterpret_cast<uint4*>(out + 8 * j) = make_uint4(pack2<T>(v[8 * j], v[8 * j + 1]), pack2<T>(v[8 * j + 2], v[8 * j + 3]),
+                                                                    pack2<T>(v[8 * j + 4], v[8 * j + 5]), pack2<T>(v[8 * j + 6], v[8 * j + 7]));
           }
         }
         tc_fence_before();
       }
       __syncwarp();
-      if (lane == 0) mbar_arrive(bar_ofree + 8 * c);
+      if (lane == 0) {  // the first chain has read both
+        mbar_arrive(bar_ofree + 8 * c);
+        if (!g.dual) mbar_arrive(bar_ofree + 8);
+      }
     }
   }
   }
@@ -528,215 +591,221 @@ __device__ __forceinline__ void mma_16816<__half>(float (&d)[4], const uint32_t 
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// The 8 x 8 matrix of 16-bit values that the warp holds (a row per four lanes), transposed.
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
 struct JoinParams {
   Params a;
   Plan plan;
   float scale2;
+  int direct;  // whole items are out already
   const float* parts;
   const float2* stats;
 };
 
-// WPU warps work on a (token, key head).  Rows of the products: 16 heads of the group.  In the first product the
-// four words of a lane's 16-byte piece of Q and K take the places of the k indices that the fragment layout gives the
-// lane; in the second one a lane holds values dn * DP/8 .. of four keys, dn = lane / 4, and column dn of product t is
-// value dn * DP/8 + t, so that lane l ends with the 2 * DP/8 values from (l % 4) * DP/4 on, of rows l / 4 and l / 4 + 8.
+// WPU warps work on a (token, key head), eight heads of its group at a time: the columns of the products, so that
+// groups of eight and fewer waste nothing.  S^T = K Q^T: keys are the 16 rows; a lane reads 16-byte pieces of two key
+// rows, whose four words take the places of the k indices that the fragment layout gives the lane, in Q alike.
+// O^T = V^T P^T: a lane reads values dn * DP/8 .. of four key rows (dn = lane / 4); rows dn and dn + 8 of product t are
+// values dn * DP/8 + 2 t and + 2 t + 1, so that it ends with DP/8 adjacent values of heads 2 (lane % 4) and + 1, onto which
+// the parts of the prefix are added in place.
 template <typename T, int DP, int WPU>
 __global__ void __launch_bounds__(128) join_kernel(JoinParams p) {
-  constexpr int NT = DP / 8;   // values a lane holds of a value row; products of the second kind
-  constexpr int LD = DP + 4;
-  extern __shared__ float join_smem[];  // per warp: 16 rows of LD, 16 x (maximum, sum)
+  constexpr int NT = DP / 8;  // values a lane holds of a head
+  extern __shared__ float join_smem[];  // (WPU > 1) per warp: 8 heads of DP, 8 x (maximum, sum)
+  constexpr int kWarp = 8 * DP + 16;
   pdl_trigger();
   pdl_wait();
   const Params& a = p.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, wi = warp % WPU;
-  float* const mine = join_smem + warp * (16 * LD + 32);
-  float* const unit0 = join_smem + (warp - wi) * (16 * LD + 32);  // of the unit's first warp
   const long long unit = (long long)blockIdx.x * (4 / WPU) + warp / WPU;
   const long long token = unit / a.kv_heads;
   const int h = (int)(unit - token * a.kv_heads);
   if (token >= a.tokens) return;
+
+  // Where the token's rows lie in the parts of the prefix.
+  int part0 = 0, parts = 0, row0 = 0, item = 0;
+  if (p.plan.kv_tiles > 0) {
+    const long long tile = token / (2 * p.plan.tile_tokens);
+    const int within = (int)(token - tile * 2 * p.plan.tile_tokens);
+    const int second = within >= p.plan.tile_tokens;
+    item = h * p.plan.row_items + (int)tile;
+    const int from = item * p.plan.kv_tiles;
+    part0 = from / p.plan.per_cta;
+    parts = (from + p.plan.kv_tiles - 1) / p.plan.per_cta - part0 + 1;
+    row0 = second * kTileRows + (within - second * p.plan.tile_tokens) * a.group;
+    if (p.direct && parts == 1) return;
+  }
+  auto part_row = [&](int i) -> long long {
+    const int cta = part0 + i;
+    const int slot = parts == 1 ? 2 * kMaxCtas + item : 2 * cta + (cta * p.plan.per_cta < item * p.plan.kv_tiles ? 1 : 0);
+    return (long long)slot * kPartRows + row0;
+  };
   long long first;
   int count;
   if (!own_keys(a, token, &first, &count)) return;  // (the whole unit)
   const int quad = lane & 3, dn = lane >> 2;
+  const bool none = count == 0 && parts == 0;
 
-  for (int g0 = 0; g0 < a.group; g0 += 16) {
-    const int rows = min(16, a.group - g0);
-    if (count > 0) {
-      uint32_t q[DP / 32][2][4];
+  for (int g0 = 0; g0 < a.group; g0 += 8) {
+    const int heads = min(8, a.group - g0);
+    float o[2][NT];  // [head 2 quad + e][value dn * NT + i]
+    float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.0f, 0.0f};
 #pragma unroll
-      for (int b = 0; b < DP / 32; ++b)
+    for (int e = 0; e < 2; ++e)
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          uint4 v = make_uint4(0, 0, 0, 0);
-          if (dn + 8 * r < rows && 32 * b + 8 * quad < a.dim)
-            v = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q.data) + token * a.q.row +
-                                                ((long long)h * a.group + g0 + dn + 8 * r) * a.q.head + 32 * b + 8 * quad);
-          q[b][r][0] = v.x; q[b][r][1] = v.y; q[b][r][2] = v.z; q[b][r][3] = v.w;
-        }
-      float o[NT][4];
+      for (int i = 0; i < NT; ++i) o[e][i] = 0.0f;
+
+    if (count > 16 * wi) {
+      uint4 q[DP / 32];
 #pragma unroll
-      for (int t = 0; t < NT; ++t) o[t][0] = o[t][1] = o[t][2] = o[t][3] = 0.0f;
-      float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.0f, 0.0f};
+      for (int b = 0; b < DP / 32; ++b) {
+        q[b] = make_uint4(0, 0, 0, 0);
+        if (dn < heads && 32 * b + 8 * quad < a.dim)
+          q[b] = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q.data) + token * a.q.row +
+                                                 ((long long)h * a.group + g0 + dn) * a.q.head + 32 * b + 8 * quad);
+      }
       const T* const keys = static_cast<const T*>(a.ko.data) + first * a.ko.row + h * a.ko.head;
       const T* const values = static_cast<const T*>(a.vo.data) + first * a.vo.row + h * a.vo.head;
       for (int k0 = 16 * wi; k0 < count; k0 += 16 * WPU) {
-        float s[2][4];
+        uint4 k[2][DP / 32];  // keys dn, dn + 8
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          s[half][0] = s[half][1] = s[half][2] = s[half][3] = 0.0f;
-          const int key = k0 + 8 * half + dn;
-          uint4 w[DP / 32];
+        for (int r = 0; r < 2; ++r)
 #pragma unroll
           for (int b = 0; b < DP / 32; ++b) {
-            w[b] = make_uint4(0, 0, 0, 0);
-            if (key < count && 32 * b + 8 * quad < a.dim)
-              w[b] = *reinterpret_cast<const uint4*>(keys + key * a.ko.row + 32 * b + 8 * quad);
+            k[r][b] = make_uint4(0, 0, 0, 0);
+            if (k0 + dn + 8 * r < count && 32 * b + 8 * quad < a.dim)
+              k[r][b] = *reinterpret_cast<const uint4*>(keys + (k0 + dn + 8 * r) * a.ko.row + 32 * b + 8 * quad);
           }
-#pragma unroll
-          for (int b = 0; b < DP / 32; ++b) {
-            const uint32_t a0[4] = {q[b][0][0], q[b][1][0], q[b][0][1], q[b][1][1]};
-            const uint32_t a1[4] = {q[b][0][2], q[b][1][2], q[b][0][3], q[b][1][3]};
-            mma_16816<T>(s[half], a0, w[b].x, w[b].y);
-            mma_16816<T>(s[half], a1, w[b].z, w[b].w);
-          }
-        }
-        // values of keys 2 quad, 2 quad + 1, + 8, + 9 (on their way during the softmax)
-        uint32_t v[4][NT / 2];
+        uint4 v[4][NT / 8];  // keys 2 quad, 2 quad + 1, + 8, + 9 (on their way during the softmax)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int key = k0 + 2 * quad + (i & 1) + 8 * (i >> 1);
 #pragma unroll
           for (int x = 0; x < NT / 8; ++x) {
-            uint4 w = make_uint4(0, 0, 0, 0);
+            v[i][x] = make_uint4(0, 0, 0, 0);
             if (key < count && dn * NT + 8 * x < a.dim)
-              w = *reinterpret_cast<const uint4*>(values + key * a.vo.row + dn * NT + 8 * x);
-            v[i][4 * x] = w.x; v[i][4 * x + 1] = w.y; v[i][4 * x + 2] = w.z; v[i][4 * x + 3] = w.w;
+              v[i][x] = *reinterpret_cast<const uint4*>(values + key * a.vo.row + dn * NT + 8 * x);
           }
         }
-        float pr[2][4];  // [row][key 2 quad, + 1, + 8, + 9]
+        float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // keys dn, dn, dn + 8, dn + 8; heads 2 quad, + 1
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          float now = top[r];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const bool there = k0 + 2 * quad + (i & 1) + 8 * (i >> 1) < count;
-            pr[r][i] = there ? s[i >> 1][2 * r + (i & 1)] * p.scale2 : -INFINITY;
-            now = fmaxf(now, pr[r][i]);
-          }
-          now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, 1));
-          now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, 2));
-          const float keep = top[r] == -INFINITY ? 0.0f : exp2_approx(top[r] - now);
-          top[r] = now;
-          sum[r] *= keep;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const bool there = k0 + 2 * quad + (i & 1) + 8 * (i >> 1) < count;
-            pr[r][i] = there ? exp2_approx(pr[r][i] - now) : 0.0f;
-            sum[r] += pr[r][i];
-          }
-#pragma unroll
-          for (int t = 0; t < NT; ++t) {
-            o[t][2 * r] *= keep;
-            o[t][2 * r + 1] *= keep;
-          }
+        for (int b = 0; b < DP / 32; ++b) {
+          const uint32_t a0[4] = {k[0][b].x, k[1][b].x, k[0][b].y, k[1][b].y}, a1[4] = {k[0][b].z, k[1][b].z, k[0][b].w, k[1][b].w};
+          mma_16816<T>(s, a0, q[b].x, q[b].y);
+          mma_16816<T>(s, a1, q[b].z, q[b].w);
         }
-        const uint32_t pa[4] = {pack2<T>(pr[0][0], pr[0][1]), pack2<T>(pr[1][0], pr[1][1]), pack2<T>(pr[0][2], pr[0][3]),
-                                pack2<T>(pr[1][2], pr[1][3])};
+        float pr[4], keep[2];
 #pragma unroll
-        for (int x = 0; x < NT / 2; ++x) {
-          mma_16816<T>(o[2 * x], pa, __byte_perm(v[0][x], v[1][x], 0x5410), __byte_perm(v[2][x], v[3][x], 0x5410));
-          mma_16816<T>(o[2 * x + 1], pa, __byte_perm(v[0][x], v[1][x], 0x7632), __byte_perm(v[2][x], v[3][x], 0x7632));
+        for (int e = 0; e < 2; ++e) {
+          const bool in0 = k0 + dn < count, in1 = k0 + dn + 8 < count;
+          const float s0 = in0 ? s[e] * p.scale2 : -INFINITY, s1 = in1 ? s[2 + e] * p.scale2 : -INFINITY;
+          float now = fmaxf(top[e], fmaxf(s0, s1));
+#pragma unroll
+          for (int d = 4; d < 32; d <<= 1) now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, d));
+          keep[e] = top[e] == -INFINITY ? 0.0f : exp2_approx(top[e] - now);
+          top[e] = now;
+          pr[e] = in0 ? exp2_approx(s0 - now) : 0.0f;
+          pr[2 + e] = in1 ? exp2_approx(s1 - now) : 0.0f;
+          sum[e] = sum[e] * keep[e] + pr[e] + pr[2 + e];
+#pragma unroll
+          for (int i = 0; i < NT; ++i) o[e][i] *= keep[e];
+        }
+        const uint32_t p0 = transposed(pack2<T>(pr[0], pr[1])), p1 = transposed(pack2<T>(pr[2], pr[3]));
+#pragma unroll
+        for (int t = 0; t < NT / 2; ++t) {
+          auto word = [&](int i) { return (t & 3) == 0 ? v[i][t / 4].x : (t & 3) == 1 ? v[i][t / 4].y : (t & 3) == 2 ? v[i][t / 4].z : v[i][t / 4].w; };
+          const uint32_t av[4] = {__byte_perm(word(0), word(1), 0x5410), __byte_perm(word(0), word(1), 0x7632),
+                                  __byte_perm(word(2), word(3), 0x5410), __byte_perm(word(2), word(3), 0x7632)};
+          float d[4] = {o[0][2 * t], o[1][2 * t], o[0][2 * t + 1], o[1][2 * t + 1]};
+          mma_16816<T>(d, av, p0, p1);
+          o[0][2 * t] = d[0]; o[1][2 * t] = d[1]; o[0][2 * t + 1] = d[2]; o[1][2 * t + 1] = d[3];
         }
       }
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 1);
-        sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 2);
-        if (dn + 8 * r < rows) {
+      for (int e = 0; e < 2; ++e)
 #pragma unroll
-          for (int e = 0; e < 2; ++e)
-#pragma unroll
-            for (int t = 0; t < NT; t += 4)
-              *reinterpret_cast<float4*>(mine + (dn + 8 * r) * LD + (2 * quad + e) * NT + t) =
-                  make_float4(o[t][2 * r + e], o[t + 1][2 * r + e], o[t + 2][2 * r + e], o[t + 3][2 * r + e]);
-          if (quad == 0) {
-            mine[16 * LD + 2 * (dn + 8 * r)] = top[r];
-            mine[16 * LD + 2 * (dn + 8 * r) + 1] = sum[r];
-          }
-        }
-      }
+        for (int d = 4; d < 32; d <<= 1) sum[e] += __shfl_xor_sync(0xffffffffu, sum[e], d);
     }
-    if (WPU == 1) __syncwarp();
-    else __syncthreads();
 
-    // Where the token's rows lie in the parts of the prefix.
-    int part0 = 0, parts = 0, chain_rows = 0, row0 = 0, item = 0;
-    bool whole = true;
-    if (p.plan.kv_tiles > 0) {
-      const long long tile = token / (2 * p.plan.tile_tokens);
-      const int within = (int)(token - tile * 2 * p.plan.tile_tokens);
-      const bool dual = a.tokens - tile * 2 * p.plan.tile_tokens > p.plan.tile_tokens;
-      item = h * p.plan.row_items + (int)tile;
-      const int from = item * p.plan.kv_tiles;
-      part0 = from / p.plan.per_cta;
-      parts = (from + p.plan.kv_tiles - 1) / p.plan.per_cta - part0 + 1;
-      whole = parts == 1;
-      const int chain = dual ? within / p.plan.tile_tokens : 0;
-      row0 = chain * kTileRows + (within - chain * p.plan.tile_tokens) * a.group + g0;
-      chain_rows = dual ? 0 : kTileRows;  // a part of the second chain behind the first one's
-    }
-    const int chains = chain_rows ? 2 : 1, all = parts * chains;
-    auto part_row = [&](int i) -> long long {
-      const int k = chains == 2 ? i >> 1 : i, cta = part0 + k;
-      const int slot = whole ? 2 * kMaxCtas + item : 2 * cta + (cta * p.plan.per_cta < item * p.plan.kv_tiles ? 1 : 0);
-      return (long long)slot * kPartRows + row0 + (chains == 2 && (i & 1) ? chain_rows : 0);
-    };
-    for (int e = wi * 32 + lane; e < rows * (DP / 4); e += WPU * 32) {
-      const int r = e / (DP / 4), d = e % (DP / 4) * 4;
-      float top = -INFINITY;
-      if (count > 0)
+    // the prefix's parts (each lane its own heads' values; a part's maximum and sum are read by eight lanes)
+    for (int i = wi; i < parts; i += WPU) {
+      const long long at = part_row(i) + g0 + 2 * quad;
 #pragma unroll
-        for (int w = 0; w < WPU; ++w)
-          if (16 * w < count) top = fmaxf(top, unit0[w * (16 * LD + 32) + 16 * LD + 2 * r]);
-      for (int i = 0; i < all; ++i) {
-        const float2 st = p.stats[part_row(i) + r];
-        if (st.y != 0.0f) top = fmaxf(top, st.x);
+      for (int e = 0; e < 2; ++e) {
+        if (2 * quad + e >= heads) continue;
+        const float2 st = p.stats[at + e];
+        float4 v[NT / 4];
+#pragma unroll
+        for (int x = 0; x < NT / 4; ++x) v[x] = *reinterpret_cast<const float4*>(p.parts + (at + e) * DP + dn * NT + 4 * x);
+        const float now = fmaxf(top[e], st.x);
+        const float keep = sum[e] == 0.0f ? 0.0f : exp2_approx(top[e] - now), weight = exp2_approx(st.x - now);
+        top[e] = now;
+        sum[e] = sum[e] * keep + st.y * weight;
+#pragma unroll
+        for (int x = 0; x < NT / 4; ++x) {
+          o[e][4 * x] = o[e][4 * x] * keep + v[x].x * weight;
+          o[e][4 * x + 1] = o[e][4 * x + 1] * keep + v[x].y * weight;
+          o[e][4 * x + 2] = o[e][4 * x + 2] * keep + v[x].z * weight;
+          o[e][4 * x + 3] = o[e][4 * x + 3] * keep + v[x].w * weight;
+        }
       }
-      float sum = 0.0f;
-      float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      if (count > 0)
+    }
+
+    if (WPU > 1) {  // the warps' states, joined by the first one
+      float* const mine = join_smem + warp * kWarp;
+      if (wi > 0) {
 #pragma unroll
-        for (int w = 0; w < WPU; ++w)
-          if (16 * w < count) {
-            const float* from = unit0 + w * (16 * LD + 32);
-            const float weight = exp2_approx(from[16 * LD + 2 * r] - top);
-            const float4 v = *reinterpret_cast<const float4*>(from + r * LD + d);
-            sum += weight * from[16 * LD + 2 * r + 1];
-            acc.x += weight * v.x; acc.y += weight * v.y; acc.z += weight * v.z; acc.w += weight * v.w;
+        for (int e = 0; e < 2; ++e) {
+#pragma unroll
+          for (int i = 0; i < NT; i += 4)
+            *reinterpret_cast<float4*>(mine + (2 * quad + e) * DP + dn * NT + i) = make_float4(o[e][i], o[e][i + 1], o[e][i + 2], o[e][i + 3]);
+          if (dn == 0) {
+            mine[8 * DP + 2 * (2 * quad + e)] = top[e];
+            mine[8 * DP + 2 * (2 * quad + e) + 1] = sum[e];
           }
-      for (int i = 0; i < all; ++i) {
-        const long long at = part_row(i) + r;
-        const float2 st = p.stats[at];
-        if (st.y == 0.0f) continue;  // a chain that had no key tile: nothing was left there
-        const float weight = exp2_approx(st.x - top);
-        const float4 v = *reinterpret_cast<const float4*>(p.parts + at * DP + d);
-        sum += weight * st.y;
-        acc.x += weight * v.x; acc.y += weight * v.y; acc.z += weight * v.z; acc.w += weight * v.w;
+        }
       }
-      const bool none = count == 0 && all == 0;
-      const float inv = none ? 0.0f : 1.0f / sum;
-      const long long head = (long long)h * a.group + g0 + r;
-      if (d < a.dim) {
-        uint2 w;
-        w.x = pack2<T>(acc.x * inv, acc.y * inv);
-        w.y = pack2<T>(acc.z * inv, acc.w * inv);
-        *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + token * a.out_row + head * a.out_head + d) = w;
+      __syncthreads();
+      if (wi == 0) {
+#pragma unroll
+        for (int w = 1; w < WPU; ++w) {
+          const float* const from = join_smem + (warp + w) * kWarp;
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float other_top = from[8 * DP + 2 * (2 * quad + e)], other_sum = from[8 * DP + 2 * (2 * quad + e) + 1];
+            if (other_sum == 0.0f) continue;  // nothing was left for that warp
+            const float now = fmaxf(top[e], other_top);
+            const float keep = sum[e] == 0.0f ? 0.0f : exp2_approx(top[e] - now), weight = exp2_approx(other_top - now);
+            top[e] = now;
+            sum[e] = sum[e] * keep + other_sum * weight;
+#pragma unroll
+            for (int i = 0; i < NT; ++i) o[e][i] = o[e][i] * keep + from[(2 * quad + e) * DP + dn * NT + i] * weight;
+          }
+        }
       }
-      if (d == 0 && a.lse) a.lse[token * a.heads + head] = none ? -INFINITY : (top + log2f(sum)) * kLn2;
     }
-    if (WPU == 1) __syncwarp();
-    else __syncthreads();
+    if (wi == 0) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        if (2 * quad + e >= heads) continue;
+        const float inv = none ? 0.0f : 1.0f / sum[e];
+        const long long head = (long long)h * a.group + g0 + 2 * quad + e;
+        T* const out = static_cast<T*>(a.out) + token * a.out_row + head * a.out_head + dn * NT;
+#pragma unroll
+        for (int x = 0; x < NT / 8; ++x)
+          if (dn * NT + 8 * x < a.dim)
+            *reinterpret_cast<uint4*>(out + 8 * x) =
+                make_uint4(pack2<T>(o[e][8 * x] * inv, o[e][8 * x + 1] * inv), pack2<T>(o[e][8 * x + 2] * inv, o[e][8 * x + 3] * inv),
+                           pack2<T>(o[e][8 * x + 4] * inv, o[e][8 * x + 5] * inv), pack2<T>(o[e][8 * x + 6] * inv, o[e][8 * x + 7] * inv));
+        if (a.lse && dn == 0) a.lse[token * a.heads + head] = none ? -INFINITY : (top[e] + log2f(sum[e])) * kLn2;
+      }
+    }
+    if (WPU > 1) __syncthreads();
   }
 }
 
@@ -800,7 +869,7 @@ template <typename T, int DP, int WPU>
 int launch_join(const JoinParams& p, cudaStream_t s) {
   const long long blocks = (p.a.tokens * p.a.kv_heads + 4 / WPU - 1) / (4 / WPU);
   ANNC_REQUIRE(blocks <= 0x7fffffffLL, ANNC_ERR_UNSUPPORTED, "prefix attention: too many tokens");
-  const size_t smem = 4 * (16 * (DP + 4) + 32) * sizeof(float);
+  const size_t smem = WPU > 1 ? 4 * (8 * DP + 16) * sizeof(float) : 0;
   ANNC_CUDA(launch_pdl(join_kernel<T, DP, WPU>, dim3((unsigned)blocks), dim3(128), smem, s, p));
   return ANNC_OK;
 }
@@ -813,14 +882,21 @@ int run_as(const Params& a, void* workspace, cudaStream_t s) {
   p.kv_heads = a.kv_heads;
   p.group = a.group;
   p.prefix = (int)a.prefix;
+  p.dim = a.dim;
   p.scale2 = a.scale * kLog2e;
   const size_t slots = 2 * kMaxCtas + (size_t)p.plan.items;
   p.parts = static_cast<float*>(workspace);
   p.stats = reinterpret_cast<float2*>(p.parts + slots * kPartRows * DP);
   p.error_word = gemm::gemm_error_word();
   if (!p.error_word) return fail(ANNC_ERR_CUDA, "the tensor-core error word is not addressable");
+  p.direct = !a.own_len && !a.q_begin;
+  p.out = a.out;
+  p.out_row = a.out_row;
+  p.out_head = a.out_head;
+  p.lse = a.lse;
   if (a.prefix > 0) ANNC_TRY((launch_prefix<T, DP>(a, p, s)));
-  const JoinParams j{a, p.plan, p.scale2, p.parts, p.stats};
+  if (p.direct && a.prefix > 0 && p.plan.per_cta % p.plan.kv_tiles == 0) return ANNC_OK;  // no item was cut
+  const JoinParams j{a, p.plan, p.scale2, p.direct, p.parts, p.stats};
   // a unit of work fills a warp; with few units (latency) four warps share one
   return a.tokens * a.kv_heads >= 1184 ? launch_join<T, DP, 1>(j, s) : launch_join<T, DP, 4>(j, s);
 }
@@ -843,7 +919,7 @@ bool tc_supported(const Params& p, int) {
   if (!rows_ok(p.q, p.tokens, p.heads, true) || p.q.head * p.group >= (1LL << 39)) return false;
   if (p.prefix > 0 && (!rows_ok(p.kp, p.prefix, p.kv_heads, true) || !rows_ok(p.vp, p.prefix, p.kv_heads, true))) return false;
   if (p.own_len && (!rows_ok(p.ko, p.own_rows, p.kv_heads, false) || !rows_ok(p.vo, p.own_rows, p.kv_heads, false))) return false;
-  return (reinterpret_cast<uintptr_t>(p.out) & 7) == 0 && p.out_row % 4 == 0 && p.out_head % 4 == 0;
+  return (reinterpret_cast<uintptr_t>(p.out) & 15) == 0 && (p.tokens == 1 || p.out_row % 8 == 0) && (p.heads == 1 || p.out_head % 8 == 0);
 }
 
 int run_tc(const Params& p, int dtype, void* workspace, cudaStream_t s) {
