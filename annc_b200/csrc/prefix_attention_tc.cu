@@ -598,6 +598,32 @@ __device__ __forceinline__ uint32_t transposed(uint32_t x) {
   return y;
 }
 
+// own_keys with a whole warp: of the entries of q_begin 32 are looked at at once.
+__device__ __forceinline__ bool own_keys_of_warp(const Params& p, int token, int lane, long long* first, int* count) {
+  *first = 0;
+  *count = 0;
+  int seq = token, behind = 0;  // tokens of the sequence behind this one
+  if (p.q_begin) {
+    int lo = 0, hi = (int)p.sequences;  // q_begin[lo] <= token < q_begin[hi]
+    if (hi == 0 || token < p.q_begin[0] || token >= p.q_begin[hi]) return false;
+    while (hi - lo > 1) {
+      const int step = (hi - lo + 31) >> 5, at = lo + step * (lane + 1);
+      const int below = __popc(__ballot_sync(0xffffffffu, at < hi && p.q_begin[at] <= token));
+      lo += step * below;
+      hi = min(hi, lo + step);
+    }
+    seq = lo;
+    behind = p.q_begin[seq + 1] - 1 - token;
+  }
+  if (!p.own_len) return true;
+  const long long begin = p.own_begin[seq];
+  const int len = p.own_len[seq] - behind;
+  if (len <= 0 || begin < 0 || begin >= p.own_rows) return true;
+  *first = begin;
+  *count = (int)min((long long)len, p.own_rows - begin);
+  return true;
+}
+
 struct JoinParams {
   Params a;
   Plan plan;
@@ -622,18 +648,17 @@ __global__ void __launch_bounds__(128) join_kernel(JoinParams p) {
   pdl_wait();
   const Params& a = p.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, wi = warp % WPU;
-  const long long unit = (long long)blockIdx.x * (4 / WPU) + warp / WPU;
-  const long long token = unit / a.kv_heads;
-  const int h = (int)(unit - token * a.kv_heads);
-  if (token >= a.tokens) return;
+  // (32-bit arithmetic throughout: with 64-bit divisions the indexes took most of the kernel's time)
+  const int unit = (int)blockIdx.x * (4 / WPU) + warp / WPU;
+  const int token = unit / a.kv_heads, h = unit - token * a.kv_heads;
+  if (token >= (int)a.tokens) return;
 
   // Where the token's rows lie in the parts of the prefix.
   int part0 = 0, parts = 0, row0 = 0, item = 0;
   if (p.plan.kv_tiles > 0) {
-    const long long tile = token / (2 * p.plan.tile_tokens);
-    const int within = (int)(token - tile * 2 * p.plan.tile_tokens);
+    const int tile = token / (2 * p.plan.tile_tokens), within = token - tile * 2 * p.plan.tile_tokens;
     const int second = within >= p.plan.tile_tokens;
-    item = h * p.plan.row_items + (int)tile;
+    item = h * p.plan.row_items + tile;
     const int from = item * p.plan.kv_tiles;
     part0 = from / p.plan.per_cta;
     parts = (from + p.plan.kv_tiles - 1) / p.plan.per_cta - part0 + 1;
@@ -647,7 +672,7 @@ __global__ void __launch_bounds__(128) join_kernel(JoinParams p) {
   };
   long long first;
   int count;
-  if (!own_keys(a, token, &first, &count)) return;  // (the whole unit)
+  if (!own_keys_of_warp(a, token, lane, &first, &count)) return;  // (the whole unit)
   const int quad = lane & 3, dn = lane >> 2;
   const bool none = count == 0 && parts == 0;
 
@@ -666,7 +691,7 @@ __global__ void __launch_bounds__(128) join_kernel(JoinParams p) {
       for (int b = 0; b < DP / 32; ++b) {
         q[b] = make_uint4(0, 0, 0, 0);
         if (dn < heads && 32 * b + 8 * quad < a.dim)
-          q[b] = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q.data) + token * a.q.row +
+          q[b] = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q.data) + (long long)token * a.q.row +
                                                  ((long long)h * a.group + g0 + dn) * a.q.head + 32 * b + 8 * quad);
       }
       const T* const keys = static_cast<const T*>(a.ko.data) + first * a.ko.row + h * a.ko.head;
@@ -795,14 +820,14 @@ __global__ void __launch_bounds__(128) join_kernel(JoinParams p) {
         if (2 * quad + e >= heads) continue;
         const float inv = none ? 0.0f : 1.0f / sum[e];
         const long long head = (long long)h * a.group + g0 + 2 * quad + e;
-        T* const out = static_cast<T*>(a.out) + token * a.out_row + head * a.out_head + dn * NT;
+        T* const out = static_cast<T*>(a.out) + (long long)token * a.out_row + head * a.out_head + dn * NT;
 #pragma unroll
         for (int x = 0; x < NT / 8; ++x)
           if (dn * NT + 8 * x < a.dim)
             *reinterpret_cast<uint4*>(out + 8 * x) =
                 make_uint4(pack2<T>(o[e][8 * x] * inv, o[e][8 * x + 1] * inv), pack2<T>(o[e][8 * x + 2] * inv, o[e][8 * x + 3] * inv),
                            pack2<T>(o[e][8 * x + 4] * inv, o[e][8 * x + 5] * inv), pack2<T>(o[e][8 * x + 6] * inv, o[e][8 * x + 7] * inv));
-        if (a.lse && dn == 0) a.lse[token * a.heads + head] = none ? -INFINITY : (top[e] + log2f(sum[e])) * kLn2;
+        if (a.lse && dn == 0) a.lse[(long long)token * a.heads + head] = none ? -INFINITY : (top[e] + log2f(sum[e])) * kLn2;
       }
     }
     if (WPU > 1) __syncthreads();
@@ -867,8 +892,7 @@ int launch_prefix(const Params& a, const PrefixParams& p, cudaStream_t s) {
 
 template <typename T, int DP, int WPU>
 int launch_join(const JoinParams& p, cudaStream_t s) {
-  const long long blocks = (p.a.tokens * p.a.kv_heads + 4 / WPU - 1) / (4 / WPU);
-  ANNC_REQUIRE(blocks <= 0x7fffffffLL, ANNC_ERR_UNSUPPORTED, "prefix attention: too many tokens");
+  const long long blocks = (p.a.tokens * p.a.kv_heads + 4 / WPU - 1) / (4 / WPU);  // (tc_supported: they fit 30 bits)
   const size_t smem = WPU > 1 ? 4 * (8 * DP + 16) * sizeof(float) : 0;
   ANNC_CUDA(launch_pdl(join_kernel<T, DP, WPU>, dim3((unsigned)blocks), dim3(128), smem, s, p));
   return ANNC_OK;
@@ -915,7 +939,7 @@ bool tc_supported(const Params& p, int) {
   if (p.dim % 8 || p.dim > 128 || p.group > kTileRows) return false;
   if (p.prefix > 0 && !(p.scale >= 0.0f)) return false;  // (the prefix kernel takes the maximum of the unscaled scores)
   const Plan plan = plan_of(p.tokens, p.kv_heads, p.group, p.prefix);
-  if ((long long)plan.row_items * p.kv_heads * (plan.kv_tiles > 0 ? plan.kv_tiles : 1) >= (1LL << 30)) return false;
+  if ((long long)plan.row_items * p.kv_heads * (plan.kv_tiles > 0 ? plan.kv_tiles : 1) >= (1LL << 30) || p.tokens * p.kv_heads >= (1LL << 30)) return false;
   if (!rows_ok(p.q, p.tokens, p.heads, true) || p.q.head * p.group >= (1LL << 39)) return false;
   if (p.prefix > 0 && (!rows_ok(p.kp, p.prefix, p.kv_heads, true) || !rows_ok(p.vp, p.prefix, p.kv_heads, true))) return false;
   if (p.own_len && (!rows_ok(p.ko, p.own_rows, p.kv_heads, false) || !rows_ok(p.vo, p.own_rows, p.kv_heads, false))) return false;
