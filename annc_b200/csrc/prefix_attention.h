@@ -41,6 +41,14 @@ struct Plan {
   int row_items;    // items of a key head
   int items, kv_tiles;
   int per_cta, ctas;
+
+  // Parts: CTA c leaves what it has of the item its share starts in at 2 c, of the one it ends in at 2 c + 1, and an item
+  // that it has all of (`parts` is 1) behind all these, at the item's number.
+#ifdef __CUDACC__
+  __device__ __forceinline__ int part_of(int item, int cta, int parts) const {
+    return parts == 1 ? 2 * kMaxCtas + item : 2 * cta + (cta * per_cta < item * kv_tiles ? 1 : 0);
+  }
+#endif
 };
 
 inline Plan plan_of(long long tokens, int kv_heads, int group, long long prefix) {
@@ -56,8 +64,6 @@ inline Plan plan_of(long long tokens, int kv_heads, int group, long long prefix)
   p.ctas = (int)((total + per - 1) / per);
   return p;
 }
-// Parts: CTA c leaves what it has of the item its share starts in at 2 c, of the one it ends in at 2 c + 1, and an
-// item that it has all of behind all these, at the item's number.
 inline int part_width(int dim) { return dim <= 64 ? 64 : 128; }
 
 bool tc_supported(const Params& p, int dtype);

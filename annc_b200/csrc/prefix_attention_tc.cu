@@ -56,13 +56,23 @@ struct Shape {
   static constexpr size_t kSmem = 1024 + kBars + 256;
 };
 
+// The own keys that a token sees; row < 0: a token of no sequence.
+struct Own {
+  long long row;
+  int count, reserved;
+};
+
 struct PrefixParams {
   Plan plan;
+  Params a;
   long long tokens;
   int kv_heads, group, prefix, dim;
   float scale2;  // scale * log2(e)
-  float* parts;   // [part][256][DP]
+  // [part][DP / 4][256] pieces of four values: a lane writes its row, so rows are adjacent (row by row the writes, 32
+  // pieces at 512 bytes from one another, took 5 us a segment)
+  float4* parts;
   float2* stats;  // [part][256]: maximum (log2 units), sum
+  Own* own;       // per token, or null
   // no own keys, every token a sequence: what a CTA has all of goes out at once
   int direct;
   void* out;
@@ -448,6 +458,13 @@ prefix_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
         n0 += 2 * g.count;
       }
     }
+  } else if (p.own) {
+    // the two warps that have nothing else to do look up, for the join, what every token sees of its sequence
+    for (long long t = (long long)blockIdx.x * 64 + (threadIdx.x - 320); t < p.tokens; t += (long long)gridDim.x * 64) {
+      Own own = {0, 0, 0};
+      if (!own_keys(p.a, t, &own.row, &own.count)) own.row = -1;
+      p.own[t] = own;
+    }
   }
   } else {
   registers_up();
@@ -543,9 +560,9 @@ prefix_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
           }
           if (!mine) continue;
           if (!direct) {
-            float4* out = reinterpret_cast<float4*>(p.parts + part_row * DP + 32 * b);
+            float4* out = p.parts + ((long long)g.part * (DP / 4) + 8 * b) * kPartRows + (g.dual ? c : 0) * kTileRows + row;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) out[j] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+            for (int j = 0; j < 8; ++j) out[j * kPartRows] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
           } else {
             T* out = static_cast<T*>(p.out) + token * p.out_row + head * p.out_head + 32 * b;
 #pragma unroll
@@ -628,9 +645,9 @@ struct JoinParams {
   Params a;
   Plan plan;
   float scale2;
-  int direct;  // whole items are out already
-  const float* parts;
+  const float4* parts;
   const float2* stats;
+  const Own* own;
 };
 
 // WPU warps work on a (token, key head), eight heads of its group at a time: the columns of the products, so that
@@ -663,16 +680,17 @@ __global__ void __launch_bounds__(128) join_kernel(JoinParams p) {
     part0 = from / p.plan.per_cta;
     parts = (from + p.plan.kv_tiles - 1) / p.plan.per_cta - part0 + 1;
     row0 = second * kTileRows + (within - second * p.plan.tile_tokens) * a.group;
-    if (p.direct && parts == 1) return;
   }
-  auto part_row = [&](int i) -> long long {
-    const int cta = part0 + i;
-    const int slot = parts == 1 ? 2 * kMaxCtas + item : 2 * cta + (cta * p.plan.per_cta < item * p.plan.kv_tiles ? 1 : 0);
-    return (long long)slot * kPartRows + row0;
-  };
   long long first;
   int count;
-  if (!own_keys_of_warp(a, token, lane, &first, &count)) return;  // (the whole unit)
+  if (p.own) {
+    const int4 own = *reinterpret_cast<const int4*>(p.own + token);
+    if (own.y < 0) return;  // (the whole unit)
+    first = (long long)own.y << 32 | (uint32_t)own.x;
+    count = own.z;
+  } else if (!own_keys_of_warp(a, token, lane, &first, &count)) {
+    return;
+  }
   const int quad = lane & 3, dn = lane >> 2;
   const bool none = count == 0 && parts == 0;
 
@@ -759,14 +777,14 @@ __global__ void __launch_bounds__(128) join_kernel(JoinParams p) {
 
     // the prefix's parts (each lane its own heads' values; a part's maximum and sum are read by eight lanes)
     for (int i = wi; i < parts; i += WPU) {
-      const long long at = part_row(i) + g0 + 2 * quad;
+      const int slot = p.plan.part_of(item, part0 + i, parts), row = row0 + g0 + 2 * quad;
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         if (2 * quad + e >= heads) continue;
-        const float2 st = p.stats[at + e];
+        const float2 st = p.stats[(long long)slot * kPartRows + row + e];
         float4 v[NT / 4];
 #pragma unroll
-        for (int x = 0; x < NT / 4; ++x) v[x] = *reinterpret_cast<const float4*>(p.parts + (at + e) * DP + dn * NT + 4 * x);
+        for (int x = 0; x < NT / 4; ++x) v[x] = p.parts[((long long)slot * (DP / 4) + dn * (NT / 4) + x) * kPartRows + row + e];
         const float now = fmaxf(top[e], st.x);
         const float keep = sum[e] == 0.0f ? 0.0f : exp2_approx(top[e] - now), weight = exp2_approx(st.x - now);
         top[e] = now;
@@ -831,6 +849,65 @@ __global__ void __launch_bounds__(128) join_kernel(JoinParams p) {
       }
     }
     if (WPU > 1) __syncthreads();
+  }
+}
+
+// ---------------------------------------------------------------- cut items without own keys
+
+// Without own keys, and every token a sequence, only items that a share's end cuts are left to add up, at most one per
+// CTA.  Block (b, y): rows 32 y .. of the item that the share of CTA b ends in.  Parts are read with rows across the lanes,
+// as they lie, and turned in shared memory.
+template <typename T, int DP>
+__global__ void __launch_bounds__(256) cut_items_kernel(JoinParams p) {
+  __shared__ float turned[32][DP + 1];
+  pdl_trigger();
+  pdl_wait();
+  const Params& a = p.a;
+  const int end = ((int)blockIdx.x + 1) * p.plan.per_cta;  // of the share
+  const int item = end / p.plan.kv_tiles, from = item * p.plan.kv_tiles;
+  if (item >= p.plan.items || end == from || (int)blockIdx.x != from / p.plan.per_cta) return;  // not cut here, or cut before already
+  const int parts = (from + p.plan.kv_tiles - 1) / p.plan.per_cta - (int)blockIdx.x + 1;
+  const int h = item / p.plan.row_items, tile = item - h * p.plan.row_items;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int row = 32 * (int)blockIdx.y + lane, second = row >= kTileRows;
+  const int in_tile = row - second * kTileRows, tokens = p.plan.tile_tokens;
+  const long long token0 = ((long long)2 * tile + second) * tokens;
+  const bool there = in_tile < tokens * a.group && token0 + in_tile / a.group < a.tokens;
+  float top = -INFINITY, sum = 0.0f;
+  if (there) {
+    for (int i = 0; i < parts; ++i) top = fmaxf(top, p.stats[(long long)p.plan.part_of(item, (int)blockIdx.x + i, parts) * kPartRows + row].x);
+    // warp w: pieces w, w + 8, ..
+    float4 acc[DP / 32];
+#pragma unroll
+    for (int x = 0; x < DP / 32; ++x) acc[x] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int i = 0; i < parts; ++i) {
+      const int slot = p.plan.part_of(item, (int)blockIdx.x + i, parts);
+      const float2 st = p.stats[(long long)slot * kPartRows + row];
+      const float weight = exp2_approx(st.x - top);
+      sum += st.y * weight;
+#pragma unroll
+      for (int x = 0; x < DP / 32; ++x) {
+        const float4 v = p.parts[((long long)slot * (DP / 4) + warp + 8 * x) * kPartRows + row];
+        acc[x].x += v.x * weight; acc[x].y += v.y * weight; acc[x].z += v.z * weight; acc[x].w += v.w * weight;
+      }
+    }
+    const float inv = 1.0f / sum;
+#pragma unroll
+    for (int x = 0; x < DP / 32; ++x) {
+      float* const to = &turned[lane][4 * (warp + 8 * x)];
+      to[0] = acc[x].x * inv; to[1] = acc[x].y * inv; to[2] = acc[x].z * inv; to[3] = acc[x].w * inv;
+    }
+    if (warp == 0 && a.lse) a.lse[(token0 + in_tile / a.group) * a.heads + (long long)h * a.group + in_tile % a.group] = (top + log2f(sum)) * kLn2;
+  }
+  __syncthreads();
+  constexpr int PER = DP / 8;  // lanes a row: eight values each
+  for (int r = threadIdx.x / PER; r < 32; r += 256 / PER) {
+    const int at = 32 * (int)blockIdx.y + r - second * kTileRows, d = threadIdx.x % PER * 8;
+    const long long token = token0 + at / a.group;
+    if (at >= tokens * a.group || token >= a.tokens || d >= a.dim) continue;
+    const float* v = &turned[r][d];
+    *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + token * a.out_row + ((long long)h * a.group + at % a.group) * a.out_head + d) =
+        make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
   }
 }
 
@@ -909,8 +986,10 @@ int run_as(const Params& a, void* workspace, cudaStream_t s) {
   p.dim = a.dim;
   p.scale2 = a.scale * kLog2e;
   const size_t slots = 2 * kMaxCtas + (size_t)p.plan.items;
-  p.parts = static_cast<float*>(workspace);
-  p.stats = reinterpret_cast<float2*>(p.parts + slots * kPartRows * DP);
+  p.a = a;
+  p.parts = static_cast<float4*>(workspace);
+  p.stats = reinterpret_cast<float2*>(p.parts + slots * kPartRows * (DP / 4));
+  p.own = a.prefix > 0 && (a.own_len || a.q_begin) ? reinterpret_cast<Own*>(p.stats + slots * kPartRows) : nullptr;
   p.error_word = gemm::gemm_error_word();
   if (!p.error_word) return fail(ANNC_ERR_CUDA, "the tensor-core error word is not addressable");
   p.direct = !a.own_len && !a.q_begin;
@@ -919,8 +998,12 @@ int run_as(const Params& a, void* workspace, cudaStream_t s) {
   p.out_head = a.out_head;
   p.lse = a.lse;
   if (a.prefix > 0) ANNC_TRY((launch_prefix<T, DP>(a, p, s)));
-  if (p.direct && a.prefix > 0 && p.plan.per_cta % p.plan.kv_tiles == 0) return ANNC_OK;  // no item was cut
-  const JoinParams j{a, p.plan, p.scale2, p.direct, p.parts, p.stats};
+  const JoinParams j{a, p.plan, p.scale2, p.parts, p.stats, p.own};
+  if (p.direct && a.prefix > 0) {
+    if (p.plan.ctas > 1 && p.plan.per_cta % p.plan.kv_tiles != 0)
+      ANNC_CUDA(launch_pdl(cut_items_kernel<T, DP>, dim3((unsigned)p.plan.ctas - 1, kPartRows / 32), dim3(256), 0, s, j));
+    return ANNC_OK;
+  }
   // a unit of work fills a warp; with few units (latency) four warps share one
   return a.tokens * a.kv_heads >= 1184 ? launch_join<T, DP, 1>(j, s) : launch_join<T, DP, 4>(j, s);
 }
@@ -932,7 +1015,7 @@ size_t tc_workspace_bytes(long long tokens, int heads, int kv_heads, int dim) {
   if (group > kTileRows || dim > 128) return 0;
   const long long per_item = 2LL * (kTileRows / group);
   const unsigned long long slots = 2ULL * kMaxCtas + (unsigned long long)((tokens + per_item - 1) / per_item) * kv_heads;
-  return (size_t)(slots * kPartRows * ((unsigned long long)part_width(dim) * 4 + 8));
+  return (size_t)(slots * kPartRows * ((unsigned long long)part_width(dim) * 4 + 8) + (unsigned long long)tokens * sizeof(Own));
 }
 
 bool tc_supported(const Params& p, int) {
