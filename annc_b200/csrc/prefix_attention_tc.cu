@@ -645,35 +645,39 @@ struct JoinParams {
   Params a;
   Plan plan;
   float scale2;
+  int tokens;  // of a unit of work
   const float4* parts;
   const float2* stats;
   const Own* own;
 };
 
-// WPU warps work on a (token, key head), eight heads of its group at a time: the columns of the products, so that
-// groups of eight and fewer waste nothing.  S^T = K Q^T: keys are the 16 rows; a lane reads 16-byte pieces of two key
+// WPU warps work on the eight columns of a product: eight heads of a (token, key head) at a time, or with smaller groups
+// the heads of p.tokens adjacent tokens.  S^T = K Q^T: keys are the 16 rows; a lane reads 16-byte pieces of two key
 // rows, whose four words take the places of the k indices that the fragment layout gives the lane, in Q alike.
 // O^T = V^T P^T: a lane reads values dn * DP/8 .. of four key rows (dn = lane / 4); rows dn and dn + 8 of product t are
-// values dn * DP/8 + 2 t and + 2 t + 1, so that it ends with DP/8 adjacent values of heads 2 (lane % 4) and + 1, onto which
-// the parts of the prefix are added in place.
+// values dn * DP/8 + 2 t and + 2 t + 1, so that it ends with DP/8 adjacent values of columns 2 (lane % 4) and + 1, onto which
+// the parts of the prefix are added in place.  Tokens take their own keys one after the other, and only their columns
+// take what a product gives: what another token's values hold (infinities, NaN) reaches no other.
 template <typename T, int DP, int WPU>
-__global__ void __launch_bounds__(128) join_kernel(JoinParams p) {
-  constexpr int NT = DP / 8;  // values a lane holds of a head
-  extern __shared__ float join_smem[];  // (WPU > 1) per warp: 8 heads of DP, 8 x (maximum, sum)
+__global__ void __launch_bounds__(128, DP == 128 ? 4 : 5) join_kernel(JoinParams p) {
+  constexpr int NT = DP / 8;  // values a lane holds of a column
+  extern __shared__ float join_smem[];  // (WPU > 1) per warp: 8 columns of DP, 8 x (maximum, sum)
   constexpr int kWarp = 8 * DP + 16;
   pdl_trigger();
   pdl_wait();
   const Params& a = p.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, wi = warp % WPU;
+  const int quad = lane & 3, dn = lane >> 2;
   // (32-bit arithmetic throughout: with 64-bit divisions the indexes took most of the kernel's time)
   const int unit = (int)blockIdx.x * (4 / WPU) + warp / WPU;
-  const int token = unit / a.kv_heads, h = unit - token * a.kv_heads;
-  if (token >= (int)a.tokens) return;
+  const int slice = unit / a.kv_heads, h = unit - slice * a.kv_heads, token0 = slice * p.tokens;
+  if (token0 >= (int)a.tokens) return;
+  const int tokens = min(p.tokens, (int)a.tokens - token0);
 
-  // Where the token's rows lie in the parts of the prefix.
+  // Where the rows lie in the parts of the prefix (a unit's tokens are in one tile).
   int part0 = 0, parts = 0, row0 = 0, item = 0;
   if (p.plan.kv_tiles > 0) {
-    const int tile = token / (2 * p.plan.tile_tokens), within = token - tile * 2 * p.plan.tile_tokens;
+    const int tile = token0 / (2 * p.plan.tile_tokens), within = token0 - tile * 2 * p.plan.tile_tokens;
     const int second = within >= p.plan.tile_tokens;
     item = h * p.plan.row_items + tile;
     const int from = item * p.plan.kv_tiles;
@@ -681,36 +685,48 @@ __global__ void __launch_bounds__(128) join_kernel(JoinParams p) {
     parts = (from + p.plan.kv_tiles - 1) / p.plan.per_cta - part0 + 1;
     row0 = second * kTileRows + (within - second * p.plan.tile_tokens) * a.group;
   }
-  long long first;
-  int count;
-  if (p.own) {
-    const int4 own = *reinterpret_cast<const int4*>(p.own + token);
-    if (own.y < 0) return;  // (the whole unit)
-    first = (long long)own.y << 32 | (uint32_t)own.x;
-    count = own.z;
-  } else if (!own_keys_of_warp(a, token, lane, &first, &count)) {
-    return;
-  }
-  const int quad = lane & 3, dn = lane >> 2;
-  const bool none = count == 0 && parts == 0;
+  const int per_token = p.tokens > 1 ? a.group : 8;  // columns
+  int of[2];                                         // the token of this lane's columns
+#pragma unroll
+  for (int e = 0; e < 2; ++e) of[e] = (2 * quad + e) / per_token;
 
   for (int g0 = 0; g0 < a.group; g0 += 8) {
-    const int heads = min(8, a.group - g0);
-    float o[2][NT];  // [head 2 quad + e][value dn * NT + i]
+    const int heads = p.tokens > 1 ? a.group : min(8, a.group - g0), columns = p.tokens > 1 ? tokens * a.group : heads;
+    float o[2][NT];  // [column 2 quad + e][value dn * NT + i]
     float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.0f, 0.0f};
+    bool valid[2] = {false, false};
 #pragma unroll
     for (int e = 0; e < 2; ++e)
 #pragma unroll
       for (int i = 0; i < NT; ++i) o[e][i] = 0.0f;
 
-    if (count > 16 * wi) {
+    for (int tt = 0; tt < tokens; ++tt) {
+      const int token = token0 + tt;
+      long long first;
+      int count;
+      if (p.own) {
+        const int4 own = *reinterpret_cast<const int4*>(p.own + token);
+        if (own.y < 0) continue;
+        first = (long long)own.y << 32 | (uint32_t)own.x;
+        count = own.z;
+      } else if (!own_keys_of_warp(a, token, lane, &first, &count)) {
+        continue;
+      }
+      bool active[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        active[e] = of[e] == tt && 2 * quad + e < columns;
+        valid[e] = valid[e] || active[e];
+      }
+      if (count <= 16 * wi) continue;
       uint4 q[DP / 32];
 #pragma unroll
       for (int b = 0; b < DP / 32; ++b) {
+        const int g = dn - tt * per_token;  // column dn is a head of this token?
         q[b] = make_uint4(0, 0, 0, 0);
-        if (dn < heads && 32 * b + 8 * quad < a.dim)
+        if (g >= 0 && g < heads && 32 * b + 8 * quad < a.dim)
           q[b] = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q.data) + (long long)token * a.q.row +
-                                                 ((long long)h * a.group + g0 + dn) * a.q.head + 32 * b + 8 * quad);
+                                                 ((long long)h * a.group + g0 + g) * a.q.head + 32 * b + 8 * quad);
       }
       const T* const keys = static_cast<const T*>(a.ko.data) + first * a.ko.row + h * a.ko.head;
       const T* const values = static_cast<const T*>(a.vo.data) + first * a.vo.row + h * a.vo.head;
@@ -735,7 +751,7 @@ __global__ void __launch_bounds__(128) join_kernel(JoinParams p) {
               v[i][x] = *reinterpret_cast<const uint4*>(values + key * a.vo.row + dn * NT + 8 * x);
           }
         }
-        float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // keys dn, dn, dn + 8, dn + 8; heads 2 quad, + 1
+        float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // keys dn, dn, dn + 8, dn + 8; columns 2 quad, + 1
 #pragma unroll
         for (int b = 0; b < DP / 32; ++b) {
           const uint32_t a0[4] = {k[0][b].x, k[1][b].x, k[0][b].y, k[1][b].y}, a1[4] = {k[0][b].z, k[1][b].z, k[0][b].w, k[1][b].w};
@@ -745,18 +761,18 @@ __global__ void __launch_bounds__(128) join_kernel(JoinParams p) {
         float pr[4], keep[2];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const bool in0 = k0 + dn < count, in1 = k0 + dn + 8 < count;
+          const bool in0 = active[e] && k0 + dn < count, in1 = active[e] && k0 + dn + 8 < count;
           const float s0 = in0 ? s[e] * p.scale2 : -INFINITY, s1 = in1 ? s[2 + e] * p.scale2 : -INFINITY;
           float now = fmaxf(top[e], fmaxf(s0, s1));
 #pragma unroll
           for (int d = 4; d < 32; d <<= 1) now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, d));
           keep[e] = top[e] == -INFINITY ? 0.0f : exp2_approx(top[e] - now);
-          top[e] = now;
           pr[e] = in0 ? exp2_approx(s0 - now) : 0.0f;
           pr[2 + e] = in1 ? exp2_approx(s1 - now) : 0.0f;
-          sum[e] = sum[e] * keep[e] + pr[e] + pr[2 + e];
-#pragma unroll
-          for (int i = 0; i < NT; ++i) o[e][i] *= keep[e];
+          if (active[e]) {
+            top[e] = now;
+            sum[e] = sum[e] * keep[e] + pr[e] + pr[2 + e];
+          }
         }
         const uint32_t p0 = transposed(pack2<T>(pr[0], pr[1])), p1 = transposed(pack2<T>(pr[2], pr[3]));
 #pragma unroll
@@ -764,23 +780,25 @@ __global__ void __launch_bounds__(128) join_kernel(JoinParams p) {
           auto word = [&](int i) { return (t & 3) == 0 ? v[i][t / 4].x : (t & 3) == 1 ? v[i][t / 4].y : (t & 3) == 2 ? v[i][t / 4].z : v[i][t / 4].w; };
           const uint32_t av[4] = {__byte_perm(word(0), word(1), 0x5410), __byte_perm(word(0), word(1), 0x7632),
                                   __byte_perm(word(2), word(3), 0x5410), __byte_perm(word(2), word(3), 0x7632)};
-          float d[4] = {o[0][2 * t], o[1][2 * t], o[0][2 * t + 1], o[1][2 * t + 1]};
+          float d[4] = {o[0][2 * t] * keep[0], o[1][2 * t] * keep[1], o[0][2 * t + 1] * keep[0], o[1][2 * t + 1] * keep[1]};
           mma_16816<T>(d, av, p0, p1);
-          o[0][2 * t] = d[0]; o[1][2 * t] = d[1]; o[0][2 * t + 1] = d[2]; o[1][2 * t + 1] = d[3];
+          if (active[0]) { o[0][2 * t] = d[0]; o[0][2 * t + 1] = d[2]; }
+          if (active[1]) { o[1][2 * t] = d[1]; o[1][2 * t + 1] = d[3]; }
         }
       }
-#pragma unroll
-      for (int e = 0; e < 2; ++e)
-#pragma unroll
-        for (int d = 4; d < 32; d <<= 1) sum[e] += __shfl_xor_sync(0xffffffffu, sum[e], d);
     }
+    // (a column's sum is spread over the lanes of its keys; so far every one of them added to the same maximum)
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+#pragma unroll
+      for (int d = 4; d < 32; d <<= 1) sum[e] += __shfl_xor_sync(0xffffffffu, sum[e], d);
 
-    // the prefix's parts (each lane its own heads' values; a part's maximum and sum are read by eight lanes)
+    // the prefix's parts (each lane its own columns' values; a part's maximum and sum are read by eight lanes)
     for (int i = wi; i < parts; i += WPU) {
       const int slot = p.plan.part_of(item, part0 + i, parts), row = row0 + g0 + 2 * quad;
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        if (2 * quad + e >= heads) continue;
+        if (2 * quad + e >= columns) continue;
         const float2 st = p.stats[(long long)slot * kPartRows + row + e];
         float4 v[NT / 4];
 #pragma unroll
@@ -835,17 +853,18 @@ __global__ void __launch_bounds__(128) join_kernel(JoinParams p) {
     if (wi == 0) {
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        if (2 * quad + e >= heads) continue;
+        if (!valid[e]) continue;
+        const bool none = sum[e] == 0.0f;  // no key at all (a largest score adds at least 1 to its sum)
         const float inv = none ? 0.0f : 1.0f / sum[e];
-        const long long head = (long long)h * a.group + g0 + 2 * quad + e;
-        T* const out = static_cast<T*>(a.out) + (long long)token * a.out_row + head * a.out_head + dn * NT;
+        const long long token = token0 + of[e], head = (long long)h * a.group + g0 + 2 * quad + e - of[e] * per_token;
+        T* const out = static_cast<T*>(a.out) + token * a.out_row + head * a.out_head + dn * NT;
 #pragma unroll
         for (int x = 0; x < NT / 8; ++x)
           if (dn * NT + 8 * x < a.dim)
             *reinterpret_cast<uint4*>(out + 8 * x) =
                 make_uint4(pack2<T>(o[e][8 * x] * inv, o[e][8 * x + 1] * inv), pack2<T>(o[e][8 * x + 2] * inv, o[e][8 * x + 3] * inv),
                            pack2<T>(o[e][8 * x + 4] * inv, o[e][8 * x + 5] * inv), pack2<T>(o[e][8 * x + 6] * inv, o[e][8 * x + 7] * inv));
-        if (a.lse && dn == 0) a.lse[(long long)token * a.heads + head] = none ? -INFINITY : (top[e] + log2f(sum[e])) * kLn2;
+        if (a.lse && dn == 0) a.lse[token * a.heads + head] = none ? -INFINITY : (top[e] + log2f(sum[e])) * kLn2;
       }
     }
     if (WPU > 1) __syncthreads();
@@ -969,7 +988,7 @@ int launch_prefix(const Params& a, const PrefixParams& p, cudaStream_t s) {
 
 template <typename T, int DP, int WPU>
 int launch_join(const JoinParams& p, cudaStream_t s) {
-  const long long blocks = (p.a.tokens * p.a.kv_heads + 4 / WPU - 1) / (4 / WPU);  // (tc_supported: they fit 30 bits)
+  const long long units = (p.a.tokens + p.tokens - 1) / p.tokens * p.a.kv_heads, blocks = (units + 4 / WPU - 1) / (4 / WPU);  // (tc_supported: they fit 30 bits)
   const size_t smem = WPU > 1 ? 4 * (8 * DP + 16) * sizeof(float) : 0;
   ANNC_CUDA(launch_pdl(join_kernel<T, DP, WPU>, dim3((unsigned)blocks), dim3(128), smem, s, p));
   return ANNC_OK;
@@ -998,14 +1017,17 @@ int run_as(const Params& a, void* workspace, cudaStream_t s) {
   p.out_head = a.out_head;
   p.lse = a.lse;
   if (a.prefix > 0) ANNC_TRY((launch_prefix<T, DP>(a, p, s)));
-  const JoinParams j{a, p.plan, p.scale2, p.parts, p.stats, p.own};
+  JoinParams j{a, p.plan, p.scale2, 1, p.parts, p.stats, p.own};
   if (p.direct && a.prefix > 0) {
     if (p.plan.ctas > 1 && p.plan.per_cta % p.plan.kv_tiles != 0)
       ANNC_CUDA(launch_pdl(cut_items_kernel<T, DP>, dim3((unsigned)p.plan.ctas - 1, kPartRows / 32), dim3(256), 0, s, j));
     return ANNC_OK;
   }
-  // a unit of work fills a warp; with few units (latency) four warps share one
-  return a.tokens * a.kv_heads >= 1184 ? launch_join<T, DP, 1>(j, s) : launch_join<T, DP, 4>(j, s);
+  // A unit of work fills a warp, with small groups several tokens' of them; with few units (latency) four warps share
+  // one token.
+  if (a.tokens * a.kv_heads < 1184) return launch_join<T, DP, 4>(j, s);
+  j.tokens = a.group < 8 ? 8 / a.group : 1;
+  return launch_join<T, DP, 1>(j, s);
 }
 
 }  // namespace
