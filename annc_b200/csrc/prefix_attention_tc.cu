@@ -45,6 +45,7 @@ using namespace annc::tc;
 
 constexpr int kThreads = 384;  // eight softmax warps, loads, products, and two that complete the group of four
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr int kPolyEvery = 4;  // of the pairs of exponentials, one in so many goes to the multiply-add units
 constexpr float kSlack = 8.0f;  // log2 of what a numerator may grow to before the maximum moves
 
 template <int DP>
@@ -181,6 +182,28 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
       : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
   return d;
 }
+// 2^x for x <= 8 on the multiply-add units, which have time left beside the 16 exponentials a cycle of the SM's special
+// ones: x = n + f with n the nearest whole number (read off the low bits of x + 1.5 * 2^23), 2^f by the polynomial of
+// degree four with the least relative error on [-1/2, 1/2] (2.6e-6, found by Remez exchange), n added to its exponent.
+// Below 2^-125 it stays there.  Not for a NaN, which comes out as some number.
+__device__ __forceinline__ float2 exp2_poly(float2 x) {
+  constexpr float kMagic = 12582912.0f;
+  x = make_float2(fmaxf(x.x, -125.0f), fmaxf(x.y, -125.0f));
+  const float2 t = add2(x, make_float2(kMagic, kMagic));
+  const float2 f = fma2(add2(t, make_float2(-kMagic, -kMagic)), make_float2(-1.0f, -1.0f), x);
+  float2 y = make_float2(0.009570101911f, 0.009570101911f);
+  y = fma2(y, f, make_float2(0.05591786032f, 0.05591786032f));
+  y = fma2(y, f, make_float2(0.2402474483f, 0.2402474483f));
+  y = fma2(y, f, make_float2(0.6931218147f, 0.6931218147f));
+  y = fma2(y, f, make_float2(0.9999992614f, 0.9999992614f));
+  return make_float2(__int_as_float(__float_as_int(y.x) + (__float_as_int(t.x) << 23)), __int_as_float(__float_as_int(y.y) + (__float_as_int(t.y) << 23)));
+}
+// The largest of three, a NaN if one is.
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi);
 template <>
@@ -235,9 +258,9 @@ __device__ __forceinline__ float max32(const uint32_t (&r)[32], int first, int v
     for (int i = 0; i < 4; ++i) {
       const float x = TAIL && first + j + i >= valid ? -INFINITY : __uint_as_float(r[j + i]);
       const float y = TAIL && first + j + 4 + i >= valid ? -INFINITY : __uint_as_float(r[j + 4 + i]);
-      m[i] = fmaxf(fmaxf(m[i], x), y);
+      m[i] = max3_nan(m[i], x, y);
     }
-  return fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+  return max3_nan(max3_nan(m[0], m[1], m[2]), m[3], m[3]);
 }
 template <typename T, bool TAIL>
 __device__ __forceinline__ void exp32(const uint32_t (&r)[32], int first, int valid, float2 scale, float2 minus_top, float2 (&sum)[2],
@@ -245,7 +268,7 @@ __device__ __forceinline__ void exp32(const uint32_t (&r)[32], int first, int va
 #pragma unroll
   for (int j = 0; j < 32; j += 2) {
     const float2 x = fma2(make_float2(__uint_as_float(r[j]), __uint_as_float(r[j + 1])), scale, minus_top);
-    float2 e = make_float2(exp2_approx(x.x), exp2_approx(x.y));
+    float2 e = j / 2 % kPolyEvery == kPolyEvery - 1 ? exp2_poly(x) : make_float2(exp2_approx(x.x), exp2_approx(x.y));
     if (TAIL) {
       if (first + j >= valid) e.x = 0.0f;
       if (first + j + 1 >= valid) e.y = 0.0f;
@@ -263,8 +286,9 @@ __device__ __forceinline__ void softmax_tile(uint32_t t_s, uint32_t t_o, float s
   tmem_ld32(t_s + 64, r2);
   tmem_ld32(t_s + 96, r3);
   tmem_ld_wait();
-  const float now = fmaxf(fmaxf(max32<TAIL>(r0, 0, valid, -INFINITY), max32<TAIL>(r1, 32, valid, -INFINITY)),
-                          fmaxf(max32<TAIL>(r2, 64, valid, -INFINITY), max32<TAIL>(r3, 96, valid, -INFINITY))) * scale;
+  const float m0 = max32<TAIL>(r0, 0, valid, -INFINITY), m1 = max32<TAIL>(r1, 32, valid, -INFINITY);
+  const float m2 = max32<TAIL>(r2, 64, valid, -INFINITY), m3 = max32<TAIL>(r3, 96, valid, -INFINITY);
+  const float now = max3_nan(max3_nan(m0, m1, m2), m3, m3) * scale;
   if (first) {
     top = now;
   } else if (__any_sync(0xffffffffu, now > top + kSlack)) {
@@ -299,6 +323,7 @@ __device__ __forceinline__ void softmax_tile(uint32_t t_s, uint32_t t_o, float s
   tmem_st16(t_s + 48, w);
   sums[0] = add2(sums[0], sums[1]);
   sum = sums[0].x + sums[0].y;
+  if (!(now < INFINITY)) sum = __uint_as_float(0x7fc00000u);  // a NaN or +inf among the scores makes the row one of NaN
   tmem_st_wait();
 }
 
@@ -659,7 +684,7 @@ struct JoinParams {
 // the parts of the prefix are added in place.  Tokens take their own keys one after the other, and only their columns
 // take what a product gives: what another token's values hold (infinities, NaN) reaches no other.
 template <typename T, int DP, int WPU>
-__global__ void __launch_bounds__(128, DP == 128 ? 4 : 5) join_kernel(JoinParams p) {
+__global__ void __launch_bounds__(WPU > 1 ? 32 * WPU : 128, WPU > 1 ? 1 : DP == 128 ? 4 : 5) join_kernel(JoinParams p) {
   constexpr int NT = DP / 8;  // values a lane holds of a column
   extern __shared__ float join_smem[];  // (WPU > 1) per warp: 8 columns of DP, 8 x (maximum, sum)
   constexpr int kWarp = 8 * DP + 16;
@@ -669,7 +694,7 @@ __global__ void __launch_bounds__(128, DP == 128 ? 4 : 5) join_kernel(JoinParams
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, wi = warp % WPU;
   const int quad = lane & 3, dn = lane >> 2;
   // (32-bit arithmetic throughout: with 64-bit divisions the indexes took most of the kernel's time)
-  const int unit = (int)blockIdx.x * (4 / WPU) + warp / WPU;
+  const int unit = WPU > 1 ? (int)blockIdx.x : (int)blockIdx.x * 4 + warp;
   const int slice = unit / a.kv_heads, h = unit - slice * a.kv_heads, token0 = slice * p.tokens;
   if (token0 >= (int)a.tokens) return;
   const int tokens = min(p.tokens, (int)a.tokens - token0);
@@ -794,6 +819,7 @@ __global__ void __launch_bounds__(128, DP == 128 ? 4 : 5) join_kernel(JoinParams
       for (int d = 4; d < 32; d <<= 1) sum[e] += __shfl_xor_sync(0xffffffffu, sum[e], d);
 
     // the prefix's parts (each lane its own columns' values; a part's maximum and sum are read by eight lanes)
+#pragma unroll 2
     for (int i = wi; i < parts; i += WPU) {
       const int slot = p.plan.part_of(item, part0 + i, parts), row = row0 + g0 + 2 * quad;
 #pragma unroll
@@ -988,9 +1014,9 @@ int launch_prefix(const Params& a, const PrefixParams& p, cudaStream_t s) {
 
 template <typename T, int DP, int WPU>
 int launch_join(const JoinParams& p, cudaStream_t s) {
-  const long long units = (p.a.tokens + p.tokens - 1) / p.tokens * p.a.kv_heads, blocks = (units + 4 / WPU - 1) / (4 / WPU);  // (tc_supported: they fit 30 bits)
-  const size_t smem = WPU > 1 ? 4 * (8 * DP + 16) * sizeof(float) : 0;
-  ANNC_CUDA(launch_pdl(join_kernel<T, DP, WPU>, dim3((unsigned)blocks), dim3(128), smem, s, p));
+  const long long units = (p.a.tokens + p.tokens - 1) / p.tokens * p.a.kv_heads, blocks = WPU > 1 ? units : (units + 3) / 4;  // (tc_supported: they fit 30 bits)
+  const size_t smem = WPU > 1 ? WPU * (8 * DP + 16) * sizeof(float) : 0;
+  ANNC_CUDA(launch_pdl(join_kernel<T, DP, WPU>, dim3((unsigned)blocks), dim3(WPU > 1 ? 32 * WPU : 128), smem, s, p));
   return ANNC_OK;
 }
 
@@ -1023,9 +1049,9 @@ int run_as(const Params& a, void* workspace, cudaStream_t s) {
       ANNC_CUDA(launch_pdl(cut_items_kernel<T, DP>, dim3((unsigned)p.plan.ctas - 1, kPartRows / 32), dim3(256), 0, s, j));
     return ANNC_OK;
   }
-  // A unit of work fills a warp, with small groups several tokens' of them; with few units (latency) four warps share
+  // A unit of work fills a warp, with small groups several tokens' of them; with few units (latency) eight warps share
   // one token.
-  if (a.tokens * a.kv_heads < 1184) return launch_join<T, DP, 4>(j, s);
+  if (a.tokens * a.kv_heads < 1184) return launch_join<T, DP, 8>(j, s);
   j.tokens = a.group < 8 ? 8 / a.group : 1;
   return launch_join<T, DP, 1>(j, s);
 }
