@@ -283,10 +283,11 @@ __device__ __forceinline__ void softmax_tile(uint32_t t_s, uint32_t t_o, float s
   uint32_t r0[32], r1[32], r2[32], r3[32];
   tmem_ld32(t_s, r0);
   tmem_ld32(t_s + 32, r1);
+  tmem_ld_wait();
   tmem_ld32(t_s + 64, r2);
   tmem_ld32(t_s + 96, r3);
-  tmem_ld_wait();
   const float m0 = max32<TAIL>(r0, 0, valid, -INFINITY), m1 = max32<TAIL>(r1, 32, valid, -INFINITY);
+  tmem_ld_wait();
   const float m2 = max32<TAIL>(r2, 64, valid, -INFINITY), m3 = max32<TAIL>(r3, 96, valid, -INFINITY);
   const float now = max3_nan(max3_nan(m0, m1, m2), m3, m3) * scale;
   if (first) {
@@ -313,11 +314,11 @@ __device__ __forceinline__ void softmax_tile(uint32_t t_s, uint32_t t_o, float s
   tmem_st16(t_s, w);
   exp32<T, TAIL>(r1, 32, valid, scale2, minus_top, sums, w);
   tmem_st16(t_s + 16, w);
-  tmem_st_wait();
+  exp32<T, TAIL>(r2, 64, valid, scale2, minus_top, sums, w);
+  tmem_st_wait();  // (of the first 64, long done by now)
   tc_fence_before();
   __syncwarp();
   if ((threadIdx.x & 31) == 0) mbar_arrive(half_ready);
-  exp32<T, TAIL>(r2, 64, valid, scale2, minus_top, sums, w);
   tmem_st16(t_s + 32, w);
   exp32<T, TAIL>(r3, 96, valid, scale2, minus_top, sums, w);
   tmem_st16(t_s + 48, w);
@@ -819,7 +820,7 @@ __global__ void __launch_bounds__(WPU > 1 ? 32 * WPU : 128, WPU > 1 ? 1 : DP == 
       for (int d = 4; d < 32; d <<= 1) sum[e] += __shfl_xor_sync(0xffffffffu, sum[e], d);
 
     // the prefix's parts (each lane its own columns' values; a part's maximum and sum are read by eight lanes)
-#pragma unroll 2
+#pragma unroll(WPU > 1 ? 2 : 1)
     for (int i = wi; i < parts; i += WPU) {
       const int slot = p.plan.part_of(item, part0 + i, parts), row = row0 + g0 + 2 * quad;
 #pragma unroll
@@ -1049,9 +1050,10 @@ int run_as(const Params& a, void* workspace, cudaStream_t s) {
       ANNC_CUDA(launch_pdl(cut_items_kernel<T, DP>, dim3((unsigned)p.plan.ctas - 1, kPartRows / 32), dim3(256), 0, s, j));
     return ANNC_OK;
   }
-  // A unit of work fills a warp, with small groups several tokens' of them; with few units (latency) eight warps share
-  // one token.
-  if (a.tokens * a.kv_heads < 1184) return launch_join<T, DP, 8>(j, s);
+  // A unit of work fills a warp, with small groups several tokens' of them; with few units (latency) four or eight
+  // warps share one token.
+  if (a.tokens * a.kv_heads <= 148) return launch_join<T, DP, 8>(j, s);
+  if (a.tokens * a.kv_heads < 1184) return launch_join<T, DP, 4>(j, s);
   j.tokens = a.group < 8 ? 8 / a.group : 1;
   return launch_join<T, DP, 1>(j, s);
 }
