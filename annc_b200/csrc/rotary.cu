@@ -13,6 +13,7 @@
 #include <cstdint>
 
 #include "common.h"
+#include "pdl.cuh"
 
 namespace annc {
 namespace rotary {
@@ -30,8 +31,9 @@ struct Params {
   const double* freq;
   float size;
   int heads0, heads;  // of the first tensor, of both
-  int dim, rot, pos64, transposed, pass;  // pass: values behind rot_dim that have to be copied
+  int dim, rot, pos64, transposed, pass, pass_pieces;  // pass: values behind rot_dim that have to be copied
   int tokens_per_block;
+  uint32_t units_magic, heads_magic;
   long long tokens;
 };
 
@@ -55,17 +57,52 @@ struct Piece<4> { using type = uint32_t; };
 template <>
 struct Piece<2> { using type = uint16_t; };
 
-// V values make a piece.  A unit of work is, in the half layout, the two pieces that hold V pairs, interleaved the
-// one piece that holds V / 2 pairs (V = 1: two pieces of one value), behind rot_dim a piece that is copied.
+// i / d by one multiplication where i * d stays below 2^32 (magic = 2^32 / d rounded up), else (magic 0) by division.
+__device__ __forceinline__ int quotient(int i, int d, uint32_t magic) { return magic ? (int)__umulhi((uint32_t)i, magic) : i / d; }
+
+// V values make a piece.  A unit of work is the two pieces that hold V pairs (in the half layout pairs / 2 values apart,
+// interleaved adjacent), behind rot_dim two pieces that are copied, or one.  (Interleaved units of one piece, with three divisions
+// each, were bound by their instructions: 8191 tokens of 40 heads of 128 bf16 42 us.)
 template <typename T, int V, bool HALF>
 __global__ void __launch_bounds__(256) rotary_kernel(Params p) {
   using P = typename Piece<V * (int)sizeof(T)>::type;
   extern __shared__ float turns[];  // cosines [tokens][pairs], then sines
+  constexpr int U = 2;  // units of a thread in flight
   const int pairs = p.rot >> 1;
   const long long t0 = (long long)blockIdx.x * p.tokens_per_block;
   const int nt = (int)min((long long)p.tokens_per_block, p.tokens - t0);
   float* const cosines = turns;
   float* const sines = turns + p.tokens_per_block * pairs;
+  const int turned = pairs / V, units = turned + p.pass / (p.pass_pieces * V);
+  const int total = nt * p.heads * units, other = HALF ? pairs : V;  // from a unit's one piece to its other
+  P a[U], b[U];
+  T* out[U];
+  int pair[U];
+
+  auto load = [&](int i0) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + 256 * u;
+      out[u] = nullptr;
+      if (i >= total) continue;
+      const int th = quotient(i, units, p.units_magic), unit = i - th * units;
+      const int t = quotient(th, p.heads, p.heads_magic);
+      int h = th - t * p.heads;
+      const Heads& x = p.x[h >= p.heads0];
+      if (h >= p.heads0) h -= p.heads0;
+      const bool turn = unit < turned;
+      const int first = !turn ? p.rot + (unit - turned) * p.pass_pieces * V : (HALF ? V : 2 * V) * unit;
+      pair[u] = turn ? t * pairs + unit * V : -1;
+      const T* in = static_cast<const T*>(x.in) + (t0 + t) * x.in_token + h * x.in_head + first;
+      out[u] = static_cast<T*>(x.out) + (t0 + t) * x.out_token + h * x.out_head + first;
+      a[u] = *reinterpret_cast<const P*>(in);
+      if (turn || p.pass_pieces == 2) b[u] = *reinterpret_cast<const P*>(in + (turn ? other : V));
+    }
+  };
+  pdl_trigger();
+  pdl_wait();
+  load(threadIdx.x);  // (on their way while the sines are worked out)
+
   for (int i = threadIdx.x; i < nt * pairs; i += 256) {
     const int t = i / pairs;
     const double at = p.pos64 ? (double)static_cast<const int64_t*>(p.positions)[t0 + t]
@@ -79,41 +116,8 @@ __global__ void __launch_bounds__(256) rotary_kernel(Params p) {
   }
   __syncthreads();
 
-  constexpr bool TWO = HALF || V == 1;  // two pieces a unit
-  constexpr int PAIRS = TWO ? V : V / 2;
-  const int turned = pairs / PAIRS, units = turned + p.pass / V;
-  const int total = nt * p.heads * units;
-  constexpr int U = 2;
   for (int i0 = threadIdx.x; i0 < total; i0 += 256 * U) {
-    P a[U], b[U];
-    T* out[U];
-    int pair[U], other[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int i = i0 + 256 * u;
-      out[u] = nullptr;
-      if (i >= total) continue;
-      const int th = i / units, unit = i - th * units;
-      const int t = th / p.heads;
-      int h = th - t * p.heads;
-      const Heads& x = p.x[h >= p.heads0];
-      if (h >= p.heads0) h -= p.heads0;
-      const T* in = static_cast<const T*>(x.in) + (t0 + t) * x.in_token + h * x.in_head;
-      out[u] = static_cast<T*>(x.out) + (t0 + t) * x.out_token + h * x.out_head;
-      int first;
-      if (unit < turned) {
-        first = HALF ? unit * V : unit * 2 * PAIRS;
-        other[u] = HALF ? pairs : 1;  // from the one piece to the other
-        pair[u] = t * pairs + unit * PAIRS;
-      } else {
-        first = p.rot + (unit - turned) * V;
-        pair[u] = -1;
-      }
-      in += first;
-      out[u] += first;
-      a[u] = *reinterpret_cast<const P*>(in);
-      if (TWO && pair[u] >= 0) b[u] = *reinterpret_cast<const P*>(in + other[u]);
-    }
+    if (i0 != (int)threadIdx.x) load(i0);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       if (!out[u]) continue;
@@ -122,22 +126,25 @@ __global__ void __launch_bounds__(256) rotary_kernel(Params p) {
         const float* s = sines + pair[u];
         T* va = reinterpret_cast<T*>(&a[u]);
         T* vb = reinterpret_cast<T*>(&b[u]);
-        if (TWO) {
+        if (HALF || V == 1) {
 #pragma unroll
           for (int e = 0; e < V; ++e) {
             const float x = to_float(va[e]), y = to_float(vb[e]);
             from_float(x * c[e] - y * s[e], &va[e]);
             from_float(y * c[e] + x * s[e], &vb[e]);
           }
-          *reinterpret_cast<P*>(out[u] + other[u]) = b[u];
         } else {
 #pragma unroll
-          for (int e = 0; e < PAIRS; ++e) {
-            const float x = to_float(va[2 * e]), y = to_float(va[2 * e + (V > 1)]);
-            from_float(x * c[e] - y * s[e], &va[2 * e]);
-            from_float(y * c[e] + x * s[e], &va[2 * e + (V > 1)]);
+          for (int e = 0; e < V; ++e) {
+            T* const v = e < V / 2 ? va + 2 * e : vb + 2 * e - V;
+            const float x = to_float(v[0]), y = to_float(v[V > 1 ? 1 : 0]);
+            from_float(x * c[e] - y * s[e], &v[0]);
+            from_float(y * c[e] + x * s[e], &v[V > 1 ? 1 : 0]);
           }
         }
+        *reinterpret_cast<P*>(out[u] + other) = b[u];
+      } else if (p.pass_pieces == 2) {
+        *reinterpret_cast<P*>(out[u] + V) = b[u];
       }
       *reinterpret_cast<P*>(out[u]) = a[u];
     }
@@ -147,9 +154,8 @@ __global__ void __launch_bounds__(256) rotary_kernel(Params p) {
 // Largest piece that every address, stride and boundary inside a head allows, in values.
 template <typename T>
 int piece_values(const annc_rotary_desc& d, int pass) {
-  const int per_piece_pairs = d.layout == ANNC_ROTARY_HALF ? d.rot_dim / 2 : d.rot_dim;
   for (int v : {16 / (int)sizeof(T), 8 / (int)sizeof(T)}) {
-    bool ok = per_piece_pairs % v == 0 && (pass == 0 || (pass % v == 0 && d.rot_dim % v == 0));
+    bool ok = d.rot_dim / 2 % v == 0 && (pass == 0 || (pass % v == 0 && d.rot_dim % v == 0));
     for (const annc_rotary_heads& x : d.x) {
       if (x.heads == 0) continue;
       ok = ok && ((reinterpret_cast<uintptr_t>(x.in) | reinterpret_cast<uintptr_t>(x.out)) & (v * sizeof(T) - 1)) == 0 &&
@@ -182,6 +188,7 @@ int launch(const annc_rotary_desc& d, cudaStream_t s) {
   p.pass = in_place ? 0 : d.head_dim - d.rot_dim;
   p.tokens = d.tokens;
   const int v = piece_values<T>(d, p.pass);
+  p.pass_pieces = p.pass % (2 * v) == 0 ? 2 : 1;
   // Tokens of a block: about 2048 pieces of work, at most what 16 KB of sines hold, but first of all a grid that
   // fills the 148 SMs four times over.
   const long long per_token = (long long)p.heads * (d.head_dim / v);
@@ -190,23 +197,18 @@ int launch(const annc_rotary_desc& d, cudaStream_t s) {
   if (tb > d.tokens / 592) tb = d.tokens / 592;
   if (tb < 1) tb = 1;
   p.tokens_per_block = (int)tb;
+  const long long units = d.rot_dim / 2 / v + p.pass / (p.pass_pieces * v), total = tb * p.heads * units;
+  if (units > 1 && total * units < (1LL << 32)) p.units_magic = (uint32_t)(((1ULL << 32) + units - 1) / units);
+  if (p.heads > 1 && total * p.heads < (1LL << 32)) p.heads_magic = (uint32_t)(((1ULL << 32) + p.heads - 1) / p.heads);
   const long long blocks = (d.tokens + tb - 1) / tb;
   ANNC_REQUIRE(blocks <= 0x7fffffffLL, ANNC_ERR_UNSUPPORTED, "rotary: too many tokens");
   const size_t smem = (size_t)tb * d.rot_dim * sizeof(float);
   const bool half = d.layout == ANNC_ROTARY_HALF;
   constexpr int V16 = 16 / (int)sizeof(T), V8 = 8 / (int)sizeof(T);
-  const unsigned g = (unsigned)blocks;
-  if (v == V16) {
-    if (half) rotary_kernel<T, V16, true><<<g, 256, smem, s>>>(p);
-    else rotary_kernel<T, V16, false><<<g, 256, smem, s>>>(p);
-  } else if (v == V8) {
-    if (half) rotary_kernel<T, V8, true><<<g, 256, smem, s>>>(p);
-    else rotary_kernel<T, V8, false><<<g, 256, smem, s>>>(p);
-  } else {
-    if (half) rotary_kernel<T, 1, true><<<g, 256, smem, s>>>(p);
-    else rotary_kernel<T, 1, false><<<g, 256, smem, s>>>(p);
-  }
-  ANNC_CUDA(cudaGetLastError());
+  void (*const kernel)(Params) = v == V16 ? (half ? rotary_kernel<T, V16, true> : rotary_kernel<T, V16, false>)
+                               : v == V8  ? (half ? rotary_kernel<T, V8, true> : rotary_kernel<T, V8, false>)
+                                          : (half ? rotary_kernel<T, 1, true> : rotary_kernel<T, 1, false>);
+  ANNC_CUDA(launch_pdl(kernel, dim3((unsigned)blocks), dim3(256), smem, s, p));
   return ANNC_OK;
 }
 
