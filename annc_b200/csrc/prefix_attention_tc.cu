@@ -3,7 +3,9 @@
 //
 // Prefix kernel.  A CTA walks through its share of key tiles (plan_of in prefix_attention.h).  Per key tile of 128 keys and
 // tile of 128 rows:  S = Q K^T (tcgen05, operands in shared memory, S in tensor memory), softmax numerators P in
-// registers (a thread per row), P back to tensor memory over S as the operand of  O += P V  (V as it lies, N-major).
+// registers (a thread per row), P back to tensor memory as the operand of  O += P V  (V as it lies, N-major).  Heads of
+// more than 64 values leave P no place but over S, so the next S waits for that product; with up to 64 values P has
+// columns of its own and the next S is made while the exponentials are taken.
 // Two such chains run side by side so that one's products cover the other's exponentials: with more than 128 rows
 // in the item the two are its two row tiles, sharing the key tiles; else they take the key tiles in turn and are added
 // at the end of the segment, each reading the other's O from tensor memory.  The running maximum of a row only moves when a score passes it by more than 2^8 in the
@@ -52,9 +54,12 @@ template <int DP>
 struct Shape {
   static constexpr int kTile = kTileKeys * DP * 2;  // bytes of 128 rows: DP / 64 blocks of 128 bytes x 128
   static constexpr int kSlots = DP == 128 ? 5 : 9;
+  // Tensor memory: S of the chains at columns 0 and 128, then O, then P if it has room of its own.
+  static constexpr bool kOwnP = DP == 64;
+  static constexpr uint32_t kO = 256, kP = kOwnP ? 384 : 0, kPStep = kOwnP ? 64 : 128;
   static constexpr int kExchange = 2 * kTile + kSlots * kTile;  // the second chain's [128] (maximum, sum)
   static constexpr int kBars = kExchange + kTileRows * 8;
-  static constexpr size_t kSmem = 1024 + kBars + 256;
+  static constexpr size_t kSmem = 1024 + kBars + 320;
 };
 
 // The own keys that a token sees; row < 0: a token of no sequence.
@@ -278,8 +283,10 @@ __device__ __forceinline__ void exp32(const uint32_t (&r)[32], int first, int va
   }
 }
 template <typename T, int DP, bool TAIL>
-__device__ __forceinline__ void softmax_tile(uint32_t t_s, uint32_t t_o, float scale, bool first, int valid, float& top, float& sum,
-                                             uint32_t half_ready) {
+__device__ __forceinline__ bool softmax_tile(uint32_t t_s, uint32_t t_p, uint32_t t_o, float scale, bool first, int valid, float& top,
+                                             float& sum, uint32_t half_ready, uint32_t scores_read, uint32_t p_used, uint32_t p_phase,
+                                             volatile int* abort_flag, int* error_word) {
+  bool ok = true;
   uint32_t r0[32], r1[32], r2[32], r3[32];
   tmem_ld32(t_s, r0);
   tmem_ld32(t_s + 32, r1);
@@ -290,10 +297,17 @@ __device__ __forceinline__ void softmax_tile(uint32_t t_s, uint32_t t_o, float s
   tmem_ld_wait();
   const float m2 = max32<TAIL>(r2, 64, valid, -INFINITY), m3 = max32<TAIL>(r3, 96, valid, -INFINITY);
   const float now = max3_nan(max3_nan(m0, m1, m2), m3, m3) * scale;
+  if (Shape<DP>::kOwnP) {
+    tc_fence_before();
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) mbar_arrive(scores_read);
+    ok = all_wait(p_used, p_phase, abort_flag, error_word);  // the product before this one: it reads P and adds to O
+    tc_fence_after();
+  }
   if (first) {
     top = now;
   } else if (__any_sync(0xffffffffu, now > top + kSlack)) {
-    // (every product before this S is complete, O among them)
+    // (the products before this are complete)
     const float keep = now > top + kSlack ? exp2_approx(top - now) : 1.0f;
     if (now > top + kSlack) top = now;
     sum *= keep;
@@ -311,21 +325,22 @@ __device__ __forceinline__ void softmax_tile(uint32_t t_s, uint32_t t_o, float s
   const float2 scale2 = make_float2(scale, scale), minus_top = make_float2(-top, -top);
   uint32_t w[16];
   exp32<T, TAIL>(r0, 0, valid, scale2, minus_top, sums, w);
-  tmem_st16(t_s, w);
+  tmem_st16(t_p, w);
   exp32<T, TAIL>(r1, 32, valid, scale2, minus_top, sums, w);
-  tmem_st16(t_s + 16, w);
+  tmem_st16(t_p + 16, w);
   exp32<T, TAIL>(r2, 64, valid, scale2, minus_top, sums, w);
   tmem_st_wait();  // (of the first 64, long done by now)
   tc_fence_before();
   __syncwarp();
   if ((threadIdx.x & 31) == 0) mbar_arrive(half_ready);
-  tmem_st16(t_s + 32, w);
+  tmem_st16(t_p + 32, w);
   exp32<T, TAIL>(r3, 96, valid, scale2, minus_top, sums, w);
-  tmem_st16(t_s + 48, w);
+  tmem_st16(t_p + 48, w);
   sums[0] = add2(sums[0], sums[1]);
   sum = sums[0].x + sums[0].y;
   if (!(now < INFINITY)) sum = __uint_as_float(0x7fc00000u);  // a NaN or +inf among the scores makes the row one of NaN
   tmem_st_wait();
+  return ok;
 }
 
 template <typename T, int DP>
@@ -341,8 +356,8 @@ prefix_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
   const uint32_t bar_full = bars, bar_empty = bars + 8 * S::kSlots;
   const uint32_t bar_q = bars + 16 * S::kSlots, bar_qfree = bar_q + 8;
   const uint32_t bar_s = bar_q + 16, bar_p = bar_q + 32, bar_o = bar_q + 48, bar_ofree = bar_q + 64, bar_h = bar_q + 80;  // per chain
-  const uint32_t bar_x = bar_q + 96;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem_raw + (bar_q + 104 - raw));
+  const uint32_t bar_x = bar_q + 96, bar_read = bar_q + 104, bar_pv = bar_q + 120;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem_raw + (bar_q + 136 - raw));
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;  // (known to be uniform)
@@ -362,6 +377,8 @@ prefix_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
       mbar_init(bar_p + 8 * c, 4);
       mbar_init(bar_o + 8 * c, 1);
       mbar_init(bar_ofree + 8 * c, 4);
+      mbar_init(bar_read + 8 * c, 4);  // (P apart) S is in registers
+      mbar_init(bar_pv + 8 * c, 1);    // (P apart) P is used
     }
     mbar_init(bar_x, 4);
     *abort_flag = 0;
@@ -374,7 +391,7 @@ prefix_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;  // S and P of the chains at columns 0 and 128, O at 256 and 384
+  const uint32_t tmem = *tmem_slot;
   pdl_trigger();
   pdl_wait();
   const int total = p.plan.items * p.plan.kv_tiles;
@@ -442,7 +459,24 @@ prefix_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
             const int steps = g.steps(c);
-            const uint32_t t_s = tmem + 128 * c, t_o = tmem + 256 + 128 * c;
+            const uint32_t t_s = tmem + 128 * c, t_o = tmem + S::kO + DP * c, t_p = tmem + S::kP + S::kPStep * c;
+            auto scores = [&]() {  // S = Q K^T
+              const uint32_t i = n0 + 2 * (uint32_t)(g.key_tile(c, step) - g.first), s = i % S::kSlots;
+              ok = all_wait(bar_full + 8 * s, (i / S::kSlots) & 1u, abort_flag, p.error_word);
+              if (ok && S::kOwnP) ok = all_wait(bar_read + 8 * c, ((steps_done[c] + step) & 1u) ^ 1u, abort_flag, p.error_word);
+              if (!ok) return;
+              tc_fence_after();
+              const uint64_t k = k_desc + s * (S::kTile >> 4), q = q_desc + (g.dual ? c : 0) * (S::kTile >> 4);
+#pragma unroll
+              for (int kk = 0; kk < DP / 16; ++kk) {
+                const uint32_t off = ((kk / 4) * kBlock + (kk % 4) * 32) >> 4;
+                umma_f16_ss(t_s, q + off, k + off, idesc_s, kk > 0 ? 1u : 0u);
+              }
+              if (!g.dual || c == 1) umma_commit_elected(bar_empty + 8 * s);
+              umma_commit_elected(bar_s + 8 * c);
+            };
+            if (S::kOwnP && step < steps) scores();
+            if (!ok) break;
             if (step > 0 && step <= steps) {  // O += P V of the step before
               const uint32_t i = n0 + 2 * (uint32_t)(g.key_tile(c, step - 1) - g.first) + 1, s = i % S::kSlots;
               const uint32_t phase = (steps_done[c] + step - 1) & 1u;
@@ -456,26 +490,15 @@ prefix_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
                 tc_fence_after();
 #pragma unroll
                 for (int kk = 4 * half; kk < 4 * half + 4; ++kk)
-                  umma_f16_ts(t_o, t_s + 8 * kk, v + (kk * 2048 >> 4), idesc_o, step > 1 || kk > 0 ? 1u : 0u);
+                  umma_f16_ts(t_o, t_p + 8 * kk, v + (kk * 2048 >> 4), idesc_o, step > 1 || kk > 0 ? 1u : 0u);
               }
               if (!ok) break;
               if (!g.dual || c == 1) umma_commit_elected(bar_empty + 8 * s);
+              if (S::kOwnP) umma_commit_elected(bar_pv + 8 * c);
               if (step == steps) umma_commit_elected(bar_o + 8 * c);
             }
-            if (step < steps) {  // S = Q K^T
-              const uint32_t i = n0 + 2 * (uint32_t)(g.key_tile(c, step) - g.first), s = i % S::kSlots;
-              ok = all_wait(bar_full + 8 * s, (i / S::kSlots) & 1u, abort_flag, p.error_word);
-              if (!ok) break;
-              tc_fence_after();
-              const uint64_t k = k_desc + s * (S::kTile >> 4), q = q_desc + (g.dual ? c : 0) * (S::kTile >> 4);
-#pragma unroll
-              for (int kk = 0; kk < DP / 16; ++kk) {
-                const uint32_t off = ((kk / 4) * kBlock + (kk % 4) * 32) >> 4;
-                umma_f16_ss(t_s, q + off, k + off, idesc_s, kk > 0 ? 1u : 0u);
-              }
-              if (!g.dual || c == 1) umma_commit_elected(bar_empty + 8 * s);
-              umma_commit_elected(bar_s + 8 * c);
-            }
+            if (!S::kOwnP && step < steps) scores();
+            if (!ok) break;
           }
           if (step == most - 1 && ok) umma_commit_elected(bar_qfree);  // the segment's last use of its rows
         }
@@ -498,7 +521,7 @@ prefix_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
     const int c = warp >> 2, q = warp & 3;
     const int row = q * 32 + lane;  // of the tile
     const uint32_t lanes = (uint32_t)(q * 32) << 16;
-    const uint32_t t_s = tmem + 128 * c + lanes, t_o = tmem + 256 + 128 * c + lanes;
+    const uint32_t t_s = tmem + 128 * c + lanes, t_o = tmem + S::kO + DP * c + lanes, t_p = tmem + S::kP + S::kPStep * c + lanes;
     const float scale = p.scale2;
     uint32_t parts = 0, done = 0, joins = 0;  // segments with key tiles, steps, segments joined: of this chain so far
     for (int at = begin; at < end && ok;) {
@@ -517,11 +540,22 @@ prefix_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
           tc_fence_after();
           const int valid = p.prefix - g.key_tile(c, step) * kTileKeys;
           // (two copies of the code: selects for every value of every tile would be a third of its instructions)
-          if (valid >= kTileKeys) softmax_tile<T, DP, false>(t_s, t_o, scale, step == 0, valid, top, sum, bar_h + 8 * c);
-          else softmax_tile<T, DP, true>(t_s, t_o, scale, step == 0, valid, top, sum, bar_h + 8 * c);
+          const uint32_t p_phase = (done & 1u) ^ 1u;
+          if (valid >= kTileKeys)
+            ok = softmax_tile<T, DP, false>(t_s, t_p, t_o, scale, step == 0, valid, top, sum, bar_h + 8 * c, bar_read + 8 * c,
+                                            bar_pv + 8 * c, p_phase, abort_flag, p.error_word);
+          else
+            ok = softmax_tile<T, DP, true>(t_s, t_p, t_o, scale, step == 0, valid, top, sum, bar_h + 8 * c, bar_read + 8 * c,
+                                           bar_pv + 8 * c, p_phase, abort_flag, p.error_word);
+          if (!ok) break;
           tc_fence_before();
-        } else if (lane == 0) {
-          mbar_arrive(bar_h + 8 * c);
+        } else {
+          if (S::kOwnP) {  // (the waits are kept in step: a warp without rows must not run two phases ahead)
+            if (lane == 0) mbar_arrive(bar_read + 8 * c);
+            ok = all_wait(bar_pv + 8 * c, (done & 1u) ^ 1u, abort_flag, p.error_word);
+            if (!ok) break;
+          }
+          if (lane == 0) mbar_arrive(bar_h + 8 * c);
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(bar_p + 8 * c);
@@ -570,7 +604,7 @@ prefix_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
           weight *= inv;
           other *= inv;
         }
-        const uint32_t t_o1 = tmem + 384 + lanes;
+        const uint32_t t_o1 = tmem + S::kO + DP + lanes;
         for (int b = 0; b < DP / 32; ++b) {
           uint32_t o[32];
           float v[32];
