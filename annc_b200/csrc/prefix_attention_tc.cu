@@ -11,6 +11,11 @@
 // at the end of the segment, each reading the other's O from tensor memory.  The running maximum of a row only moves when a score passes it by more than 2^8 in the
 // exponential: until then O keeps its scale, the numerators grow to at most 256, and O is rescaled hardly ever.
 //
+// What bounds it: with 64 values the 16 exponentials a cycle of the SM (2048 of some 2560 cycles for two tiles of 128 x 128;
+// a half, a third, a quarter or a sixth of them on the multiply-add units by a polynomial: 212, 187, 181 and 188 us where
+// it is 184 without), with 128 values the way from P to the next S, which waits for two products (2048 cycles of
+// products in some 3700).  Sixteen softmax warps, two for a row, had 96 registers each and were slower (210 us for 134).
+//
 //   warps 0-3, 4-7   softmax of the two chains, rescaling of O, parts
 //   warp 8           TMA: rows, then keys and values through a ring of tiles
 //   warp 9           tensor memory, all products
@@ -47,7 +52,6 @@ using namespace annc::tc;
 
 constexpr int kThreads = 384;  // eight softmax warps, loads, products, and two that complete the group of four
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-constexpr int kPolyEvery = 4;  // of the pairs of exponentials, one in so many goes to the multiply-add units
 constexpr float kSlack = 8.0f;  // log2 of what a numerator may grow to before the maximum moves
 
 template <int DP>
@@ -187,26 +191,9 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
       : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
   return d;
 }
-// 2^x for x <= 8 on the multiply-add units, which have time left beside the 16 exponentials a cycle of the SM's special
-// ones: x = n + f with n the nearest whole number (read off the low bits of x + 1.5 * 2^23), 2^f by the polynomial of
-// degree four with the least relative error on [-1/2, 1/2] (2.6e-6, found by Remez exchange), n added to its exponent.
-// Below 2^-125 it stays there.  Not for a NaN, which comes out as some number.
-__device__ __forceinline__ float2 exp2_poly(float2 x) {
-  constexpr float kMagic = 12582912.0f;
-  x = make_float2(fmaxf(x.x, -125.0f), fmaxf(x.y, -125.0f));
-  const float2 t = add2(x, make_float2(kMagic, kMagic));
-  const float2 f = fma2(add2(t, make_float2(-kMagic, -kMagic)), make_float2(-1.0f, -1.0f), x);
-  float2 y = make_float2(0.009570101911f, 0.009570101911f);
-  y = fma2(y, f, make_float2(0.05591786032f, 0.05591786032f));
-  y = fma2(y, f, make_float2(0.2402474483f, 0.2402474483f));
-  y = fma2(y, f, make_float2(0.6931218147f, 0.6931218147f));
-  y = fma2(y, f, make_float2(0.9999992614f, 0.9999992614f));
-  return make_float2(__int_as_float(__float_as_int(y.x) + (__float_as_int(t.x) << 23)), __int_as_float(__float_as_int(y.y) + (__float_as_int(t.y) << 23)));
-}
-// The largest of three, a NaN if one is.
-__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+__device__ __forceinline__ float max3(float a, float b, float c) {
   float d;
-  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
 template <typename T>
@@ -263,9 +250,9 @@ __device__ __forceinline__ float max32(const uint32_t (&r)[32], int first, int v
     for (int i = 0; i < 4; ++i) {
       const float x = TAIL && first + j + i >= valid ? -INFINITY : __uint_as_float(r[j + i]);
       const float y = TAIL && first + j + 4 + i >= valid ? -INFINITY : __uint_as_float(r[j + 4 + i]);
-      m[i] = max3_nan(m[i], x, y);
+      m[i] = max3(m[i], x, y);
     }
-  return max3_nan(max3_nan(m[0], m[1], m[2]), m[3], m[3]);
+  return max3(max3(m[0], m[1], m[2]), m[3], m[3]);
 }
 template <typename T, bool TAIL>
 __device__ __forceinline__ void exp32(const uint32_t (&r)[32], int first, int valid, float2 scale, float2 minus_top, float2 (&sum)[2],
@@ -273,7 +260,7 @@ __device__ __forceinline__ void exp32(const uint32_t (&r)[32], int first, int va
 #pragma unroll
   for (int j = 0; j < 32; j += 2) {
     const float2 x = fma2(make_float2(__uint_as_float(r[j]), __uint_as_float(r[j + 1])), scale, minus_top);
-    float2 e = j / 2 % kPolyEvery == kPolyEvery - 1 ? exp2_poly(x) : make_float2(exp2_approx(x.x), exp2_approx(x.y));
+    float2 e = make_float2(exp2_approx(x.x), exp2_approx(x.y));
     if (TAIL) {
       if (first + j >= valid) e.x = 0.0f;
       if (first + j + 1 >= valid) e.y = 0.0f;
@@ -296,7 +283,7 @@ __device__ __forceinline__ bool softmax_tile(uint32_t t_s, uint32_t t_p, uint32_
   const float m0 = max32<TAIL>(r0, 0, valid, -INFINITY), m1 = max32<TAIL>(r1, 32, valid, -INFINITY);
   tmem_ld_wait();
   const float m2 = max32<TAIL>(r2, 64, valid, -INFINITY), m3 = max32<TAIL>(r3, 96, valid, -INFINITY);
-  const float now = max3_nan(max3_nan(m0, m1, m2), m3, m3) * scale;
+  const float now = max3(max3(m0, m1, m2), m3, m3) * scale;
   if (Shape<DP>::kOwnP) {
     tc_fence_before();
     __syncwarp();
@@ -338,7 +325,6 @@ __device__ __forceinline__ bool softmax_tile(uint32_t t_s, uint32_t t_p, uint32_
   tmem_st16(t_p + 48, w);
   sums[0] = add2(sums[0], sums[1]);
   sum = sums[0].x + sums[0].y;
-  if (!(now < INFINITY)) sum = __uint_as_float(0x7fc00000u);  // a NaN or +inf among the scores makes the row one of NaN
   tmem_st_wait();
   return ok;
 }
