@@ -25,7 +25,8 @@ __device__ __forceinline__ void from_float(float x, __half* y) { *y = __float2ha
 
 constexpr int kMaxDim = 256;
 
-// One warp a token and head, one key at a time, lanes along the head's values: takes every stride and head size.
+// One warp a token and head, lanes along the head's values, four keys at a time: takes every stride, head size, group and
+// scale, for the calls that the tensor-core kernels do not (tc_supported).
 template <typename T>
 __global__ void __launch_bounds__(128) attention_rows_kernel(Params p) {
   const int lane = threadIdx.x & 31;
@@ -36,7 +37,7 @@ __global__ void __launch_bounds__(128) attention_rows_kernel(Params p) {
   long long first;
   int count;
   if (!own_keys(p, token, &first, &count)) return;
-  constexpr int N = kMaxDim / 32;
+  constexpr int N = kMaxDim / 32, U = 4;
   float q[N], acc[N] = {}, top = -INFINITY, sum = 0.0f;
   const T* qp = static_cast<const T*>(p.q.data) + token * p.q.row + h * p.q.head;
 #pragma unroll
@@ -45,23 +46,45 @@ __global__ void __launch_bounds__(128) attention_rows_kernel(Params p) {
     const Rows& k = part ? p.ko : p.kp;
     const Rows& v = part ? p.vo : p.vp;
     const long long from = part ? first : 0, to = part ? first + count : p.prefix;
-    for (long long j = from; j < to; ++j) {
-      const T* kr = static_cast<const T*>(k.data) + j * k.row + g * k.head;
-      const T* vr = static_cast<const T*>(v.data) + j * v.row + g * v.head;
-      float s = 0.0f;
+    for (long long j = from; j < to; j += U) {
+      float s[U], w[U];
 #pragma unroll
-      for (int i = 0; i < N; ++i)
-        if (lane + 32 * i < p.dim) s = fmaf(q[i], to_float(kr[lane + 32 * i]), s);
+      for (int u = 0; u < U; ++u) {
+        s[u] = 0.0f;
+        if (j + u >= to) continue;
+        const T* kr = static_cast<const T*>(k.data) + (j + u) * k.row + g * k.head;
 #pragma unroll
-      for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
-      s *= p.scale;
-      const float now = fmaxf(top, s);
-      const float keep = top == now ? 1.0f : expf(top - now), w = expf(s - now);
+        for (int i = 0; i < N; ++i)
+          if (lane + 32 * i < p.dim) s[u] = fmaf(q[i], to_float(kr[lane + 32 * i]), s[u]);
+      }
+#pragma unroll
+      for (int d = 16; d > 0; d >>= 1)
+#pragma unroll
+        for (int u = 0; u < U; ++u) s[u] += __shfl_xor_sync(0xffffffffu, s[u], d);
+      float now = top;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        s[u] = j + u < to ? s[u] * p.scale : -INFINITY;
+        now = fmaxf(now, s[u]);
+      }
+      const float keep = top == now ? 1.0f : expf(top - now);
       top = now;
-      sum = sum * keep + w;
+      sum *= keep;
 #pragma unroll
-      for (int i = 0; i < N; ++i)
-        if (lane + 32 * i < p.dim) acc[i] = acc[i] * keep + w * to_float(vr[lane + 32 * i]);
+      for (int u = 0; u < U; ++u) {
+        w[u] = j + u < to ? expf(s[u] - now) : 0.0f;
+        sum += w[u];
+      }
+#pragma unroll
+      for (int i = 0; i < N; ++i) acc[i] *= keep;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (j + u >= to) continue;
+        const T* vr = static_cast<const T*>(v.data) + (j + u) * v.row + g * v.head;
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+          if (lane + 32 * i < p.dim) acc[i] = fmaf(w[u], to_float(vr[lane + 32 * i]), acc[i]);
+      }
     }
   }
   const bool none = p.prefix + count == 0;

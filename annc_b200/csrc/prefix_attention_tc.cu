@@ -687,6 +687,8 @@ __device__ __forceinline__ bool own_keys_of_warp(const Params& p, int token, int
   return true;
 }
 
+__device__ __forceinline__ void prefetch_l1(const void* at) { asm volatile("prefetch.global.L1 [%0];" ::"l"(at)); }
+
 struct JoinParams {
   Params a;
   Plan plan;
@@ -736,8 +738,15 @@ __global__ void __launch_bounds__(WPU > 1 ? 32 * WPU : 128, WPU > 1 ? 1 : DP == 
 #pragma unroll
   for (int e = 0; e < 2; ++e) of[e] = (2 * quad + e) / per_token;
 
+  long long own_first = -1;  // of token `lane`
+  int own_count = 0;
+  if (p.own && lane < tokens) {
+    const int4 own = *reinterpret_cast<const int4*>(p.own + token0 + lane);
+    own_first = (long long)own.y << 32 | (uint32_t)own.x;
+    own_count = own.z;
+  }
   for (int g0 = 0; g0 < a.group; g0 += 8) {
-    const int heads = p.tokens > 1 ? a.group : min(8, a.group - g0), columns = p.tokens > 1 ? tokens * a.group : heads;
+    const int columns = p.tokens > 1 ? tokens * a.group : min(8, a.group - g0);
     float o[2][NT];  // [column 2 quad + e][value dn * NT + i]
     float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.0f, 0.0f};
     bool valid[2] = {false, false};
@@ -746,15 +755,31 @@ __global__ void __launch_bounds__(WPU > 1 ? 32 * WPU : 128, WPU > 1 ? 1 : DP == 
 #pragma unroll
       for (int i = 0; i < NT; ++i) o[e][i] = 0.0f;
 
+    uint4 q[DP / 32];  // of column dn
+#pragma unroll
+    for (int b = 0; b < DP / 32; ++b) {
+      q[b] = make_uint4(0, 0, 0, 0);
+      if (dn < columns && 32 * b + 8 * quad < a.dim)
+        q[b] = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q.data) + (long long)(token0 + dn / per_token) * a.q.row +
+                                               ((long long)h * a.group + g0 + dn % per_token) * a.q.head + 32 * b + 8 * quad);
+    }
     for (int tt = 0; tt < tokens; ++tt) {
       const int token = token0 + tt;
       long long first;
       int count;
       if (p.own) {
-        const int4 own = *reinterpret_cast<const int4*>(p.own + token);
-        if (own.y < 0) continue;
-        first = (long long)own.y << 32 | (uint32_t)own.x;
-        count = own.z;
+        first = __shfl_sync(0xffffffffu, own_first, tt);
+        count = __shfl_sync(0xffffffffu, own_count, tt);
+        if (first < 0) continue;
+        // the next token's first keys are on their way meanwhile
+        const long long next = __shfl_sync(0xffffffffu, own_first, tt + 1);
+        const int there = __shfl_sync(0xffffffffu, own_count, tt + 1);
+        if (WPU == 1 && tt + 1 < tokens && (lane & 15) < there) {
+          const Rows& rows = lane < 16 ? a.ko : a.vo;
+          const T* at = static_cast<const T*>(rows.data) + (next + (lane & 15)) * rows.row + h * rows.head;
+          prefetch_l1(at);
+          if (DP == 128) prefetch_l1(at + 64);
+        }
       } else if (!own_keys_of_warp(a, token, lane, &first, &count)) {
         continue;
       }
@@ -765,15 +790,6 @@ __global__ void __launch_bounds__(WPU > 1 ? 32 * WPU : 128, WPU > 1 ? 1 : DP == 
         valid[e] = valid[e] || active[e];
       }
       if (count <= 16 * wi) continue;
-      uint4 q[DP / 32];
-#pragma unroll
-      for (int b = 0; b < DP / 32; ++b) {
-        const int g = dn - tt * per_token;  // column dn is a head of this token?
-        q[b] = make_uint4(0, 0, 0, 0);
-        if (g >= 0 && g < heads && 32 * b + 8 * quad < a.dim)
-          q[b] = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q.data) + (long long)token * a.q.row +
-                                                 ((long long)h * a.group + g0 + g) * a.q.head + 32 * b + 8 * quad);
-      }
       const T* const keys = static_cast<const T*>(a.ko.data) + first * a.ko.row + h * a.ko.head;
       const T* const values = static_cast<const T*>(a.vo.data) + first * a.vo.row + h * a.vo.head;
       for (int k0 = 16 * wi; k0 < count; k0 += 16 * WPU) {

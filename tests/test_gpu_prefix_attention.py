@@ -118,6 +118,33 @@ def test_batch_sizes(tokens, prefix):
     b.check()
 
 
+@pytest.mark.parametrize("heads,kv,dim,prefix", [(1, 1, 64, 200), (4, 2, 128, 300), (12, 4, 64, 70), (10, 2, 40, 129), (16, 2, 128, 40),
+                                                 (40, 1, 64, 500)])
+def test_many_tokens(heads, kv, dim, prefix):
+    # enough tokens that a warp of the joining kernel takes the heads of several (groups below eight)
+    tokens = 1400 // kv + 3
+    b = Batch([1] * tokens, [(i * 7) % 23 for i in range(tokens)], heads, kv, dim, prefix, seed=heads)
+    b.run()
+    b.check()
+
+
+def test_many_ragged_tokens():
+    nq = [1 + (i * 5) % 9 for i in range(300)] + [0, 40, 1]
+    b = Batch(nq, [(i * 11) % 30 for i in range(303)], 4, 2, 64, 260, F16, seed=2)
+    b.run()
+    b.check()
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("heads,kv,tokens,prefix", [(8, 8, 1, 5000), (8, 2, 3, 20000), (8, 2, 40, 9000), (8, 1, 300, 2500), (4, 4, 300, 700),
+                                                    (6, 2, 97, 3333), (4, 1, 5, 128), (2, 1, 700, 129), (96, 1, 4, 1500)])
+def test_without_own_keys(heads, kv, tokens, prefix, dim):
+    # items that one CTA has all of, and items that are cut between two, three or many
+    b = Batch([1] * tokens, [0] * tokens, heads, kv, dim, prefix, seed=tokens)
+    b.run(own=False)
+    b.check(own=False)
+
+
 @pytest.mark.parametrize("dtype", [BF16, F16])
 @pytest.mark.parametrize("prefix", [0, 1, 130, 513])
 def test_sequences_of_several_tokens(prefix, dtype):
@@ -202,6 +229,77 @@ def test_infinities_and_nans_reach_only_their_rows(dim):
     for t in range(200):
         for h in range(2):
             assert bool(finite[t, h]) == ((t, h) not in bad), (t, h)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_infinities_and_nans_of_other_tokens_keys(dim):
+    # tokens that share a warp, of sequences of one and of several tokens: what one may not see reaches it in no way
+    nq = [1, 1, 3, 1, 4, 2] * 130
+    b = Batch(nq, [3, 5, 6, 2, 4, 9] * 130, 2, 1, dim, 150, seed=4)
+    hidden = {}
+    starts = np.cumsum(b.nq) - b.nq
+    for s in range(0, len(nq), 13):
+        last = int(b.begin[s] + b.no[s] - 1)  # the own key that only the sequence's last token sees
+        (b.ko if s % 2 else b.vo)[last] = float("nan") if s % 3 else float("inf")
+        hidden[int(starts[s] + b.nq[s] - 1)] = True
+    b.run()
+    finite = torch.isfinite(b.out.float()).all(-1).all(-1).cpu().numpy()
+    assert [t for t in range(len(finite)) if not finite[t]] == sorted(hidden)
+
+
+def test_infinite_scores():
+    # a row all of whose scores are -inf, or that has one of +inf, is one of NaN, as the formula has it; others stay
+    for dim in (64, 128):
+        b = Batch([1] * 130, [0] * 130, 2, 1, dim, 300, F16, seed=6)
+        b.kp.fill_(0)
+        b.kp[:, 0, 0] = 60000.0
+        b.q.fill_(0)
+        b.q[3, 0, 0] = -60000.0
+        b.q[3, 1, 0] = 1.0
+        b.kp[200, 0, 0] = float("inf")
+        b.q[5, 0, 0] = 1.0
+        b.q[6, 0, 0] = -1.0
+        b.run(own=False, scale=1e35)  # scores of -3.6e44, 6e39 and +-inf
+        bad = ~torch.isfinite(b.out.float()).all(-1)
+        assert bool(bad[3].all()) and bool(bad[5, 0]) and bool(bad[6, 0])
+        # (zero queries meet the infinite key: 0 * inf)
+        assert bool(bad.all())
+        b.kp[200, 0, 0] = 0
+        b.run(own=False, scale=1e35)
+        bad = ~torch.isfinite(b.out.float()).all(-1)
+        assert sorted(map(tuple, bad.nonzero().tolist())) == [(3, 0), (3, 1), (5, 0), (6, 0)]
+
+
+def test_first_call_of_a_process_may_be_captured():
+    import subprocess
+    import sys
+    code = """
+import torch
+from annc_b200 import device as dev
+torch.cuda.init()
+x = torch.randn((40, 96), device="cuda")
+q, s, w, ws = dev.i8_rows(40, 96), torch.empty(40, device="cuda"), dev.i8_rows(64, 96).fill_(1), torch.ones(64, device="cuda")
+c = torch.empty((40, 64), dtype=torch.bfloat16, device="cuda")
+rot, plan = dev.Rotary(32), dev.PrefixAttention(2, 1, 32, 40)
+kv, out, pos = torch.randn((70, 1, 32), device="cuda").bfloat16(), torch.empty((40, 2, 32), dtype=torch.bfloat16, device="cuda"), torch.arange(40, device="cuda")
+def calls():
+    dev.quantize_rows(x, q, s)
+    dev.gemm_i8(q, s, w, ws, c)
+    rot.run(pos, c.view(40, 2, 32), c.view(40, 2, 32))
+    plan.run(c.view(40, 2, 32), kv, kv, out)
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    calls()
+graph.replay()
+got = out.clone()
+calls()
+assert torch.equal(got, out) and bool(torch.isfinite(out.float()).all())
+print("fine")
+"""
+    import os
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "fine" in r.stdout, r.stderr[-2000:]
 
 
 def test_strided_operands():
