@@ -15,8 +15,8 @@
 // a half, a third, a quarter or a sixth of them on the multiply-add units by a polynomial: 212, 187, 181 and 188 us where
 // it is 184 without), with 128 values the way from P to the next S, which waits for two products (2048 cycles of
 // products in some 3700).  Sixteen softmax warps, two for a row, had 96 registers each and were slower (210 us for 134), and so
-were half tiles of 64 keys with two places for S, which need no wait (161 us): half of a softmax step's time does not
-depend on the number of keys.
+// were half tiles of 64 keys with two places for S, which need no wait (161 us): half of a softmax step's time does not
+// depend on the number of keys.
 //
 //   warps 0-3, 4-7   softmax of the two chains, rescaling of O, parts
 //   warp 8           TMA: rows, then keys and values through a ring of tiles
