@@ -8,8 +8,9 @@
 // columns of its own and the next S is made while the exponentials are taken.
 // Two such chains run side by side so that one's products cover the other's exponentials: with more than 128 rows
 // in the item the two are its two row tiles, sharing the key tiles; else they take the key tiles in turn and are added
-// at the end of the segment, each reading the other's O from tensor memory.  The running maximum of a row only moves when a score passes it by more than 2^8 in the
-// exponential: until then O keeps its scale, the numerators grow to at most 256, and O is rescaled hardly ever.
+// at the end of the segment, the first one reading the other's O from tensor memory.  The running maximum of a row only
+// moves when a score passes it by more than 2^8 in the exponential: until then O keeps its scale, the numerators grow to
+// at most 256, and O is rescaled hardly ever.
 //
 // What bounds it: with 64 values the 16 exponentials a cycle of the SM (2048 of some 2560 cycles for two tiles of 128 x 128;
 // a half, a third, a quarter or a sixth of them on the multiply-add units by a polynomial: 212, 187, 181 and 188 us where
