@@ -153,13 +153,13 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(QuantParams p) {
 
   auto store = [&](int piece, const T (&v)[V]) {
     Guess g[V];
-    bool doubt = false;
+    float worst = 0.0f;
 #pragma unroll
     for (int e = 0; e < V; ++e) {
       g[e] = guess_of(to_float(v[e]), s.scale, s.inv);
-      doubt = doubt || !(fabsf(g[e].rem) < half);
+      worst = fmaxf(worst, fabsf(g[e].rem));
     }
-    if (doubt) {  // hardly ever: a quotient next to a half, or a row that is not finite
+    if (!(worst < half)) {  // hardly ever: a quotient next to a half, or a row that is not finite (half is NaN then)
 #pragma unroll
       for (int e = 0; e < V; ++e) g[e].sum = s.finite ? settled(g[e], half) : 0.0f;
     }
