@@ -59,7 +59,8 @@ inline Plan plan_of(long long tokens, int kv_heads, int group, long long prefix)
   p.kv_tiles = (int)((prefix + kTileKeys - 1) / kTileKeys);
   const long long total = (long long)p.items * p.kv_tiles;
   long long per = (total + kMaxCtas - 1) / kMaxCtas;
-  if (per < 2) per = 2;  // (two key tiles of a small item run side by side)
+  if (per < 2 && p.kv_tiles > 1) per = 2;  // (two key tiles of a small item run side by side)
+  if (per < 1) per = 1;
   p.per_cta = (int)per;
   p.ctas = (int)((total + per - 1) / per);
   return p;

@@ -75,6 +75,14 @@ struct Own {
   int count, reserved;
 };
 
+// Whether the join kernel takes the prefix too, and there is no prefix kernel: always up to 64 keys, further with few
+// (token, key head).  us with / without the prefix kernel: 500 ragged sequences, 8 heads of 64, 64 keys 30 / 27, 100 30 /
+// 32; 2048 tokens, 2 key heads of 128, 64 keys 35 / 32, 100 35 / 43; 64 tokens, 8 key heads, 128 keys 18 / 14, 200 16 / 18;
+// one token, 8 heads, 256 keys 9.7 / 6.0, 400 10.2 / 8.0.
+inline bool is_short(long long prefix, long long units) {
+  return prefix <= 64 || (units <= 512 && prefix <= 128) || (units <= 64 && prefix <= 320);
+}
+
 struct PrefixParams {
   Plan plan;
   Params a;
@@ -696,7 +704,8 @@ struct JoinParams {
   Params a;
   Plan plan;
   float scale2;
-  int tokens;  // of a unit of work
+  int short_prefix;  // keys of a prefix that is taken here, like own keys; else 0
+  int tokens;        // of a unit of work
   const float4* parts;
   const float2* stats;
   const Own* own;
@@ -709,7 +718,8 @@ struct JoinParams {
 // values dn * DP/8 + 2 t and + 2 t + 1, so that it ends with DP/8 adjacent values of columns 2 (lane % 4) and + 1, onto which
 // the parts of the prefix are added in place.  Tokens take their own keys one after the other, and only their columns
 // take what a product gives: what another token's values hold (infinities, NaN) reaches no other.
-template <typename T, int DP, int WPU>
+// SHORT: the whole prefix is taken here (in a kernel of its own: the registers that this takes cost the other one 3 to 10 us).
+template <typename T, int DP, int WPU, bool SHORT>
 __global__ void __launch_bounds__(WPU > 1 ? 32 * WPU : 128, WPU > 1 ? 1 : DP == 128 ? 4 : 5) join_kernel(JoinParams p) {
   constexpr int NT = DP / 8;  // values a lane holds of a column
   extern __shared__ float join_smem[];  // (WPU > 1) per warp: 8 columns of DP, 8 x (maximum, sum)
@@ -743,7 +753,7 @@ __global__ void __launch_bounds__(WPU > 1 ? 32 * WPU : 128, WPU > 1 ? 1 : DP == 
 
   long long own_first = -1;  // of token `lane`
   int own_count = 0;
-  if (p.own && lane < tokens) {
+  if (!SHORT && p.own && lane < tokens) {
     const int4 own = *reinterpret_cast<const int4*>(p.own + token0 + lane);
     own_first = (long long)own.y << 32 | (uint32_t)own.x;
     own_count = own.z;
@@ -766,35 +776,40 @@ __global__ void __launch_bounds__(WPU > 1 ? 32 * WPU : 128, WPU > 1 ? 1 : DP == 
         q[b] = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q.data) + (long long)(token0 + dn / per_token) * a.q.row +
                                                ((long long)h * a.group + g0 + dn % per_token) * a.q.head + 32 * b + 8 * quad);
     }
-    for (int tt = 0; tt < tokens; ++tt) {
+    for (int tt = SHORT ? -1 : 0; tt < tokens; ++tt) {  // -1: a short prefix, which all columns see
       const int token = token0 + tt;
-      long long first;
-      int count;
-      if (p.own) {
-        first = __shfl_sync(0xffffffffu, own_first, tt);
-        count = __shfl_sync(0xffffffffu, own_count, tt);
-        if (first < 0) continue;
-        // the next token's first keys are on their way meanwhile
-        const long long next = __shfl_sync(0xffffffffu, own_first, tt + 1);
-        const int there = __shfl_sync(0xffffffffu, own_count, tt + 1);
-        if (WPU == 1 && tt + 1 < tokens && (lane & 15) < there) {
-          const Rows& rows = lane < 16 ? a.ko : a.vo;
-          const T* at = static_cast<const T*>(rows.data) + (next + (lane & 15)) * rows.row + h * rows.head;
-          prefetch_l1(at);
-          if (DP == 128) prefetch_l1(at + 64);
+      long long first = 0;
+      int count = p.short_prefix;
+      const bool own = !SHORT || tt >= 0;
+      if (own) {
+        if (!SHORT && p.own) {
+          first = __shfl_sync(0xffffffffu, own_first, tt);
+          count = __shfl_sync(0xffffffffu, own_count, tt);
+          if (first < 0) continue;
+          // the next token's first keys are on their way meanwhile
+          const long long next = __shfl_sync(0xffffffffu, own_first, tt + 1);
+          const int there = __shfl_sync(0xffffffffu, own_count, tt + 1);
+          if (WPU == 1 && tt + 1 < tokens && (lane & 15) < there) {
+            const Rows& rows = lane < 16 ? a.ko : a.vo;
+            const T* at = static_cast<const T*>(rows.data) + (next + (lane & 15)) * rows.row + h * rows.head;
+            prefetch_l1(at);
+            if (DP == 128) prefetch_l1(at + 64);
+          }
+        } else if (!own_keys_of_warp(a, token, lane, &first, &count)) {
+          continue;
         }
-      } else if (!own_keys_of_warp(a, token, lane, &first, &count)) {
-        continue;
       }
       bool active[2];
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        active[e] = of[e] == tt && 2 * quad + e < columns;
-        valid[e] = valid[e] || active[e];
+        active[e] = (!own || of[e] == tt) && 2 * quad + e < columns;
+        valid[e] = valid[e] || (own && active[e]);
       }
       if (count <= 16 * wi) continue;
-      const T* const keys = static_cast<const T*>(a.ko.data) + first * a.ko.row + h * a.ko.head;
-      const T* const values = static_cast<const T*>(a.vo.data) + first * a.vo.row + h * a.vo.head;
+      const Rows& key_rows = own ? a.ko : a.kp;
+      const Rows& value_rows = own ? a.vo : a.vp;
+      const T* const keys = static_cast<const T*>(key_rows.data) + first * key_rows.row + h * key_rows.head;
+      const T* const values = static_cast<const T*>(value_rows.data) + first * value_rows.row + h * value_rows.head;
       for (int k0 = 16 * wi; k0 < count; k0 += 16 * WPU) {
         uint4 k[2][DP / 32];  // keys dn, dn + 8
 #pragma unroll
@@ -803,7 +818,7 @@ __global__ void __launch_bounds__(WPU > 1 ? 32 * WPU : 128, WPU > 1 ? 1 : DP == 
           for (int b = 0; b < DP / 32; ++b) {
             k[r][b] = make_uint4(0, 0, 0, 0);
             if (k0 + dn + 8 * r < count && 32 * b + 8 * quad < a.dim)
-              k[r][b] = *reinterpret_cast<const uint4*>(keys + (k0 + dn + 8 * r) * a.ko.row + 32 * b + 8 * quad);
+              k[r][b] = *reinterpret_cast<const uint4*>(keys + (k0 + dn + 8 * r) * key_rows.row + 32 * b + 8 * quad);
           }
         uint4 v[4][NT / 8];  // keys 2 quad, 2 quad + 1, + 8, + 9 (on their way during the softmax)
 #pragma unroll
@@ -813,7 +828,7 @@ __global__ void __launch_bounds__(WPU > 1 ? 32 * WPU : 128, WPU > 1 ? 1 : DP == 
           for (int x = 0; x < NT / 8; ++x) {
             v[i][x] = make_uint4(0, 0, 0, 0);
             if (key < count && dn * NT + 8 * x < a.dim)
-              v[i][x] = *reinterpret_cast<const uint4*>(values + key * a.vo.row + dn * NT + 8 * x);
+              v[i][x] = *reinterpret_cast<const uint4*>(values + key * value_rows.row + dn * NT + 8 * x);
           }
         }
         float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // keys dn, dn, dn + 8, dn + 8; columns 2 quad, + 1
@@ -1054,16 +1069,18 @@ int launch_prefix(const Params& a, const PrefixParams& p, cudaStream_t s) {
 
 template <typename T, int DP, int WPU>
 int launch_join(const JoinParams& p, cudaStream_t s) {
+  void (*const kernel)(JoinParams) = p.short_prefix ? join_kernel<T, DP, WPU, true> : join_kernel<T, DP, WPU, false>;
   const long long units = (p.a.tokens + p.tokens - 1) / p.tokens * p.a.kv_heads, blocks = WPU > 1 ? units : (units + 3) / 4;  // (tc_supported: they fit 30 bits)
   const size_t smem = WPU > 1 ? WPU * (8 * DP + 16) * sizeof(float) : 0;
-  ANNC_CUDA(launch_pdl(join_kernel<T, DP, WPU>, dim3((unsigned)blocks), dim3(WPU > 1 ? 32 * WPU : 128), smem, s, p));
+  ANNC_CUDA(launch_pdl(kernel, dim3((unsigned)blocks), dim3(WPU > 1 ? 32 * WPU : 128), smem, s, p));
   return ANNC_OK;
 }
 
 template <typename T, int DP>
 int run_as(const Params& a, void* workspace, cudaStream_t s) {
   PrefixParams p = {};
-  p.plan = plan_of(a.tokens, a.kv_heads, a.group, a.prefix);
+  const bool short_prefix = is_short(a.prefix, a.tokens * a.kv_heads);
+  p.plan = plan_of(a.tokens, a.kv_heads, a.group, short_prefix ? 0 : a.prefix);
   p.tokens = a.tokens;
   p.kv_heads = a.kv_heads;
   p.group = a.group;
@@ -1074,7 +1091,7 @@ int run_as(const Params& a, void* workspace, cudaStream_t s) {
   p.a = a;
   p.parts = static_cast<float4*>(workspace);
   p.stats = reinterpret_cast<float2*>(p.parts + slots * kPartRows * (DP / 4));
-  p.own = a.prefix > 0 && (a.own_len || a.q_begin) ? reinterpret_cast<Own*>(p.stats + slots * kPartRows) : nullptr;
+  p.own = !short_prefix && (a.own_len || a.q_begin) ? reinterpret_cast<Own*>(p.stats + slots * kPartRows) : nullptr;
   p.error_word = gemm::gemm_error_word();
   if (!p.error_word) return fail(ANNC_ERR_CUDA, "the tensor-core error word is not addressable");
   p.direct = !a.own_len && !a.q_begin;
@@ -1082,18 +1099,22 @@ int run_as(const Params& a, void* workspace, cudaStream_t s) {
   p.out_row = a.out_row;
   p.out_head = a.out_head;
   p.lse = a.lse;
-  if (a.prefix > 0) ANNC_TRY((launch_prefix<T, DP>(a, p, s)));
-  JoinParams j{a, p.plan, p.scale2, 1, p.parts, p.stats, p.own};
-  if (p.direct && a.prefix > 0) {
+  if (!short_prefix) ANNC_TRY((launch_prefix<T, DP>(a, p, s)));
+  JoinParams j{a, p.plan, p.scale2, short_prefix ? (int)a.prefix : 0, 1, p.parts, p.stats, p.own};
+  if (p.direct && !short_prefix) {
     if (p.plan.ctas > 1 && p.plan.per_cta % p.plan.kv_tiles != 0)
       ANNC_CUDA(launch_pdl(cut_items_kernel<T, DP>, dim3((unsigned)p.plan.ctas - 1, kPartRows / 32), dim3(256), 0, s, j));
     return ANNC_OK;
   }
-  // A unit of work fills a warp, with small groups several tokens' of them; with few units (latency) four or eight
-  // warps share one token.
-  if (a.tokens * a.kv_heads <= 148) return launch_join<T, DP, 8>(j, s);
-  if (a.tokens * a.kv_heads < 1184) return launch_join<T, DP, 4>(j, s);
-  j.tokens = a.group < 8 ? 8 / a.group : 1;
+  // A unit of work fills a warp.  Small groups: several tokens' heads, if that leaves eight warps for every SM.  Few units with
+  // something to do for more than one warp (chunks of own keys, going by the size of their buffer, and parts): four
+  // or eight warps for each.
+  const long long units = a.tokens * a.kv_heads;
+  const long long own = a.own_len && a.sequences > 0 ? a.own_rows / a.sequences : 0;
+  const long long chunks = (own + j.short_prefix + 15) / 16 + (short_prefix ? 0 : p.plan.kv_tiles / p.plan.per_cta + 1);
+  if (units <= 148 && chunks > 4) return launch_join<T, DP, 8>(j, s);
+  if (units < 1184 && chunks > 4) return launch_join<T, DP, 4>(j, s);
+  while (2 * j.tokens * a.group <= 8 && units / (2 * j.tokens) >= 148 * 8) j.tokens *= 2;
   return launch_join<T, DP, 1>(j, s);
 }
 

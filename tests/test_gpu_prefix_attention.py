@@ -88,7 +88,7 @@ class Batch:
 
 @pytest.mark.parametrize("dtype", [BF16, F16])
 @pytest.mark.parametrize("dim", [64, 128])
-@pytest.mark.parametrize("prefix", [1, 2, 63, 127, 128, 129, 255, 257, 1000])
+@pytest.mark.parametrize("prefix", [1, 2, 63, 127, 128, 129, 255, 257, 320, 321, 383, 384, 385, 511, 513, 640, 1000])
 def test_single_tokens(prefix, dim, dtype):
     b = Batch([1] * 5, [0, 1, 3, 17, 40], 8, 2, dim, prefix, dtype, seed=prefix)
     b.run()
@@ -96,16 +96,18 @@ def test_single_tokens(prefix, dim, dtype):
 
 
 @pytest.mark.parametrize("dim", [1, 7, 8, 16, 24, 32, 40, 72, 80, 96, 100, 120, 136, 192, 256])
-def test_head_sizes(dim):
-    b = Batch([1, 2, 3], [0, 2, 30], 4, 2, dim, 300, seed=dim)
+@pytest.mark.parametrize("prefix", [300, 700])
+def test_head_sizes(dim, prefix):
+    b = Batch([1, 2, 3], [0, 2, 30], 4, 2, dim, prefix, seed=dim)
     b.run()
     b.check()
 
 
 @pytest.mark.parametrize("heads,kv", [(1, 1), (8, 8), (3, 1), (5, 1), (6, 2), (7, 1), (12, 4), (32, 1), (64, 1), (40, 8), (96, 1),
                                       (128, 1), (130, 1), (300, 2)])
-def test_head_groups(heads, kv):
-    b = Batch([1] * 9, [4, 0, 9, 1, 2, 3, 5, 8, 13], heads, kv, 64, 200, seed=heads)
+@pytest.mark.parametrize("dim,prefix", [(64, 200), (64, 500), (128, 500)])
+def test_head_groups(heads, kv, dim, prefix):
+    b = Batch([1] * 9, [4, 0, 9, 1, 2, 3, 5, 8, 13], heads, kv, dim, prefix, seed=heads)
     b.run()
     b.check()
 
@@ -119,7 +121,7 @@ def test_batch_sizes(tokens, prefix):
 
 
 @pytest.mark.parametrize("heads,kv,dim,prefix", [(1, 1, 64, 200), (4, 2, 128, 300), (12, 4, 64, 70), (10, 2, 40, 129), (16, 2, 128, 40),
-                                                 (40, 1, 64, 500)])
+                                                 (40, 1, 64, 500), (2, 1, 64, 64), (3, 1, 128, 17)])
 def test_many_tokens(heads, kv, dim, prefix):
     # enough tokens that a warp of the joining kernel takes the heads of several (groups below eight)
     tokens = 1400 // kv + 3
@@ -146,7 +148,7 @@ def test_without_own_keys(heads, kv, tokens, prefix, dim):
 
 
 @pytest.mark.parametrize("dtype", [BF16, F16])
-@pytest.mark.parametrize("prefix", [0, 1, 130, 513])
+@pytest.mark.parametrize("prefix", [0, 1, 130, 513, 1025])
 def test_sequences_of_several_tokens(prefix, dtype):
     # no token, fewer own keys than tokens, as many, more; a long sequence
     nq = [1, 0, 3, 5, 2, 8, 1, 70, 0]
