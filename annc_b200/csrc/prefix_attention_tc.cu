@@ -873,27 +873,63 @@ __global__ void __launch_bounds__(WPU > 1 ? 32 * WPU : 128, WPU > 1 ? 1 : DP == 
 #pragma unroll
       for (int d = 4; d < 32; d <<= 1) sum[e] += __shfl_xor_sync(0xffffffffu, sum[e], d);
 
-    // the prefix's parts (each lane its own columns' values; a part's maximum and sum are read by eight lanes)
-#pragma unroll(WPU > 1 ? 2 : 1)
-    for (int i = wi; i < parts; i += WPU) {
-      const int slot = p.plan.part_of(item, part0 + i, parts), row = row0 + g0 + 2 * quad;
+    // the prefix's parts, each lane its own columns' values; a part's maximum and sum are read by eight lanes
+    auto fold = [&](int e, float2 st, const float4 (&v)[NT / 4]) {
+      const float now = fmaxf(top[e], st.x);
+      const float keep = sum[e] == 0.0f ? 0.0f : exp2_approx(top[e] - now), weight = exp2_approx(st.x - now);
+      top[e] = now;
+      sum[e] = sum[e] * keep + st.y * weight;
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        if (2 * quad + e >= columns) continue;
-        const float2 st = p.stats[(long long)slot * kPartRows + row + e];
-        float4 v[NT / 4];
+      for (int x = 0; x < NT / 4; ++x) {
+        o[e][4 * x] = o[e][4 * x] * keep + v[x].x * weight;
+        o[e][4 * x + 1] = o[e][4 * x + 1] * keep + v[x].y * weight;
+        o[e][4 * x + 2] = o[e][4 * x + 2] * keep + v[x].z * weight;
+        o[e][4 * x + 3] = o[e][4 * x + 3] * keep + v[x].w * weight;
+      }
+    };
+    const int row = row0 + g0 + 2 * quad;
+    const auto stats_of = [&](int slot, int e) { return p.stats[(long long)slot * kPartRows + row + e]; };
+    const auto value_of = [&](int slot, int e, int x) { return p.parts[((long long)slot * (DP / 4) + dn * (NT / 4) + x) * kPartRows + row + e]; };
+    if constexpr (WPU == 1) {
+#pragma unroll 1
+      for (int i = 0; i < parts; ++i) {
+        const int slot = p.plan.part_of(item, part0 + i, parts);
 #pragma unroll
-        for (int x = 0; x < NT / 4; ++x) v[x] = p.parts[((long long)slot * (DP / 4) + dn * (NT / 4) + x) * kPartRows + row + e];
-        const float now = fmaxf(top[e], st.x);
-        const float keep = sum[e] == 0.0f ? 0.0f : exp2_approx(top[e] - now), weight = exp2_approx(st.x - now);
-        top[e] = now;
-        sum[e] = sum[e] * keep + st.y * weight;
+        for (int e = 0; e < 2; ++e) {
+          if (2 * quad + e >= columns) continue;
+          const float2 st = stats_of(slot, e);
+          float4 v[NT / 4];
 #pragma unroll
-        for (int x = 0; x < NT / 4; ++x) {
-          o[e][4 * x] = o[e][4 * x] * keep + v[x].x * weight;
-          o[e][4 * x + 1] = o[e][4 * x + 1] * keep + v[x].y * weight;
-          o[e][4 * x + 2] = o[e][4 * x + 2] * keep + v[x].z * weight;
-          o[e][4 * x + 3] = o[e][4 * x + 3] * keep + v[x].w * weight;
+          for (int x = 0; x < NT / 4; ++x) v[x] = value_of(slot, e, x);
+          fold(e, st, v);
+        }
+      }
+    } else {
+      // Few units with many parts wait for memory: two parts' loads go out together (371 rows of 3 heads over 10450
+      // keys: 32.4 us, one part at a time 34.2). With one warp to a unit there are other warps to run meanwhile, and
+      // the second part's registers cost more than they bring (4096 rows of 16 heads over 2048 keys: 104 us, 94 so).
+#pragma unroll 1
+      for (int i = wi; i < parts; i += 2 * WPU) {
+        float2 st[2][2];
+        float4 v[2][2][NT / 4];
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          const int slot = p.plan.part_of(item, part0 + min(i + n * WPU, parts - 1), parts);
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            if (2 * quad + e >= columns) continue;
+            st[n][e] = stats_of(slot, e);
+#pragma unroll
+            for (int x = 0; x < NT / 4; ++x) v[n][e][x] = value_of(slot, e, x);
+          }
+        }
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          if (i + n * WPU >= parts) break;
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            if (2 * quad + e < columns) fold(e, st[n][e], v[n][e]);
+          }
         }
       }
     }
