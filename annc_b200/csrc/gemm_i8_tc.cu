@@ -90,6 +90,16 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
       : "r"(taddr)
       : "memory");
 }
+// 16 lanes x 32 columns; a thread gets, of each eight columns c = 8 g .., columns 2 (lane % 4) and the next of rows lane / 4
+// (r[4 g], r[4 g + 1]) and lane / 4 + 8 (r[4 g + 2], r[4 g + 3]).
+__device__ __forceinline__ void tmem_ld_16x256(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
 // D s32; A and B signed 8-bit, both K-major.
 __host__ __device__ constexpr uint32_t i8_idesc(int m, int n) {
   return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
@@ -447,65 +457,109 @@ gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
         }
       }
     } else {
-      // warp (q, half): tokens 32 q .. of this CTA's 128, channels 128 half ..; a lane is a token
+      // warp (q, half): tokens 32 q .. of this CTA's 128, channels 128 half ..  A lane takes two of each eight channels for
+      // four tokens, so that it needs 32 channels' scales and biases, not 128, and gets them by shuffles: with a token
+      // a lane the two shuffles a value bounded the epilogue.
       constexpr int COLS = 128 / (int)sizeof(T);  // channels of a chunk: 128 bytes of C
-      const int q = warp & 3, half = (warp - 2) >> 2;
+      const int q = warp & 3, half = (warp - 2) >> 2, quad = lane & 3, row = lane >> 2;
       uint8_t* const stg = gen_base + kPairStages * kPairStage + (warp - 2) * 4096;
+      // Of the warp's channels 8 G + 2 u + e this lane fetches u = quad, G = row and row + 8; tokens row + 8 h are its own.
+      struct Scales {
+        float sb[2][2], bias[2][2], sa[4];
+      };
+      auto fetch = [&](int tile) {
+        Scales f;
+        int m0, n0;
+        tile_coords(tiles, tile, &m0, &n0);
+        m0 += (int)rank * (kPairTile / 2) + q * 32;
+        n0 += half * (kPairTile / 2);
+#pragma unroll
+        for (int g = 0; g < 2; ++g)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int n = n0 + 8 * (row + 8 * g) + 2 * quad + e;
+            f.sb[g][e] = n < p.n ? p.scale_b[n] : 0.0f;
+            f.bias[g][e] = n < p.n && p.bias ? p.bias[n] : 0.0f;
+          }
+#pragma unroll
+        for (int h = 0; h < 4; ++h) f.sa[h] = m0 + row + 8 * h < p.m ? p.scale_a[m0 + row + 8 * h] : 0.0f;
+        return f;
+      };
       uint32_t count = 0;
       bool ok = true;
+      Scales next = fetch(pair);  // (the grid has no more pairs than tiles)
       for (int tile = pair; tile < tiles.count && ok; tile += pairs, ++count) {
         int m0, n0;
         tile_coords(tiles, tile, &m0, &n0);
         m0 += (int)rank * (kPairTile / 2) + q * 32;
         n0 += half * (kPairTile / 2);
         const uint32_t acc = count & 1u;
-        // four channels a lane of the warp's 128, handed round by shuffles below
-        float sb[4], bias[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int n = n0 + 4 * lane + e;
-          sb[e] = n < p.n ? p.scale_b[n] : 0.0f;
-          bias[e] = n < p.n && p.bias ? p.bias[n] : 0.0f;
-        }
-        const float sa = m0 + lane < p.m ? p.scale_a[m0 + lane] : 0.0f;
+        const Scales at = next;
+        if (tile + pairs < tiles.count) next = fetch(tile + pairs);  // on their way under this tile
         ok = __all_sync(0xffffffffu, mbar_wait(bar_tfull + 8 * acc, (count >> 1) & 1u, abort_flag, error_word)) != 0;
         if (!ok) break;
         tc_fence_after();
         const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16) + acc * (uint32_t)kPairTile + half * (kPairTile / 2);
-        uint32_t r[32];
-        if (m0 < p.m && n0 < p.n) tmem_ld32(taddr, r);
+        uint32_t r[2][16];  // tokens 0 .. 15 and 16 .. 31 of the warp's
+        if (m0 < p.m && n0 < p.n) {
+          tmem_ld_16x256(taddr, r[0]);
+          tmem_ld_16x256(taddr + (16u << 16), r[1]);
+        }
 #pragma unroll 1
         for (int c0 = 0; c0 < kPairTile / 2; c0 += COLS) {
           if (m0 >= p.m || n0 + c0 >= p.n) break;  // warp-uniform
-          uint32_t words[32];  // the lane's 128 bytes
+          bool free_to_write = !TMA_STORE;
 #pragma unroll
-          for (int h = 0; h < COLS / 32; ++h) {
-            float v[32];
-            const int first = (c0 + 32 * h) / 4;
+          for (int x = 0; x < COLS / 32; ++x) {
+            const int first = c0 + 32 * x;
+            float v[32];  // [channel group g][token h][e]
             tmem_ld_wait();
 #pragma unroll
-            for (int j = 0; j < 32; ++j)
-              v[j] = scaled((int)r[j], sa, __shfl_sync(0xffffffffu, sb[j & 3], first + (j >> 2)),
-                            __shfl_sync(0xffffffffu, bias[j & 3], first + (j >> 2)));
-            // (channels behind n are products of zeros with a scale of zero)
-            if (c0 + 32 * h + 32 < kPairTile / 2) tmem_ld32(taddr + c0 + 32 * h + 32, r);
-            activate(p.act, v);
-            if (sizeof(T) == 4) {
+            for (int g = 0; g < 4; ++g) {
+              // group first / 8 + g: the same half of the warp's sixteen for all g
+              const int from = ((first / 8 + g) & 7) * 4 + quad;
+              float s2[2], b2[2];
 #pragma unroll
-              for (int j = 0; j < 32; ++j) words[j] = __float_as_uint(v[j]);
+              for (int e = 0; e < 2; ++e) {
+                s2[e] = __shfl_sync(0xffffffffu, first < 64 ? at.sb[0][e] : at.sb[1][e], from);
+                b2[e] = __shfl_sync(0xffffffffu, first < 64 ? at.bias[0][e] : at.bias[1][e], from);
+              }
+#pragma unroll
+              for (int h = 0; h < 4; ++h)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) v[8 * g + 2 * h + e] = scaled((int)r[h >> 1][4 * g + 2 * (h & 1) + e], at.sa[h], s2[e], b2[e]);
+            }
+            // (channels behind n are products of zeros with a scale of zero)
+            if (first + 32 < kPairTile / 2) {
+              tmem_ld_16x256(taddr + first + 32, r[0]);
+              tmem_ld_16x256(taddr + (16u << 16) + first + 32, r[1]);
+            }
+            activate(p.act, v);
+            if (!free_to_write) {
+              if (lane == 0) bulk_wait_read<0>();  // the chunk before has left the staging tile
+              __syncwarp();
+              free_to_write = true;
+            }
+            if (sizeof(T) == 4) {
+              // 8 bytes a lane; odd rows take group g ^ 2, so that the sixteen lanes of a store meet all banks
+#pragma unroll
+              for (int g = 0; g < 4; ++g)
+#pragma unroll
+                for (int h = 0; h < 4; ++h) {
+                  const bool odd = row & 1;
+                  const float lo = odd ? v[8 * (g ^ 2) + 2 * h] : v[8 * g + 2 * h], hi = odd ? v[8 * (g ^ 2) + 2 * h + 1] : v[8 * g + 2 * h + 1];
+                  const int piece = 2 * (g ^ (odd ? 2 : 0)) + (quad >> 1);
+                  *reinterpret_cast<float2*>(stg + (row + 8 * h) * 128 + ((piece ^ row) << 4) + (quad & 1) * 8) = make_float2(lo, hi);
+                }
             } else {
 #pragma unroll
-              for (int j = 0; j < 16; ++j) words[16 * h + j] = pack2<T>(v[2 * j], v[2 * j + 1]);
+              for (int g = 0; g < 4; ++g)
+#pragma unroll
+                for (int h = 0; h < 4; ++h)
+                  *reinterpret_cast<uint32_t*>(stg + (row + 8 * h) * 128 + (((4 * x + g) ^ row) << 4) + quad * 4) =
+                      pack2<T>(v[8 * g + 2 * h], v[8 * g + 2 * h + 1]);
             }
           }
-          if (TMA_STORE) {
-            if (lane == 0) bulk_wait_read<0>();  // the chunk before has left the staging tile
-            __syncwarp();
-          }
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-            *reinterpret_cast<uint4*>(stg + lane * 128 + ((j ^ (lane & 7)) << 4)) =
-                make_uint4(words[4 * j], words[4 * j + 1], words[4 * j + 2], words[4 * j + 3]);
           if (TMA_STORE) {
             fence_proxy_async();
             __syncwarp();
@@ -639,27 +693,30 @@ int launch_pair_as(const Params& p, int* error_word, cudaStream_t s) {
   ANNC_CUDA(cudaLaunchKernelEx(&cfg, kernel, ta, tb, tc, p, t, error_word));
   return ANNC_OK;
 }
+// (a TMA store clips at the tensor's edge in pieces of 16 bytes)
+bool pair_stores_by_tma(const Params& p) {
+  const int size = p.c_dtype == ANNC_F32 ? 4 : 2, piece = 16 / size;
+  return (reinterpret_cast<uintptr_t>(p.c) & 15) == 0 && p.ldc % piece == 0 && p.n % piece == 0 && p.ldc * (long long)size < (1LL << 40);
+}
 template <typename T>
 int launch_pair(const Params& p, int* error_word, cudaStream_t s) {
-  constexpr int kPiece = 16 / (int)sizeof(T);
-  // (a TMA store clips at the tensor's edge in pieces of 16 bytes)
-  const bool tma = (reinterpret_cast<uintptr_t>(p.c) & 15) == 0 && p.ldc % kPiece == 0 && p.n % kPiece == 0 &&
-                   p.ldc * (long long)sizeof(T) < (1LL << 40);
-  return tma ? launch_pair_as<T, true>(p, error_word, s) : launch_pair_as<T, false>(p, error_word, s);
+  return pair_stores_by_tma(p) ? launch_pair_as<T, true>(p, error_word, s) : launch_pair_as<T, false>(p, error_word, s);
 }
 
 }  // namespace
 
 // Which kernel and shape: the smallest of their times as these sums model them (us, bf16 output, figures fitted to
-// 45 products from 1 x 512 x 256 to 16384 x 8192 x 256; 148 SMs).
+// 64 products from 1 x 512 x 256 to 16384 x 8192 x 256; 148 SMs).
 //   split  2.4 for launch and prologue; per round of CTAs a k-step 0.165 + 0.00014 TN (latency: a CTA streams alone on
-//          its SM; 0.286 for 256 tokens, 48 KB) and, unsplit, 0.0098 TN to write the tile; split, once 0.6 + 0.022 TN
-//          for the sums of the cluster
-//   pair   6.1 for launch, prologue and the last tile's epilogue; a k-step 0.31, a tile at least the 3.3 that the
-//          epilogue under it takes
+//          its SM; 0.286 for 256 tokens, 48 KB) and, unsplit, 0.0098 TN to write the tile; 2.6 for each further round (its
+//          CTAs start, allocate tensor memory and fill their stages); split, once 0.6 + 0.022 TN for the sums of the
+//          cluster
+//   pair   2.9 for launch and prologue and the last tile's epilogue; a k-step 0.31, a tile at least what the epilogue under
+//          it takes, 3.0, and 5.2 if C's rows do not allow TMA
 // Measured, split kernel's best / pair: 1024 x 1024 x 1024 4.8 / 8.3, 512 x 4096 x 2048 7.2 / 10.8, 1024 x 4096 x 2048 10.2 /
 // 11.5, 2048 x 1024 x 8192 16.1 / 24.3, 4096 x 1024 x 8192 24.8 / 25.1, 700 x 8192 x 4096 28.1 / 25.6, 2048 x 4096 x 2048
-// 19.9 / 16.7, 8192 x 4096 x 2048 73 / 49.
+// 19.7 / 15.4, 16384 x 256 x 1024 7.8 / 8.3, 16384 x 512 x 1024 15.3 / 11.3, 16384 x 1024 x 64 21.7 / 15.3, 8192 x 4096 x 2048
+// 74 / 46.
 Route route_of(const Params& p) {
   Route best = {ROUTE_SIMT, 0, 0};
   // TMA wants rows on 16 bytes
@@ -669,7 +726,8 @@ Route route_of(const Params& p) {
   if (pair_tiles > (1LL << 30)) return best;
   const double main = 0.31 * kt;
   const long long pair_rounds = (pair_tiles + 73) / 74;
-  double us = 6.1 + main + (double)(pair_rounds - 1) * (main > 3.3 ? main : 3.3);
+  const double epilogue = pair_stores_by_tma(p) ? 3.0 : 5.2;
+  double us = 2.9 + epilogue + main + (double)(pair_rounds - 1) * (main > epilogue ? main : epilogue);
   best.kind = ROUTE_PAIR;
   for (int tn = 16; tn <= 256; tn *= 2) {
     const long long tiles = ((p.n + 127LL) / 128) * ((p.m + tn - 1LL) / tn);
@@ -679,7 +737,7 @@ Route route_of(const Params& p) {
       if (split > 1 && tiles > (split == 8 ? 15 : split == 4 ? 33 : 74)) break;
       const long long rounds = (tiles * split + 147) / 148;
       const double step = tn == 256 ? 0.286 : 0.165 + 0.00014 * tn;
-      const double t = 2.4 + (double)rounds * ((kt + split - 1) / split * step + (split == 1 ? 0.0098 * tn : 0.0)) +
+      const double t = 2.4 + (double)rounds * ((kt + split - 1) / split * step + (split == 1 ? 0.0098 * tn : 0.0)) + 2.6 * (double)(rounds - 1) +
                        (split > 1 ? 0.6 + 0.022 * tn : 0.0);
       if (t < us) {
         us = t;
