@@ -526,8 +526,8 @@ gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
               }
 #pragma unroll
               for (int h = 0; h < 4; ++h)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) v[8 * g + 2 * h + e] = scaled((int)r[h >> 1][4 * g + 2 * (h & 1) + e], at.sa[h], s2[e], b2[e]);
+                scaled2((int)r[h >> 1][4 * g + 2 * (h & 1)], (int)r[h >> 1][4 * g + 2 * (h & 1) + 1], at.sa[h], make_float2(s2[0], s2[1]),
+                        make_float2(b2[0], b2[1]), &v[8 * g + 2 * h], &v[8 * g + 2 * h + 1]);
             }
             // (channels behind n are products of zeros with a scale of zero)
             if (first + 32 < kPairTile / 2) {
