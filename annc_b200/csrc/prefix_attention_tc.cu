@@ -706,10 +706,18 @@ struct JoinParams {
   float scale2;
   int short_prefix;  // keys of a prefix that is taken here, like own keys; else 0
   int tokens;        // of a unit of work
+  uint32_t kv_heads_magic, item_magic, per_cta_magic;  // for quotient()
+  int per_token_magic;                                 // 64 / columns a token, rounded up: x / columns = x * it >> 6 for x < 8
   const float4* parts;
   const float2* stats;
   const Own* own;
 };
+
+// i / d by one multiplication where i * d stays below 2^32 (magic = 2^32 / d rounded up), else (magic 0) by division.
+inline uint32_t magic_of(int d, long long most) { return d > 1 && most * d < (1LL << 32) ? (uint32_t)(((1ULL << 32) + d - 1) / d) : 0u; }
+__device__ __forceinline__ int quotient(int i, int d, uint32_t magic) {
+  return magic ? (int)__umulhi((uint32_t)i, magic) : d == 1 ? i : i / d;
+}
 
 // WPU warps work on the eight columns of a product: eight heads of a (token, key head) at a time, or with smaller groups
 // the heads of p.tokens adjacent tokens.  S^T = K Q^T: keys are the 16 rows; a lane reads 16-byte pieces of two key
@@ -729,27 +737,28 @@ __global__ void __launch_bounds__(WPU > 1 ? 32 * WPU : 128, WPU > 1 ? 1 : DP == 
   const Params& a = p.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, wi = warp % WPU;
   const int quad = lane & 3, dn = lane >> 2;
-  // (32-bit arithmetic throughout: with 64-bit divisions the indexes took most of the kernel's time)
+  // (32-bit arithmetic by multiplication: with 64-bit divisions the indexes took most of the kernel's time, with 32-bit ones a tenth)
   const int unit = WPU > 1 ? (int)blockIdx.x : (int)blockIdx.x * 4 + warp;
-  const int slice = unit / a.kv_heads, h = unit - slice * a.kv_heads, token0 = slice * p.tokens;
+  const int slice = quotient(unit, a.kv_heads, p.kv_heads_magic), h = unit - slice * a.kv_heads, token0 = slice * p.tokens;
   if (token0 >= (int)a.tokens) return;
   const int tokens = min(p.tokens, (int)a.tokens - token0);
 
   // Where the rows lie in the parts of the prefix (a unit's tokens are in one tile).
   int part0 = 0, parts = 0, row0 = 0, item = 0;
   if (p.plan.kv_tiles > 0) {
-    const int tile = token0 / (2 * p.plan.tile_tokens), within = token0 - tile * 2 * p.plan.tile_tokens;
+    const int tile = quotient(token0, 2 * p.plan.tile_tokens, p.item_magic), within = token0 - tile * 2 * p.plan.tile_tokens;
     const int second = within >= p.plan.tile_tokens;
     item = h * p.plan.row_items + tile;
     const int from = item * p.plan.kv_tiles;
-    part0 = from / p.plan.per_cta;
-    parts = (from + p.plan.kv_tiles - 1) / p.plan.per_cta - part0 + 1;
+    part0 = quotient(from, p.plan.per_cta, p.per_cta_magic);
+    parts = quotient(from + p.plan.kv_tiles - 1, p.plan.per_cta, p.per_cta_magic) - part0 + 1;
     row0 = second * kTileRows + (within - second * p.plan.tile_tokens) * a.group;
   }
   const int per_token = p.tokens > 1 ? a.group : 8;  // columns
   int of[2];                                         // the token of this lane's columns
 #pragma unroll
-  for (int e = 0; e < 2; ++e) of[e] = (2 * quad + e) / per_token;
+  for (int e = 0; e < 2; ++e) of[e] = (2 * quad + e) * p.per_token_magic >> 6;
+  const int of_dn = dn * p.per_token_magic >> 6;
 
   long long own_first = -1;  // of token `lane`
   int own_count = 0;
@@ -773,9 +782,87 @@ __global__ void __launch_bounds__(WPU > 1 ? 32 * WPU : 128, WPU > 1 ? 1 : DP == 
     for (int b = 0; b < DP / 32; ++b) {
       q[b] = make_uint4(0, 0, 0, 0);
       if (dn < columns && 32 * b + 8 * quad < a.dim)
-        q[b] = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q.data) + (long long)(token0 + dn / per_token) * a.q.row +
-                                               ((long long)h * a.group + g0 + dn % per_token) * a.q.head + 32 * b + 8 * quad);
+        q[b] = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q.data) + (long long)(token0 + of_dn) * a.q.row +
+                                               ((long long)h * a.group + g0 + dn - of_dn * per_token) * a.q.head + 32 * b + 8 * quad);
     }
+    // The prefix's parts, each lane its own columns' values; a part's maximum and sum are read by eight lanes.  (First, so
+    // that their way from memory is under the own keys'.)
+    auto fold = [&](int e, float2 st, const float4 (&v)[NT / 4]) {
+      const float now = fmaxf(top[e], st.x);
+      const float keep = sum[e] == 0.0f ? 0.0f : exp2_approx(top[e] - now), weight = exp2_approx(st.x - now);
+      top[e] = now;
+      sum[e] = sum[e] * keep + st.y * weight;
+#pragma unroll
+      for (int x = 0; x < NT / 4; ++x) {
+        o[e][4 * x] = o[e][4 * x] * keep + v[x].x * weight;
+        o[e][4 * x + 1] = o[e][4 * x + 1] * keep + v[x].y * weight;
+        o[e][4 * x + 2] = o[e][4 * x + 2] * keep + v[x].z * weight;
+        o[e][4 * x + 3] = o[e][4 * x + 3] * keep + v[x].w * weight;
+      }
+    };
+    const int row = row0 + g0 + 2 * quad;
+    const auto stats_of = [&](int slot, int e) { return p.stats[(long long)slot * kPartRows + row + e]; };
+    const auto value_of = [&](int slot, int e, int x) { return p.parts[((long long)slot * (DP / 4) + dn * (NT / 4) + x) * kPartRows + row + e]; };
+    if constexpr (WPU == 1) {
+      if (parts > 0) {  // (most often the only one: straight to its place, the loads wait for the first use)
+        const int slot = p.plan.part_of(item, part0, parts);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          if (2 * quad + e >= columns) continue;
+          const float2 st = stats_of(slot, e);
+          top[e] = st.x;
+          sum[e] = st.y;
+#pragma unroll
+          for (int x = 0; x < NT / 4; ++x) {
+            const float4 v = value_of(slot, e, x);
+            o[e][4 * x] = v.x; o[e][4 * x + 1] = v.y; o[e][4 * x + 2] = v.z; o[e][4 * x + 3] = v.w;
+          }
+        }
+      }
+#pragma unroll 1
+      for (int i = 1; i < parts; ++i) {
+        const int slot = p.plan.part_of(item, part0 + i, parts);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          if (2 * quad + e >= columns) continue;
+          const float2 st = stats_of(slot, e);
+          float4 v[NT / 4];
+#pragma unroll
+          for (int x = 0; x < NT / 4; ++x) v[x] = value_of(slot, e, x);
+          fold(e, st, v);
+        }
+      }
+    } else {
+      // Few units with many parts wait for memory: two parts' loads go out together (371 rows of 3 heads over 10450
+      // keys: 32.4 us, one part at a time 34.2). With one warp to a unit there are other warps to run meanwhile, and
+      // the second part's registers cost more than they bring (4096 rows of 16 heads over 2048 keys: 104 us, 94 so).
+#pragma unroll 1
+      for (int i = wi; i < parts; i += 2 * WPU) {
+        float2 st[2][2];
+        float4 v[2][2][NT / 4];
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          const int slot = p.plan.part_of(item, part0 + min(i + n * WPU, parts - 1), parts);
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            if (2 * quad + e >= columns) continue;
+            st[n][e] = stats_of(slot, e);
+#pragma unroll
+            for (int x = 0; x < NT / 4; ++x) v[n][e][x] = value_of(slot, e, x);
+          }
+        }
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          if (i + n * WPU >= parts) break;
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            if (2 * quad + e < columns) fold(e, st[n][e], v[n][e]);
+          }
+        }
+      }
+    }
+    if (dn > 0) sum[0] = sum[1] = 0.0f;  // (from here on a column's sum is spread over the eight lanes)
+
     for (int tt = SHORT ? -1 : 0; tt < tokens; ++tt) {  // -1: a short prefix, which all columns see
       const int token = token0 + tt;
       long long first = 0;
@@ -872,67 +959,6 @@ __global__ void __launch_bounds__(WPU > 1 ? 32 * WPU : 128, WPU > 1 ? 1 : DP == 
     for (int e = 0; e < 2; ++e)
 #pragma unroll
       for (int d = 4; d < 32; d <<= 1) sum[e] += __shfl_xor_sync(0xffffffffu, sum[e], d);
-
-    // the prefix's parts, each lane its own columns' values; a part's maximum and sum are read by eight lanes
-    auto fold = [&](int e, float2 st, const float4 (&v)[NT / 4]) {
-      const float now = fmaxf(top[e], st.x);
-      const float keep = sum[e] == 0.0f ? 0.0f : exp2_approx(top[e] - now), weight = exp2_approx(st.x - now);
-      top[e] = now;
-      sum[e] = sum[e] * keep + st.y * weight;
-#pragma unroll
-      for (int x = 0; x < NT / 4; ++x) {
-        o[e][4 * x] = o[e][4 * x] * keep + v[x].x * weight;
-        o[e][4 * x + 1] = o[e][4 * x + 1] * keep + v[x].y * weight;
-        o[e][4 * x + 2] = o[e][4 * x + 2] * keep + v[x].z * weight;
-        o[e][4 * x + 3] = o[e][4 * x + 3] * keep + v[x].w * weight;
-      }
-    };
-    const int row = row0 + g0 + 2 * quad;
-    const auto stats_of = [&](int slot, int e) { return p.stats[(long long)slot * kPartRows + row + e]; };
-    const auto value_of = [&](int slot, int e, int x) { return p.parts[((long long)slot * (DP / 4) + dn * (NT / 4) + x) * kPartRows + row + e]; };
-    if constexpr (WPU == 1) {
-#pragma unroll 1
-      for (int i = 0; i < parts; ++i) {
-        const int slot = p.plan.part_of(item, part0 + i, parts);
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          if (2 * quad + e >= columns) continue;
-          const float2 st = stats_of(slot, e);
-          float4 v[NT / 4];
-#pragma unroll
-          for (int x = 0; x < NT / 4; ++x) v[x] = value_of(slot, e, x);
-          fold(e, st, v);
-        }
-      }
-    } else {
-      // Few units with many parts wait for memory: two parts' loads go out together (371 rows of 3 heads over 10450
-      // keys: 32.4 us, one part at a time 34.2). With one warp to a unit there are other warps to run meanwhile, and
-      // the second part's registers cost more than they bring (4096 rows of 16 heads over 2048 keys: 104 us, 94 so).
-#pragma unroll 1
-      for (int i = wi; i < parts; i += 2 * WPU) {
-        float2 st[2][2];
-        float4 v[2][2][NT / 4];
-#pragma unroll
-        for (int n = 0; n < 2; ++n) {
-          const int slot = p.plan.part_of(item, part0 + min(i + n * WPU, parts - 1), parts);
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            if (2 * quad + e >= columns) continue;
-            st[n][e] = stats_of(slot, e);
-#pragma unroll
-            for (int x = 0; x < NT / 4; ++x) v[n][e][x] = value_of(slot, e, x);
-          }
-        }
-#pragma unroll
-        for (int n = 0; n < 2; ++n) {
-          if (i + n * WPU >= parts) break;
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            if (2 * quad + e < columns) fold(e, st[n][e], v[n][e]);
-          }
-        }
-      }
-    }
 
     if (WPU > 1) {  // the warps' states, joined by the first one
       float* const mine = join_smem + warp * kWarp;
@@ -1104,7 +1130,12 @@ int launch_prefix(const Params& a, const PrefixParams& p, cudaStream_t s) {
 }
 
 template <typename T, int DP, int WPU>
-int launch_join(const JoinParams& p, cudaStream_t s) {
+int launch_join(JoinParams p, cudaStream_t s) {
+  p.kv_heads_magic = magic_of(p.a.kv_heads, p.a.tokens * p.a.kv_heads);
+  p.item_magic = magic_of(2 * p.plan.tile_tokens, p.a.tokens);
+  p.per_cta_magic = magic_of(p.plan.per_cta, (long long)p.plan.items * p.plan.kv_tiles);
+  const int per_token = p.tokens > 1 ? p.a.group : 8;
+  p.per_token_magic = (64 + per_token - 1) / per_token;
   void (*const kernel)(JoinParams) = p.short_prefix ? join_kernel<T, DP, WPU, true> : join_kernel<T, DP, WPU, false>;
   const long long units = (p.a.tokens + p.tokens - 1) / p.tokens * p.a.kv_heads, blocks = WPU > 1 ? units : (units + 3) / 4;  // (tc_supported: they fit 30 bits)
   const size_t smem = WPU > 1 ? WPU * (8 * DP + 16) * sizeof(float) : 0;
@@ -1136,7 +1167,15 @@ int run_as(const Params& a, void* workspace, cudaStream_t s) {
   p.out_head = a.out_head;
   p.lse = a.lse;
   if (!short_prefix) ANNC_TRY((launch_prefix<T, DP>(a, p, s)));
-  JoinParams j{a, p.plan, p.scale2, short_prefix ? (int)a.prefix : 0, 1, p.parts, p.stats, p.own};
+  JoinParams j = {};
+  j.a = a;
+  j.plan = p.plan;
+  j.scale2 = p.scale2;
+  j.short_prefix = short_prefix ? (int)a.prefix : 0;
+  j.tokens = 1;
+  j.parts = p.parts;
+  j.stats = p.stats;
+  j.own = p.own;
   if (p.direct && !short_prefix) {
     if (p.plan.ctas > 1 && p.plan.per_cta % p.plan.kv_tiles != 0)
       ANNC_CUDA(launch_pdl(cut_items_kernel<T, DP>, dim3((unsigned)p.plan.ctas - 1, kPartRows / 32), dim3(256), 0, s, j));
