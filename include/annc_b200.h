@@ -634,7 +634,8 @@ int annc_i8_weight_dev(const float* b_kn, int64_t ldb, int8_t* b_nk, int64_t ldq
                        int64_t k, int64_t n, void* stream);
 
 /* C[m,n] = act(sum_k A[m,k] B[n,k] * scale_a[m] * scale_b[n] + bias[n]).  The sums are exact
- * (32-bit integers; k up to 131071); scalings, bias and activation are f32, C is rounded once. */
+ * (32-bit integers; k up to 131071); scalings, bias and activation are f32, C is rounded once.  A
+ * bounded wait that ran out is reported by annc_gemm_check. */
 typedef struct annc_gemm_i8_desc {
   int64_t m, n, k;
   int64_t lda, ldb, ldc;
@@ -707,7 +708,10 @@ int annc_rotary_dev(const annc_rotary_desc* desc, void* stream);
  * own_len entries that reach outside 0 .. own_rows are clamped to it.
  * The prefix is read once for all tokens.  workspace: 16-byte aligned scratch of
  * annc_prefix_attention_workspace_bytes(tokens, heads, kv_heads, head_dim) bytes (for at most so
- * many tokens), one call at a time. */
+ * many tokens), one call at a time: calls that may overlap (two streams, two graphs) need one each.
+ * Head sizes that are multiples of 8 up to 128, rows and heads of all tensors on 16 bytes, at most
+ * 128 heads to a key head and scale >= 0 run on the tensor cores; other calls a row at a time, some
+ * ten times slower.  annc_gemm_check reports a bounded wait that ran out, as for the products. */
 typedef struct annc_prefix_attention_desc {
   int32_t dtype;                 /* ANNC_BF16 or ANNC_F16: q, keys, values, out */
   int32_t heads, kv_heads, head_dim; /* head_dim 1 .. 256 */
