@@ -705,7 +705,8 @@ int annc_rotary_dev(const annc_rotary_desc* desc, void* stream);
  * q_begin[s] .. q_begin[s+1] - 1 (ascending); without q_begin every token is a sequence.  Tokens
  * outside all sequences are left as they are in out and lse.  A token that sees no key gets zeros
  * and lse -inf; lse is the natural logarithm of the sum of exp(scale * q . k).  own_begin /
- * own_len entries that reach outside 0 .. own_rows are clamped to it.
+ * own_len entries that reach outside 0 .. own_rows are clamped to it.  out and lse must not overlap
+ * an input.
  * The prefix is read once for all tokens.  workspace: 16-byte aligned scratch of
  * annc_prefix_attention_workspace_bytes(tokens, heads, kv_heads, head_dim) bytes (for at most so
  * many tokens), one call at a time: calls that may overlap (two streams, two graphs) need one each.

@@ -154,6 +154,35 @@ def test_epilogues(m, n, k, act, dtype):
     check_product(a, sa, b, sb, None, act, dtype)
 
 
+@pytest.mark.parametrize("act", [ACT_NONE, ACT_RELU, ACT_SIGMOID])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m,n,k", [(16384, 264, 640), (6000, 1001, 2048), (9001, 520, 1100), (4099, 1192, 1024), (16200, 640, 32)])
+def test_tall_products(m, n, k, act, dtype):
+    # tiles of CTA pairs one after the other; tails of both sides; rows of C that TMA stores, and rows that it does not
+    a, sa, b, sb, bias = operands(m, n, k, 7)
+    assert device.gemm_i8_kernel_name(a, sa, b, sb, torch.empty((m, n), dtype=dtype, device="cuda")) == "tcgen05_pair_i8"
+    wide = torch.full((m + 2, n), 5.0, dtype=dtype, device="cuda")
+    check_product(a, sa, b, sb, bias if n % 16 else None, act, dtype, wide[:m])
+    assert bool((wide[m:] == 5.0).all())
+
+
+@pytest.mark.parametrize("n", [24, 264])
+def test_sigmoid_far_out(n):
+    # values from -110 to 110: zero only where the smallest normal number is not reached, one at the other end
+    m, k = 3000, 16
+    a, b = device.i8_rows(m, k), device.i8_rows(n, k)
+    a.zero_()
+    b.zero_()
+    bias = torch.linspace(-110, 110, n, device="cuda")
+    c = torch.empty((m, n), device="cuda")
+    device.gemm_i8(a, torch.ones(m, device="cuda"), b, torch.ones(n, device="cuda"), c, bias=bias, activation=ACT_SIGMOID)
+    want = torch.sigmoid(bias.double())
+    # the exponent's product rounds once (|x| 2^-24 of the power), its factor log2(e) is off by 0.23 2^-24; exp2, the sum and
+    # the reciprocal within 2 ulp each
+    tol = want * (bias.double().abs() * 1.25 * 2.0 ** -24 + 6 * 2.0 ** -23) + torch.finfo(torch.float32).tiny
+    assert bool(((c.double() - want).abs() <= tol).all())
+
+
 @pytest.mark.parametrize("m,n,k", [(1, 40, 131071), (200, 300, 70000)])
 def test_long_sums_are_exact(m, n, k):
     # all operands -128: the largest sum there is, 2^31 - 16384 at k = 131071

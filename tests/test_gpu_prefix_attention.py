@@ -4,6 +4,7 @@ Bound of an output value, with u = half a step of the type: the weights may be r
 the values (u each; f16 also loses up to 2^-25 of the row's largest weight where a small one is no longer normal),
 scores are off by delta = scale * sum|q||k| * (dim + 2) 2^-24, exponentials and joins of partial sums by 2^-18, and a
 sum of n positive terms in fp32 by n 2^-24 on either side of the quotient; the result is rounded once more (u)."""
+import copy
 import math
 
 import numpy as np
@@ -128,6 +129,32 @@ def test_many_tokens(heads, kv, dim, prefix):
     b = Batch([1] * tokens, [(i * 7) % 23 for i in range(tokens)], heads, kv, dim, prefix, seed=heads)
     b.run()
     b.check()
+
+
+def some_of(b, tokens):
+    """The given tokens (each a sequence) of a batch that has run, to be checked."""
+    c = copy.copy(b)
+    at = torch.as_tensor(tokens, device="cuda")
+    c.nq, c.no, c.begin = np.ones(len(tokens), np.int64), b.no[tokens], b.begin[tokens]
+    c.q, c.out, c.lse = b.q[at], b.out[at], b.lse[at]
+    return c
+
+
+@pytest.mark.parametrize("heads,kv", [(1, 1), (2, 1), (3, 1), (4, 1), (5, 1), (2, 2), (8, 4), (12, 4), (16, 2)])
+@pytest.mark.parametrize("dim,prefix", [(64, 40), (64, 129), (128, 700), (40, 300)])
+def test_warps_with_the_heads_of_several_tokens(heads, kv, dim, prefix):
+    tokens = 9700 // kv + 5
+    b = Batch([1] * tokens, [(i * 7) % 23 if i % 3 else 0 for i in range(tokens)], heads, kv, dim, prefix, seed=heads + dim)
+    b.run()
+    some_of(b, np.unique(np.concatenate([np.arange(12), np.arange(60, 68), np.arange(0, tokens, 311), tokens - 1 - np.arange(9)]))).check()
+
+
+def test_index_products_beyond_32_bits():
+    # tokens * key heads * key heads is 5.2e9
+    tokens, kv = 20000, 512
+    b = Batch([1] * tokens, [0] * tokens, kv, kv, 8, 3, seed=5)
+    b.run(own=False)
+    some_of(b, np.array([0, 1, 7, 8, 9999, 16383, 16384, 19998, 19999])).check(own=False)
 
 
 def test_many_ragged_tokens():
