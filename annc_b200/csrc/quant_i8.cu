@@ -90,6 +90,14 @@ __device__ __forceinline__ uint32_t top_bits(uint32_t top) {
   return __float_as_uint(to_float(v));
 }
 
+template <int BYTES>
+struct Words;
+template <>
+struct Words<16> { using type = uint4; };
+template <>
+struct Words<8> { using type = uint2; };
+template <>
+struct Words<4> { using type = uint32_t; };
 struct QuantParams {
   const void* x;
   long long ld;
@@ -98,17 +106,21 @@ struct QuantParams {
   float* scale;
   long long rows;
   int cols;
+  int unit;  // (QUADS) values of a load: 4, 2 or 1
 };
+// WIDE: rows of x are whole 16-byte pieces at 16-byte addresses.  QUADS: four values, loaded as x's addresses allow and
+// stored as a word (rows of q at 4-byte addresses); the last piece of a row may have fewer.  SINGLES: one value at a time.
+// us by quads / singles: 4730 x 2583 bf16 15.4 / 21.0, 1756 x 1121 f32 4.6 / 6.9, 15000 x 213 f16 7.3 / 6.6.
+enum Pieces { WIDE, QUADS, SINGLES };
 
 // TPR threads take a row; a thread keeps NV pieces of V values in registers between the maximum and the rounding, so
-// that a row of up to TPR * NV * V values is read once; what is longer is read again, from L2.  VEC: rows of whole 16-byte
-// pieces at 16-byte addresses; else one value at a time.  Bound by memory once the rounding takes few enough
-// instructions (8192 x 2048 bf16 31 us with rintf, a conversion and a branch for every value) and a thread has several
-// pieces on their way (65536 x 256 bf16, a warp a row, one piece a lane, 27 us).
-template <typename T, int TPR, bool VEC>
+// that a row of up to TPR * NV * V values is read once; what is longer is read again, from L2.  Bound by memory once the
+// rounding takes few enough instructions (8192 x 2048 bf16 31 us with rintf, a conversion and a branch for every value) and a
+// thread has several pieces on their way (65536 x 256 bf16, a warp a row, one piece a lane, 27 us).
+template <typename T, int TPR, Pieces KIND>
 __global__ void __launch_bounds__(256) quantize_rows_kernel(QuantParams p) {
-  constexpr int V = VEC ? 16 / (int)sizeof(T) : 1;
-  constexpr int NV = VEC ? 8 : 16;
+  constexpr int V = KIND == WIDE ? 16 / (int)sizeof(T) : KIND == QUADS ? 4 : 1;
+  constexpr int NV = KIND == SINGLES ? 16 : 8;
   const int t = threadIdx.x % TPR, lane = threadIdx.x & 31;
   const long long at_row = (long long)blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
   pdl_trigger();
@@ -117,12 +129,30 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(QuantParams p) {
   const long long row = there ? at_row : 0;
   const T* x = static_cast<const T*>(p.x) + row * p.ld;
   int8_t* q = p.q + row * p.ldq;
-  const int pieces = there ? p.cols / V : 0;
+  const int pieces = there ? (p.cols + V - 1) / V : 0;
 
   alignas(16) T keep[NV][V];
   auto load = [&](int piece, T (&to)[V]) {
-    if (VEC) *reinterpret_cast<uint4*>(to) = *(reinterpret_cast<const uint4*>(x) + piece);
-    else to[0] = x[piece];
+    if constexpr (KIND == WIDE) {
+      *reinterpret_cast<uint4*>(to) = *(reinterpret_cast<const uint4*>(x) + piece);
+    } else if constexpr (KIND == QUADS) {
+      using Four = typename Words<4 * sizeof(T)>::type;
+      using Two = typename Words<2 * sizeof(T)>::type;
+      if (4 * piece + 4 > p.cols) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) to[e] = 4 * piece + e < p.cols ? x[4 * piece + e] : T(0.0f);
+      } else if (p.unit == 4) {
+        *reinterpret_cast<Four*>(to) = *(reinterpret_cast<const Four*>(x) + piece);
+      } else if (p.unit == 2) {
+        reinterpret_cast<Two*>(to)[0] = reinterpret_cast<const Two*>(x)[2 * piece];
+        reinterpret_cast<Two*>(to)[1] = reinterpret_cast<const Two*>(x)[2 * piece + 1];
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) to[e] = x[4 * piece + e];
+      }
+    } else {
+      to[0] = x[piece];
+    }
   };
   uint32_t top = 0;
 #pragma unroll
@@ -173,7 +203,9 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(QuantParams p) {
         const uint32_t hi = __byte_perm(__float_as_uint(g[4 * j + 2].sum), __float_as_uint(g[4 * j + 3].sum), 0x0040);
         w[j] = __byte_perm(lo, hi, 0x5410);
       }
-      if (V == 8) *(reinterpret_cast<uint2*>(q) + piece) = make_uint2(w[0], w[V / 4 - 1]);
+      if (KIND == QUADS && 4 * piece + 4 > p.cols) {
+        for (int e = 0; 4 * piece + e < p.cols; ++e) q[4 * piece + e] = (int8_t)(w[0] >> (8 * e));
+      } else if (V == 8) *(reinterpret_cast<uint2*>(q) + piece) = make_uint2(w[0], w[V / 4 - 1]);
       else *(reinterpret_cast<uint32_t*>(q) + piece) = w[0];
     }
   };
@@ -281,20 +313,27 @@ int run_simt(const Params& p, cudaStream_t s) {
 }
 
 template <typename T>
-int launch_quantize(const QuantParams& p, cudaStream_t s) {
+int launch_quantize(QuantParams p, cudaStream_t s) {
   constexpr int V = 16 / (int)sizeof(T);
-  const bool vec = p.cols % V == 0 && p.ld % V == 0 && (reinterpret_cast<uintptr_t>(p.x) & 15) == 0 && p.ldq % V == 0 &&
-                   (reinterpret_cast<uintptr_t>(p.q) & (V - 1)) == 0;
-  const int pieces = p.cols / (vec ? V : 1), kept = vec ? 8 : 16;
-  // as few threads a row as hold it in registers, but two blocks an SM if the rows give them
+  if (p.rows == 1) p.ld = p.ldq = 0;  // (where a next row would be does not matter)
+  const bool wide = p.cols % V == 0 && p.ld % V == 0 && (reinterpret_cast<uintptr_t>(p.x) & 15) == 0 && p.ldq % V == 0 &&
+                    (reinterpret_cast<uintptr_t>(p.q) & (V - 1)) == 0;
+  const bool quads = !wide && p.ldq % 4 == 0 && (reinterpret_cast<uintptr_t>(p.q) & 3) == 0;
+  for (p.unit = 4; p.unit > 1 && (p.ld % p.unit || (reinterpret_cast<uintptr_t>(p.x) & (p.unit * sizeof(T) - 1))); p.unit /= 2) {
+  }
+  const int each = wide ? V : quads ? 4 : 1, pieces = (p.cols + each - 1) / each;
+  // As few threads a row as hold it in registers (eight pieces each, 16 singles), but two blocks an SM if the rows give them.
+  // 64 threads read up to half of a row again before 256 take it, which wait for one another: 8192 x 5120 bf16 33 / 43 us,
+  // 16384 x 8192 80 / 95, 2000 x 6000 11.6 / 10.8.  (16 threads that do so: 8192 x 2048 14.8 us, 64 threads 12.0.)
   int tpr = 4;
-  while (tpr < 256 && (pieces > kept * tpr || p.rows * tpr < 2 * 148 * 256)) tpr *= 4;
+  while (tpr < 256 && (pieces > (tpr == 64 || each == 1 ? 16 : 8) * tpr || p.rows * tpr < 2 * 148 * 256)) tpr *= 4;
   const long long blocks = (p.rows + 256 / tpr - 1) / (256 / tpr);
   ANNC_REQUIRE(blocks <= 0x7fffffffLL, ANNC_ERR_UNSUPPORTED, "quantize rows: too many rows");
-  static void (*const kernels[2][4])(QuantParams) = {
-      {quantize_rows_kernel<T, 4, false>, quantize_rows_kernel<T, 16, false>, quantize_rows_kernel<T, 64, false>, quantize_rows_kernel<T, 256, false>},
-      {quantize_rows_kernel<T, 4, true>, quantize_rows_kernel<T, 16, true>, quantize_rows_kernel<T, 64, true>, quantize_rows_kernel<T, 256, true>}};
-  ANNC_CUDA(launch_pdl(kernels[vec][tpr == 4 ? 0 : tpr == 16 ? 1 : tpr == 64 ? 2 : 3], dim3((unsigned)blocks), dim3(256), 0, s, p));
+  static void (*const kernels[3][4])(QuantParams) = {
+      {quantize_rows_kernel<T, 4, WIDE>, quantize_rows_kernel<T, 16, WIDE>, quantize_rows_kernel<T, 64, WIDE>, quantize_rows_kernel<T, 256, WIDE>},
+      {quantize_rows_kernel<T, 4, QUADS>, quantize_rows_kernel<T, 16, QUADS>, quantize_rows_kernel<T, 64, QUADS>, quantize_rows_kernel<T, 256, QUADS>},
+      {quantize_rows_kernel<T, 4, SINGLES>, quantize_rows_kernel<T, 16, SINGLES>, quantize_rows_kernel<T, 64, SINGLES>, quantize_rows_kernel<T, 256, SINGLES>}};
+  ANNC_CUDA(launch_pdl(kernels[wide ? WIDE : quads ? QUADS : SINGLES][tpr == 4 ? 0 : tpr == 16 ? 1 : tpr == 64 ? 2 : 3], dim3((unsigned)blocks), dim3(256), 0, s, p));
   return ANNC_OK;
 }
 

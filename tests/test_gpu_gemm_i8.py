@@ -63,6 +63,22 @@ def test_quantize_strided_and_odd_addresses(dtype):
     assert bool((q[:, 300:] == 99).all())  # what lies behind a row stays
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("pitch", [1100, 1102, 1101])
+def test_quantize_by_quads(dtype, pitch):
+    # every alignment of a row and every rest of four, in registers and read again, one row and many
+    big = torch.randn((40, pitch), device="cuda", generator=gen(pitch)).to(dtype)
+    for rows in (1, 40):
+        for cols in (1, 2, 3, 4, 5, 30, 255, 256, 257, 258, 1090):
+            for first in range(5):
+                q = torch.full((rows, 1104), 99, dtype=torch.int8, device="cuda")
+                check_quantize(big[:rows, first:first + cols], q[:, :cols])
+                assert bool((q[:, cols:] == 99).all())
+    wide = torch.randn((2, 33001), device="cuda", generator=gen(1)).to(dtype)
+    for first, cols in ((0, 33001), (1, 32999), (2, 32994)):
+        check_quantize(wide[:, first:first + cols])
+
+
 def test_quantize_at_the_borders_of_steps():
     # quotients next to a half: k + 1/2 steps and the fp32 neighbours of that, for steps that are not powers of two
     rows = []
