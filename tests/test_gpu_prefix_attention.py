@@ -157,6 +157,26 @@ def test_index_products_beyond_32_bits():
     some_of(b, np.array([0, 1, 7, 8, 9999, 16383, 16384, 19998, 19999])).check(own=False)
 
 
+@pytest.mark.parametrize("nq", [[3] + [0] * 70 + [1] * 50 + [0] * 33 + [40] + [0] * 31 + [2, 0, 1],
+                                [0] * 40 + [1] * 3 + [0, 0, 5] * 45 + [0] * 64, [31, 1, 32, 33, 0, 64, 7], [1] * 129 + [0] * 32 + [1] * 64,
+                                [0] * 2000 + [1] * 70 + [0] * 1100 + [2] * 30])
+def test_sequences_without_tokens(nq):
+    # runs of empty sequences around the 32 tokens and the 32 entries that a warp looks at together
+    b = Batch(nq, [(i * 13) % 29 for i in range(len(nq))], 2, 1, 64, 300, seed=len(nq))
+    b.run()
+    b.check()
+
+
+def test_tokens_before_the_first_sequence():
+    b = Batch([1] * 70 + [2] * 20, [(i * 13) % 29 for i in range(90)], 2, 1, 64, 300, seed=9)
+    b.q_begin[:41] = 40  # the first 40 tokens belong to no sequence, sequences 0 to 39 have none
+    b.run(ragged=True)
+    assert bool((b.out[:40] == 77).all()) and bool((b.lse[:40] == 77).all())
+    c = copy.copy(b)
+    c.nq, c.no, c.begin, c.q, c.out, c.lse = b.nq[40:], b.no[40:], b.begin[40:], b.q[40:], b.out[40:], b.lse[40:]
+    c.check()
+
+
 def test_many_ragged_tokens():
     nq = [1 + (i * 5) % 9 for i in range(300)] + [0, 40, 1]
     b = Batch(nq, [(i * 11) % 30 for i in range(303)], 4, 2, 64, 260, F16, seed=2)
