@@ -67,12 +67,13 @@ __global__ void __launch_bounds__(128) attention_rows_kernel(Params p) {
         s[u] = j + u < to ? s[u] * p.scale : -INFINITY;
         now = fmaxf(now, s[u]);
       }
-      const float keep = top == now ? 1.0f : expf(top - now);
+      const float base = now == -INFINITY ? 0.0f : now;  // (all scores so far are -inf: weights of 0, not of exp(-inf + inf))
+      const float keep = expf(top - base);
       top = now;
       sum *= keep;
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        w[u] = j + u < to ? expf(s[u] - now) : 0.0f;
+        w[u] = j + u < to ? expf(s[u] - base) : 0.0f;
         sum += w[u];
       }
 #pragma unroll

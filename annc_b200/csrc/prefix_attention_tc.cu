@@ -183,6 +183,9 @@ __device__ __forceinline__ float exp2_approx(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// What is subtracted from scores whose maximum is `top`: nothing where all of them are -inf, so that their
+// numerators are 0 and not exp(-inf + inf).
+__device__ __forceinline__ float base_of(float top) { return top == -INFINITY ? 0.0f : top; }
 // Two fp32 operations in one instruction.
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
   float2 d;
@@ -294,7 +297,7 @@ __device__ __forceinline__ bool softmax_tile(uint32_t t_s, uint32_t t_p, uint32_
   const float m0 = max32<TAIL>(r0, 0, valid, -INFINITY), m1 = max32<TAIL>(r1, 32, valid, -INFINITY);
   tmem_ld_wait();
   const float m2 = max32<TAIL>(r2, 64, valid, -INFINITY), m3 = max32<TAIL>(r3, 96, valid, -INFINITY);
-  const float now = max3(max3(m0, m1, m2), m3, m3) * scale;
+  const float most = max3(max3(m0, m1, m2), m3, m3), now = most * scale;
   if (Shape<DP>::kOwnP) {
     tc_fence_before();
     __syncwarp();
@@ -319,8 +322,10 @@ __device__ __forceinline__ bool softmax_tile(uint32_t t_s, uint32_t t_p, uint32_
       tmem_st16(t_o + 16 * b, o);
     }
   }
+  // No score above -inf so far: numerators of 0.  (A finite product that only the scale takes to -inf stays NaN.)
+  const float base = most == -INFINITY ? base_of(top) : top;
   float2 sums[2] = {make_float2(sum, 0.0f), make_float2(0.0f, 0.0f)};
-  const float2 scale2 = make_float2(scale, scale), minus_top = make_float2(-top, -top);
+  const float2 scale2 = make_float2(scale, scale), minus_top = make_float2(-base, -base);
   uint32_t w[16];
   exp32<T, TAIL>(r0, 0, valid, scale2, minus_top, sums, w);
   tmem_st16(t_p, w);
@@ -577,9 +582,9 @@ prefix_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
         if (!ok) break;
         ++joins;
         const float2 o = exchange[row];
-        const float now = fmaxf(top, o.x);
-        weight = exp2_approx(top - now);
-        other = exp2_approx(o.x - now);
+        const float now = fmaxf(top, o.x), base = base_of(now);
+        weight = exp2_approx(top - base);
+        other = exp2_approx(o.x - base);
         sum = sum * weight + o.y * other;
         top = now;
       } else if (!g.dual && c == 1) {
@@ -771,7 +776,7 @@ __global__ void __launch_bounds__(WPU > 1 ? 32 * WPU : 128, WPU > 1 ? 1 : DP == 
     const int columns = p.tokens > 1 ? tokens * a.group : min(8, a.group - g0);
     float o[2][NT];  // [column 2 quad + e][value dn * NT + i]
     float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.0f, 0.0f};
-    bool valid[2] = {false, false};
+    int seen[2] = {-1, -1};  // own keys of the columns' tokens; -1: of no sequence
 #pragma unroll
     for (int e = 0; e < 2; ++e)
 #pragma unroll
@@ -788,8 +793,8 @@ __global__ void __launch_bounds__(WPU > 1 ? 32 * WPU : 128, WPU > 1 ? 1 : DP == 
     // The prefix's parts, each lane its own columns' values; a part's maximum and sum are read by eight lanes.  (First, so
     // that their way from memory is under the own keys'.)
     auto fold = [&](int e, float2 st, const float4 (&v)[NT / 4]) {
-      const float now = fmaxf(top[e], st.x);
-      const float keep = sum[e] == 0.0f ? 0.0f : exp2_approx(top[e] - now), weight = exp2_approx(st.x - now);
+      const float now = fmaxf(top[e], st.x), base = base_of(now);
+      const float keep = exp2_approx(top[e] - base), weight = exp2_approx(st.x - base);
       top[e] = now;
       sum[e] = sum[e] * keep + st.y * weight;
 #pragma unroll
@@ -890,7 +895,7 @@ __global__ void __launch_bounds__(WPU > 1 ? 32 * WPU : 128, WPU > 1 ? 1 : DP == 
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         active[e] = (!own || of[e] == tt) && 2 * quad + e < columns;
-        valid[e] = valid[e] || (own && active[e]);
+        if (own && active[e]) seen[e] = count;
       }
       if (count <= 16 * wi) continue;
       const Rows& key_rows = own ? a.ko : a.kp;
@@ -933,9 +938,10 @@ __global__ void __launch_bounds__(WPU > 1 ? 32 * WPU : 128, WPU > 1 ? 1 : DP == 
           float now = fmaxf(top[e], fmaxf(s0, s1));
 #pragma unroll
           for (int d = 4; d < 32; d <<= 1) now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, d));
-          keep[e] = top[e] == -INFINITY ? 0.0f : exp2_approx(top[e] - now);
-          pr[e] = in0 ? exp2_approx(s0 - now) : 0.0f;
-          pr[2 + e] = in1 ? exp2_approx(s1 - now) : 0.0f;
+          const float base = base_of(now);
+          keep[e] = exp2_approx(top[e] - base);
+          pr[e] = in0 ? exp2_approx(s0 - base) : 0.0f;
+          pr[2 + e] = in1 ? exp2_approx(s1 - base) : 0.0f;
           if (active[e]) {
             top[e] = now;
             sum[e] = sum[e] * keep[e] + pr[e] + pr[2 + e];
@@ -982,9 +988,8 @@ __global__ void __launch_bounds__(WPU > 1 ? 32 * WPU : 128, WPU > 1 ? 1 : DP == 
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             const float other_top = from[8 * DP + 2 * (2 * quad + e)], other_sum = from[8 * DP + 2 * (2 * quad + e) + 1];
-            if (other_sum == 0.0f) continue;  // nothing was left for that warp
-            const float now = fmaxf(top[e], other_top);
-            const float keep = sum[e] == 0.0f ? 0.0f : exp2_approx(top[e] - now), weight = exp2_approx(other_top - now);
+            const float now = fmaxf(top[e], other_top), base = base_of(now);
+            const float keep = exp2_approx(top[e] - base), weight = exp2_approx(other_top - base);
             top[e] = now;
             sum[e] = sum[e] * keep + other_sum * weight;
 #pragma unroll
@@ -996,8 +1001,8 @@ __global__ void __launch_bounds__(WPU > 1 ? 32 * WPU : 128, WPU > 1 ? 1 : DP == 
     if (wi == 0) {
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        if (!valid[e]) continue;
-        const bool none = sum[e] == 0.0f;  // no key at all (a largest score adds at least 1 to its sum)
+        if (seen[e] < 0) continue;
+        const bool none = seen[e] == 0 && a.prefix == 0;  // no key at all (keys whose scores are all -inf give 0 / 0)
         const float inv = none ? 0.0f : 1.0f / sum[e];
         const long long token = token0 + of[e], head = (long long)h * a.group + g0 + 2 * quad + e - of[e] * per_token;
         T* const out = static_cast<T*>(a.out) + token * a.out_row + head * a.out_head + dn * NT;
@@ -1038,6 +1043,7 @@ __global__ void __launch_bounds__(256) cut_items_kernel(JoinParams p) {
   float top = -INFINITY, sum = 0.0f;
   if (there) {
     for (int i = 0; i < parts; ++i) top = fmaxf(top, p.stats[(long long)p.plan.part_of(item, (int)blockIdx.x + i, parts) * kPartRows + row].x);
+    const float base = base_of(top);
     // warp w: pieces w, w + 8, ..
     float4 acc[DP / 32];
 #pragma unroll
@@ -1045,7 +1051,7 @@ __global__ void __launch_bounds__(256) cut_items_kernel(JoinParams p) {
     for (int i = 0; i < parts; ++i) {
       const int slot = p.plan.part_of(item, (int)blockIdx.x + i, parts);
       const float2 st = p.stats[(long long)slot * kPartRows + row];
-      const float weight = exp2_approx(st.x - top);
+      const float weight = exp2_approx(st.x - base);
       sum += st.y * weight;
 #pragma unroll
       for (int x = 0; x < DP / 32; ++x) {

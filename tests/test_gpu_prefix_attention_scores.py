@@ -1,0 +1,122 @@
+"""Shared-prefix attention where scores are infinite or far out: keys masked through an extra value of the head.
+
+The queries hold 1 in the head's last place, the keys 0 there, or the mask.  A masked key has weight zero and adds
+nothing to any sum, so that a row is held to the same row without its masked keys, under the bound of that row."""
+import copy
+import math
+
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+import torch
+import annc_b200  # noqa: F401,E402  (no fallback: a missing library fails the collection)
+from annc_b200 import device  # noqa: E402
+from tests.test_gpu_prefix_attention import BF16, F16, Batch, some_of  # noqa: E402
+
+INF = float("inf")
+
+
+def maskable(*args, **kw):
+    """A batch whose keys have a place for a mask."""
+    b = Batch(*args, **kw)
+    b.q[..., -1], b.kp[..., -1], b.ko[..., -1] = 1, 0, 0
+    return b
+
+
+def check_without(b, keep, tokens=None, own=True):
+    """b has run; the prefix keys that are not in `keep` were masked."""
+    c = some_of(b, tokens) if tokens is not None else copy.copy(b)
+    c.kp, c.vp = b.kp[keep], b.vp[keep]
+    c.check(own=own)
+
+
+def run_of(first, count, prefix):
+    keep = torch.ones(prefix, dtype=torch.bool, device="cuda")
+    keep[first:first + count] = False
+    return keep
+
+
+# ---------------------------------------------------------------- scores of -inf
+
+# (tokens, heads, key heads, prefix): items that one CTA has all of and items that are cut, one row tile (two chains that
+# take the key tiles in turn) and two; each without own keys and with them
+@pytest.mark.parametrize("tokens,heads,kv,prefix", [(3, 4, 2, 20000), (700, 4, 4, 1700), (600, 8, 1, 1300), (5, 2, 1, 1500)])
+@pytest.mark.parametrize("dim,dtype", [(64, BF16), (128, F16)])
+@pytest.mark.parametrize("own", [True, False])
+def test_runs_of_hidden_keys(tokens, heads, kv, prefix, dim, dtype, own):
+    some = np.unique(np.linspace(0, tokens - 1, 7).astype(int))
+    for count in (128, 129, 1000):
+        for first in (0, 128, 129, prefix // 2 // 128 * 128, prefix // 2 + 5, prefix - count):
+            b = maskable([1] * tokens, [(i * 5) % 7 for i in range(tokens)], heads, kv, dim, prefix, dtype, seed=count + first)
+            keep = run_of(first, count, prefix)
+            b.kp[~keep, :, -1] = -INF
+            b.run(own=own)
+            check_without(b, keep, some, own)
+
+
+@pytest.mark.parametrize("dim,dtype", [(64, F16), (128, BF16)])
+@pytest.mark.parametrize("tokens,kv,prefix", [(5, 2, 20000), (600, 1, 1300), (5, 2, 700), (4, 2, 40)])
+def test_all_of_a_prefix_hidden(tokens, kv, prefix, dim, dtype):
+    # the own keys alone are left; where there are none either, every score is -inf: NaN, and lse -inf
+    no = np.array([(i * 5) % 7 for i in range(tokens)])
+    b = maskable([1] * tokens, no, 4, kv, dim, prefix, dtype, seed=prefix)
+    b.kp[..., -1] = -INF
+    b.run()
+    some = np.unique(np.linspace(0, tokens - 1, 30).astype(int))
+    check_without(b, torch.zeros(prefix, dtype=torch.bool, device="cuda"), some[no[some] > 0])
+    lost = torch.from_numpy(np.flatnonzero(no == 0)).cuda()
+    assert bool(torch.isnan(b.out[lost]).all()) and bool((b.lse[lost] == -INF).all())
+    b.run(own=False)
+    assert bool(torch.isnan(b.out).all()) and bool((b.lse == -INF).all())
+
+
+@pytest.mark.parametrize("dim,dtype", [(64, BF16), (128, F16), (40, F16)])
+@pytest.mark.parametrize("tokens", [2, 40, 1500])
+def test_hidden_keys_of_a_short_prefix_and_of_sequences(tokens, dim, dtype):
+    # the first keys of a short prefix, and the first own keys of every sequence, in steps around 16
+    for hidden in (1, 15, 16, 17, 32, 47):
+        no = np.array([(i * 11) % 50 for i in range(tokens)])
+        for prefix, hidden_prefix in ((0, 0), (50, hidden), (50, 50), (700, 300)):
+            b = maskable([1] * tokens, no, 4, 2, dim, prefix, dtype, seed=hidden)
+            b.kp[:hidden_prefix, :, -1] = -INF
+            for t in range(tokens):
+                b.ko[int(b.begin[t]):int(b.begin[t]) + min(hidden, int(no[t])), :, -1] = -INF
+            b.run()
+            c = copy.copy(b)
+            c.kp, c.vp = b.kp[hidden_prefix:], b.vp[hidden_prefix:]
+            c.begin, c.no = b.begin + np.minimum(no, hidden), no - np.minimum(no, hidden)
+            some = np.unique(np.linspace(0, tokens - 1, 60).astype(int))
+            left = (prefix - hidden_prefix + c.no[some]) > 0
+            some_of(c, some[left]).check()
+            lost = [int(t) for t in some[~left] if prefix + no[t] > 0]  # keys, none of them with a finite score
+            assert not lost or bool(torch.isnan(b.out[lost]).all()) and bool((b.lse[lost] == -INF).all())
+            none = [int(t) for t in some[~left] if prefix + no[t] == 0]
+            assert not none or bool((b.out[none] == 0).all()) and bool((b.lse[none] == -INF).all())
+
+
+@pytest.mark.parametrize("dim,scale", [(136, 0.09), (60, 0.1), (64, -0.3)])
+def test_hidden_keys_row_by_row(dim, scale):
+    for first, count in ((0, 3), (0, 4), (0, 9), (40, 30), (96, 4)):
+        b = maskable([1, 1, 3], [0, 9, 4], 4, 2, dim, 100, seed=count)
+        keep = run_of(first, count, 100)
+        b.kp[~keep, :, -1] = -math.copysign(INF, scale)
+        b.run(scale=scale)
+        c = copy.copy(b)
+        c.kp, c.vp = b.kp[keep], b.vp[keep]
+        c.check(scale=scale)
+    b.kp[..., -1] = -math.copysign(INF, scale)
+    b.run(own=False, scale=scale)
+    assert bool(torch.isnan(b.out).all()) and bool((b.lse == -INF).all())
+
+
+def test_a_hidden_key_with_an_infinite_value_shows():
+    # weight zero times infinity is NaN, as the formula has it, in the row's other key heads nothing
+    for prefix, hidden in ((700, 130), (40, 16)):
+        b = maskable([1] * 3, [0] * 3, 4, 2, 64, prefix, seed=8)
+        b.kp[:hidden, :, -1] = -INF
+        b.vp[3, 0, 5] = INF
+        b.run(own=False)
+        bad = torch.isnan(b.out)
+        assert bool(bad[:, :2, 5].all()) and int(bad.sum()) == 6
