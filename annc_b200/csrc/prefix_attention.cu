@@ -38,7 +38,8 @@ __global__ void __launch_bounds__(128) attention_rows_kernel(Params p) {
   int count;
   if (!own_keys(p, token, &first, &count)) return;
   constexpr int N = kMaxDim / 32, U = 4;
-  float q[N], acc[N] = {}, top = -INFINITY, sum = 0.0f;
+  // (the maximum starts at the lowest number, not at -inf: scores of -inf alone then have weights of 0, not of exp(-inf + inf))
+  float q[N], acc[N] = {}, top = -3.402823466e38f, sum = 0.0f;
   const T* qp = static_cast<const T*>(p.q.data) + token * p.q.row + h * p.q.head;
 #pragma unroll
   for (int i = 0; i < N; ++i) q[i] = lane + 32 * i < p.dim ? to_float(qp[lane + 32 * i]) : 0.0f;
@@ -64,16 +65,15 @@ __global__ void __launch_bounds__(128) attention_rows_kernel(Params p) {
       float now = top;
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        s[u] = j + u < to ? s[u] * p.scale : -INFINITY;
+        s[u] = j + u < to ? __fmul_rn(s[u], p.scale) : -INFINITY;
         now = fmaxf(now, s[u]);
       }
-      const float base = now == -INFINITY ? 0.0f : now;  // (all scores so far are -inf: weights of 0, not of exp(-inf + inf))
-      const float keep = expf(top - base);
+      const float keep = expf(top - now);
       top = now;
       sum *= keep;
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        w[u] = j + u < to ? expf(s[u] - base) : 0.0f;
+        w[u] = j + u < to ? expf(__fsub_rn(s[u], now)) : 0.0f;
         sum += w[u];
       }
 #pragma unroll

@@ -55,7 +55,10 @@ using namespace annc::tc;
 
 constexpr int kThreads = 384;  // eight softmax warps, loads, products, and two that complete the group of four
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-constexpr float kSlack = 8.0f;  // log2 of what a numerator may grow to before the maximum moves
+constexpr float kSlack = 8.0f * kLn2;  // what a score may pass the maximum by before that moves: a numerator of 2^8
+constexpr float kFar = 2097152.0f;     // scores from here on are rounded before their maximum is subtracted (softmax_tile)
+// Maxima start here, not at -inf: where every score is -inf the numerators are then 0, not exp(-inf + inf).
+constexpr float kLowest = -3.402823466e38f;
 
 template <int DP>
 struct Shape {
@@ -88,11 +91,11 @@ struct PrefixParams {
   Params a;
   long long tokens;
   int kv_heads, group, prefix, dim;
-  float scale2;  // scale * log2(e)
+  float scale, scale2;  // scale2: scale * log2(e)
   // [part][DP / 4][256] pieces of four values: a lane writes its row, so rows are adjacent (row by row the writes, 32
   // pieces at 512 bytes from one another, took 5 us a segment)
   float4* parts;
-  float2* stats;  // [part][256]: maximum (log2 units), sum
+  float2* stats;  // [part][256]: maximum, sum
   Own* own;       // per token, or null
   // no own keys, every token a sequence: what a CTA has all of goes out at once
   int direct;
@@ -183,9 +186,6 @@ __device__ __forceinline__ float exp2_approx(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// What is subtracted from scores whose maximum is `top`: nothing where all of them are -inf, so that their
-// numerators are 0 and not exp(-inf + inf).
-__device__ __forceinline__ float base_of(float top) { return top == -INFINITY ? 0.0f : top; }
 // Two fp32 operations in one instruction.
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
   float2 d;
@@ -253,7 +253,7 @@ __device__ __forceinline__ Segment segment_at(const PrefixParams& p, int at, int
 }
 
 // A row's 128 scores of one key tile (in tensor memory, a lane each) -> numerators in the operands' type in their
-// place; the row's maximum `top` (log2 units: scale * score) and sum follow, and O where the maximum moves.  `half_ready` is
+// place; the row's maximum `top` (of scale * q . k) and sum follow, and O where the maximum moves.  `half_ready` is
 // signalled when the first 64 keys' numerators are written.  TAIL: only the first `valid` keys are there.
 template <bool TAIL>
 __device__ __forceinline__ float max32(const uint32_t (&r)[32], int first, int valid, float top) {
@@ -269,11 +269,11 @@ __device__ __forceinline__ float max32(const uint32_t (&r)[32], int first, int v
   return max3(max3(m[0], m[1], m[2]), m[3], m[3]);
 }
 template <typename T, bool TAIL>
-__device__ __forceinline__ void exp32(const uint32_t (&r)[32], int first, int valid, float2 scale, float2 minus_top, float2 (&sum)[2],
+__device__ __forceinline__ void exp32(const uint32_t (&r)[32], int first, int valid, float2 by, float2 minus, float2 (&sum)[2],
                                       uint32_t (&w)[16]) {
 #pragma unroll
   for (int j = 0; j < 32; j += 2) {
-    const float2 x = fma2(make_float2(__uint_as_float(r[j]), __uint_as_float(r[j + 1])), scale, minus_top);
+    const float2 x = fma2(make_float2(__uint_as_float(r[j]), __uint_as_float(r[j + 1])), by, minus);
     float2 e = make_float2(exp2_approx(x.x), exp2_approx(x.y));
     if (TAIL) {
       if (first + j >= valid) e.x = 0.0f;
@@ -284,8 +284,8 @@ __device__ __forceinline__ void exp32(const uint32_t (&r)[32], int first, int va
   }
 }
 template <typename T, int DP, bool TAIL>
-__device__ __forceinline__ bool softmax_tile(uint32_t t_s, uint32_t t_p, uint32_t t_o, float scale, bool first, int valid, float& top,
-                                             float& sum, uint32_t half_ready, uint32_t scores_read, uint32_t p_used, uint32_t p_phase,
+__device__ __forceinline__ bool softmax_tile(uint32_t t_s, uint32_t t_p, uint32_t t_o, float scale, float scale2, bool first, int valid,
+                                             float& top, float& sum, uint32_t half_ready, uint32_t scores_read, uint32_t p_used, uint32_t p_phase,
                                              volatile int* abort_flag, int* error_word) {
   bool ok = true;
   uint32_t r0[32], r1[32], r2[32], r3[32];
@@ -305,39 +305,59 @@ __device__ __forceinline__ bool softmax_tile(uint32_t t_s, uint32_t t_p, uint32_
     ok = all_wait(p_used, p_phase, abort_flag, error_word);  // the product before this one: it reads P and adds to O
     tc_fence_after();
   }
-  if (first) {
-    top = now;
-  } else if (__any_sync(0xffffffffu, now > top + kSlack)) {
-    // (the products before this are complete)
-    const float keep = now > top + kSlack ? exp2_approx(top - now) : 1.0f;
-    if (now > top + kSlack) top = now;
-    sum *= keep;
+  // The numerator is 2^(score * scale2 - top * log2 e) in one operation, whose product is not rounded while the maximum is:
+  // nothing as long as that is small.  Far out it is a power of anything, and where no score is above -inf that of NaN.
+  const bool moves = first || now - top > kSlack, far = fabsf(now) >= kFar;
+  const float old_top = top;
+  if (moves) top = fmaxf(now, kLowest);
+  float minus = -top * kLog2e;
+  if (__any_sync(0xffffffffu, far || (moves && !first))) {
+    if (!first) {
+      // (the products before this are complete)
+      const float keep = moves ? exp2_approx((old_top - top) * kLog2e) : 1.0f;
+      sum *= keep;
 #pragma unroll 1
-    for (int b = 0; b < DP / 16; ++b) {
-      uint32_t o[16];
-      tmem_ld16(t_o + 16 * b, o);
-      tmem_ld_wait();
+      for (int b = 0; b < DP / 16; ++b) {
+        uint32_t o[16];
+        tmem_ld16(t_o + 16 * b, o);
+        tmem_ld_wait();
 #pragma unroll
-      for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * keep);
-      tmem_st16(t_o + 16 * b, o);
+        for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * keep);
+        tmem_st16(t_o + 16 * b, o);
+      }
+    }
+    if (__any_sync(0xffffffffu, far)) {
+      // Scores are rounded, then the maximum is subtracted, so that equal ones stay equal, and what is left is put in
+      // their place as if it had come out of the product.  (Finite products that the scale takes to -inf, with nothing
+      // above them so far, become NaN.)
+      const float base = top == kLowest && most != -INFINITY ? now : top, up = 1.0f / scale;
+      minus = 0.0f;
+      auto settle = [&](uint32_t (&r)[32]) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+          asm volatile("{\n\t.reg .f32 x;\n\tmov.b32 x, %0;\n\tmul.rn.f32 x, x, %1;\n\tsub.rn.f32 x, x, %2;\n\tmul.rn.f32 x, x, %3;\n\tmov.b32 %0, x;\n\t}"
+                       : "+r"(r[j]) : "f"(scale), "f"(base), "f"(up));
+      };
+      settle(r0);
+      settle(r1);
+      settle(r2);
+      settle(r3);
     }
   }
-  // No score above -inf so far: numerators of 0.  (A finite product that only the scale takes to -inf stays NaN.)
-  const float base = most == -INFINITY ? base_of(top) : top;
   float2 sums[2] = {make_float2(sum, 0.0f), make_float2(0.0f, 0.0f)};
-  const float2 scale2 = make_float2(scale, scale), minus_top = make_float2(-base, -base);
+  const float2 by = make_float2(scale2, scale2), minus2 = make_float2(minus, minus);
   uint32_t w[16];
-  exp32<T, TAIL>(r0, 0, valid, scale2, minus_top, sums, w);
+  exp32<T, TAIL>(r0, 0, valid, by, minus2, sums, w);
   tmem_st16(t_p, w);
-  exp32<T, TAIL>(r1, 32, valid, scale2, minus_top, sums, w);
+  exp32<T, TAIL>(r1, 32, valid, by, minus2, sums, w);
   tmem_st16(t_p + 16, w);
-  exp32<T, TAIL>(r2, 64, valid, scale2, minus_top, sums, w);
+  exp32<T, TAIL>(r2, 64, valid, by, minus2, sums, w);
   tmem_st_wait();  // (of the first 64, long done by now)
   tc_fence_before();
   __syncwarp();
   if ((threadIdx.x & 31) == 0) mbar_arrive(half_ready);
   tmem_st16(t_p + 32, w);
-  exp32<T, TAIL>(r3, 96, valid, scale2, minus_top, sums, w);
+  exp32<T, TAIL>(r3, 96, valid, by, minus2, sums, w);
   tmem_st16(t_p + 48, w);
   sums[0] = add2(sums[0], sums[1]);
   sum = sums[0].x + sums[0].y;
@@ -524,7 +544,6 @@ prefix_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
     const int row = q * 32 + lane;  // of the tile
     const uint32_t lanes = (uint32_t)(q * 32) << 16;
     const uint32_t t_s = tmem + 128 * c + lanes, t_o = tmem + S::kO + DP * c + lanes, t_p = tmem + S::kP + S::kPStep * c + lanes;
-    const float scale = p.scale2;
     uint32_t parts = 0, done = 0, joins = 0;  // segments with key tiles, steps, segments joined: of this chain so far
     for (int at = begin; at < end && ok;) {
       const Segment g = segment_at(p, at, begin, end);
@@ -534,7 +553,7 @@ prefix_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
       const long long token0 = (long long)(2 * g.tile + (g.dual ? c : 0)) * p.plan.tile_tokens;
       const int rows = (int)min((long long)p.plan.tile_tokens, p.tokens - token0) * p.group;
       const bool any = q * 32 < rows;  // of this warp's
-      float top = -INFINITY, sum = 0.0f;  // top in units of log2: scale * score
+      float top = kLowest, sum = 0.0f;
       for (int step = 0; step < steps; ++step, ++done) {
         ok = all_wait(bar_s + 8 * c, done & 1u, abort_flag, p.error_word);
         if (!ok) break;
@@ -544,10 +563,10 @@ prefix_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
           // (two copies of the code: selects for every value of every tile would be a third of its instructions)
           const uint32_t p_phase = (done & 1u) ^ 1u;
           if (valid >= kTileKeys)
-            ok = softmax_tile<T, DP, false>(t_s, t_p, t_o, scale, step == 0, valid, top, sum, bar_h + 8 * c, bar_read + 8 * c,
+            ok = softmax_tile<T, DP, false>(t_s, t_p, t_o, p.scale, p.scale2, step == 0, valid, top, sum, bar_h + 8 * c, bar_read + 8 * c,
                                             bar_pv + 8 * c, p_phase, abort_flag, p.error_word);
           else
-            ok = softmax_tile<T, DP, true>(t_s, t_p, t_o, scale, step == 0, valid, top, sum, bar_h + 8 * c, bar_read + 8 * c,
+            ok = softmax_tile<T, DP, true>(t_s, t_p, t_o, p.scale, p.scale2, step == 0, valid, top, sum, bar_h + 8 * c, bar_read + 8 * c,
                                            bar_pv + 8 * c, p_phase, abort_flag, p.error_word);
           if (!ok) break;
           tc_fence_before();
@@ -582,9 +601,9 @@ prefix_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
         if (!ok) break;
         ++joins;
         const float2 o = exchange[row];
-        const float now = fmaxf(top, o.x), base = base_of(now);
-        weight = exp2_approx(top - base);
-        other = exp2_approx(o.x - base);
+        const float now = fmaxf(top, o.x);
+        weight = exp2_approx((top - now) * kLog2e);
+        other = exp2_approx((o.x - now) * kLog2e);
         sum = sum * weight + o.y * other;
         top = now;
       } else if (!g.dual && c == 1) {
@@ -599,7 +618,7 @@ prefix_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
         const int head = g.head * p.group + row % p.group;
         if (mine) {
           if (!direct) p.stats[part_row] = make_float2(top, sum);
-          else if (p.lse) p.lse[token * p.kv_heads * p.group + head] = (top + log2f(sum)) * kLn2;
+          else if (p.lse) p.lse[token * p.kv_heads * p.group + head] = top + log2f(sum) * kLn2;
         }
         if (direct) {
           const float inv = 1.0f / sum;
@@ -708,7 +727,6 @@ __device__ __forceinline__ void prefetch_l1(const void* at) { asm volatile("pref
 struct JoinParams {
   Params a;
   Plan plan;
-  float scale2;
   int short_prefix;  // keys of a prefix that is taken here, like own keys; else 0
   int tokens;        // of a unit of work
   uint32_t kv_heads_magic, item_magic, per_cta_magic;  // for quotient()
@@ -793,8 +811,8 @@ __global__ void __launch_bounds__(WPU > 1 ? 32 * WPU : 128, WPU > 1 ? 1 : DP == 
     // The prefix's parts, each lane its own columns' values; a part's maximum and sum are read by eight lanes.  (First, so
     // that their way from memory is under the own keys'.)
     auto fold = [&](int e, float2 st, const float4 (&v)[NT / 4]) {
-      const float now = fmaxf(top[e], st.x), base = base_of(now);
-      const float keep = exp2_approx(top[e] - base), weight = exp2_approx(st.x - base);
+      const float now = fmaxf(top[e], st.x);
+      const float keep = exp2_approx((top[e] - now) * kLog2e), weight = exp2_approx((st.x - now) * kLog2e);
       top[e] = now;
       sum[e] = sum[e] * keep + st.y * weight;
 #pragma unroll
@@ -934,14 +952,13 @@ __global__ void __launch_bounds__(WPU > 1 ? 32 * WPU : 128, WPU > 1 ? 1 : DP == 
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const bool in0 = active[e] && k0 + dn < count, in1 = active[e] && k0 + dn + 8 < count;
-          const float s0 = in0 ? s[e] * p.scale2 : -INFINITY, s1 = in1 ? s[2 + e] * p.scale2 : -INFINITY;
-          float now = fmaxf(top[e], fmaxf(s0, s1));
+          const float s0 = in0 ? __fmul_rn(s[e], a.scale) : -INFINITY, s1 = in1 ? __fmul_rn(s[2 + e], a.scale) : -INFINITY;
+          float now = max3(fmaxf(top[e], kLowest), s0, s1);
 #pragma unroll
           for (int d = 4; d < 32; d <<= 1) now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, d));
-          const float base = base_of(now);
-          keep[e] = exp2_approx(top[e] - base);
-          pr[e] = in0 ? exp2_approx(s0 - base) : 0.0f;
-          pr[2 + e] = in1 ? exp2_approx(s1 - base) : 0.0f;
+          keep[e] = exp2_approx((top[e] - now) * kLog2e);
+          pr[e] = in0 ? exp2_approx(__fsub_rn(s0, now) * kLog2e) : 0.0f;
+          pr[2 + e] = in1 ? exp2_approx(__fsub_rn(s1, now) * kLog2e) : 0.0f;
           if (active[e]) {
             top[e] = now;
             sum[e] = sum[e] * keep[e] + pr[e] + pr[2 + e];
@@ -983,17 +1000,28 @@ __global__ void __launch_bounds__(WPU > 1 ? 32 * WPU : 128, WPU > 1 ? 1 : DP == 
       __syncthreads();
       if (wi == 0) {
 #pragma unroll
-        for (int w = 1; w < WPU; ++w) {
-          const float* const from = join_smem + (warp + w) * kWarp;
+        for (int e = 0; e < 2; ++e) {
+          const float* const from = join_smem + warp * kWarp + (2 * quad + e) * DP + dn * NT;
+          const float2* const stats = reinterpret_cast<const float2*>(join_smem + warp * kWarp + 8 * DP) + 2 * quad + e;
+          float2 st[WPU];
+          float now = fmaxf(top[e], kLowest);
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const float other_top = from[8 * DP + 2 * (2 * quad + e)], other_sum = from[8 * DP + 2 * (2 * quad + e) + 1];
-            const float now = fmaxf(top[e], other_top), base = base_of(now);
-            const float keep = exp2_approx(top[e] - base), weight = exp2_approx(other_top - base);
-            top[e] = now;
-            sum[e] = sum[e] * keep + other_sum * weight;
+          for (int w = 1; w < WPU; ++w) {
+            st[w] = stats[w * (kWarp / 2)];
+            now = fmaxf(now, st[w].x);
+          }
+          const float keep = exp2_approx((top[e] - now) * kLog2e);
+          top[e] = now;
+          sum[e] *= keep;
 #pragma unroll
-            for (int i = 0; i < NT; ++i) o[e][i] = o[e][i] * keep + from[(2 * quad + e) * DP + dn * NT + i] * weight;
+          for (int i = 0; i < NT; ++i) o[e][i] *= keep;
+#pragma unroll
+          for (int w = 1; w < WPU; ++w) {
+            if (st[w].x == -INFINITY) continue;  // nothing was left for that warp
+            const float weight = exp2_approx((st[w].x - now) * kLog2e);
+            sum[e] += st[w].y * weight;
+#pragma unroll
+            for (int i = 0; i < NT; ++i) o[e][i] += from[w * kWarp + i] * weight;
           }
         }
       }
@@ -1012,7 +1040,7 @@ __global__ void __launch_bounds__(WPU > 1 ? 32 * WPU : 128, WPU > 1 ? 1 : DP == 
             *reinterpret_cast<uint4*>(out + 8 * x) =
                 make_uint4(pack2<T>(o[e][8 * x] * inv, o[e][8 * x + 1] * inv), pack2<T>(o[e][8 * x + 2] * inv, o[e][8 * x + 3] * inv),
                            pack2<T>(o[e][8 * x + 4] * inv, o[e][8 * x + 5] * inv), pack2<T>(o[e][8 * x + 6] * inv, o[e][8 * x + 7] * inv));
-        if (a.lse && dn == 0) a.lse[token * a.heads + head] = none ? -INFINITY : (top[e] + log2f(sum[e])) * kLn2;
+        if (a.lse && dn == 0) a.lse[token * a.heads + head] = none ? -INFINITY : top[e] + log2f(sum[e]) * kLn2;
       }
     }
     if (WPU > 1) __syncthreads();
@@ -1040,10 +1068,9 @@ __global__ void __launch_bounds__(256) cut_items_kernel(JoinParams p) {
   const int in_tile = row - second * kTileRows, tokens = p.plan.tile_tokens;
   const long long token0 = ((long long)2 * tile + second) * tokens;
   const bool there = in_tile < tokens * a.group && token0 + in_tile / a.group < a.tokens;
-  float top = -INFINITY, sum = 0.0f;
+  float top = kLowest, sum = 0.0f;
   if (there) {
     for (int i = 0; i < parts; ++i) top = fmaxf(top, p.stats[(long long)p.plan.part_of(item, (int)blockIdx.x + i, parts) * kPartRows + row].x);
-    const float base = base_of(top);
     // warp w: pieces w, w + 8, ..
     float4 acc[DP / 32];
 #pragma unroll
@@ -1051,7 +1078,7 @@ __global__ void __launch_bounds__(256) cut_items_kernel(JoinParams p) {
     for (int i = 0; i < parts; ++i) {
       const int slot = p.plan.part_of(item, (int)blockIdx.x + i, parts);
       const float2 st = p.stats[(long long)slot * kPartRows + row];
-      const float weight = exp2_approx(st.x - base);
+      const float weight = exp2_approx((st.x - top) * kLog2e);
       sum += st.y * weight;
 #pragma unroll
       for (int x = 0; x < DP / 32; ++x) {
@@ -1065,7 +1092,7 @@ __global__ void __launch_bounds__(256) cut_items_kernel(JoinParams p) {
       float* const to = &turned[lane][4 * (warp + 8 * x)];
       to[0] = acc[x].x * inv; to[1] = acc[x].y * inv; to[2] = acc[x].z * inv; to[3] = acc[x].w * inv;
     }
-    if (warp == 0 && a.lse) a.lse[(token0 + in_tile / a.group) * a.heads + (long long)h * a.group + in_tile % a.group] = (top + log2f(sum)) * kLn2;
+    if (warp == 0 && a.lse) a.lse[(token0 + in_tile / a.group) * a.heads + (long long)h * a.group + in_tile % a.group] = top + log2f(sum) * kLn2;
   }
   __syncthreads();
   constexpr int PER = DP / 8;  // lanes a row: eight values each
@@ -1159,6 +1186,7 @@ int run_as(const Params& a, void* workspace, cudaStream_t s) {
   p.group = a.group;
   p.prefix = (int)a.prefix;
   p.dim = a.dim;
+  p.scale = a.scale;
   p.scale2 = a.scale * kLog2e;
   const size_t slots = 2 * kMaxCtas + (size_t)p.plan.items;
   p.a = a;
@@ -1176,7 +1204,6 @@ int run_as(const Params& a, void* workspace, cudaStream_t s) {
   JoinParams j = {};
   j.a = a;
   j.plan = p.plan;
-  j.scale2 = p.scale2;
   j.short_prefix = short_prefix ? (int)a.prefix : 0;
   j.tokens = 1;
   j.parts = p.parts;
@@ -1211,7 +1238,7 @@ size_t tc_workspace_bytes(long long tokens, int heads, int kv_heads, int dim) {
 
 bool tc_supported(const Params& p, int) {
   if (p.dim % 8 || p.dim > 128 || p.group > kTileRows) return false;
-  if (p.prefix > 0 && !(p.scale >= 0.0f)) return false;  // (the prefix kernel takes the maximum of the unscaled scores)
+  if (p.prefix > 0 && !(p.scale >= 0.0f && std::isfinite(p.scale * kLog2e))) return false;  // (the prefix kernel takes the maximum of the unscaled scores)
   const Plan plan = plan_of(p.tokens, p.kv_heads, p.group, p.prefix);
   if ((long long)plan.row_items * p.kv_heads * (plan.kv_tiles > 0 ? plan.kv_tiles : 1) >= (1LL << 30) || p.tokens * p.kv_heads >= (1LL << 30)) return false;
   if (!rows_ok(p.q, p.tokens, p.heads, true) || p.q.head * p.group >= (1LL << 39)) return false;

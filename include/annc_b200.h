@@ -705,7 +705,8 @@ int annc_rotary_dev(const annc_rotary_desc* desc, void* stream);
  * q_begin[s] .. q_begin[s+1] - 1 (ascending); without q_begin every token is a sequence.  Tokens
  * outside all sequences are left as they are in out and lse.  A token that sees no key gets zeros
  * and lse -inf; lse is the natural logarithm of the sum of exp(scale * q . k).  A key whose score
- * is -inf has weight zero; a token that sees only such keys gets NaN and lse -inf.  own_begin /
+ * is -inf has weight zero; a token that sees only such keys gets NaN and lse -inf.  Scores are f32:
+ * a token with scores beyond its range may get NaN.  own_begin /
  * own_len entries that reach outside 0 .. own_rows are clamped to it.  out and lse must not overlap
  * an input.
  * The prefix is read once for all tokens.  workspace: 16-byte aligned scratch of

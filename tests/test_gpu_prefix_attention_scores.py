@@ -120,3 +120,85 @@ def test_a_hidden_key_with_an_infinite_value_shows():
         b.run(own=False)
         bad = torch.isnan(b.out)
         assert bool(bad[:, :2, 5].all()) and int(bad.sum()) == 6
+
+
+# ---------------------------------------------------------------- scores far out
+
+@pytest.mark.parametrize("tokens,heads,kv,prefix", [(3, 4, 2, 20000), (700, 4, 4, 1700), (600, 8, 1, 1300), (5, 2, 1, 1500), (5, 2, 1, 60)])
+@pytest.mark.parametrize("dim,dtype", [(64, BF16), (128, F16)])
+@pytest.mark.parametrize("own", [True, False])
+def test_runs_of_keys_with_the_lowest_value(tokens, heads, kv, prefix, dim, dtype, own):
+    low = torch.finfo(dtype).min
+    some = np.unique(np.linspace(0, tokens - 1, 7).astype(int))
+    for count in (128, 129, 1000) if prefix > 1000 else (16, 17, 50):
+        for first in (0, 128, prefix // 2 + 5, prefix - count) if prefix > 1000 else (0, 7, prefix - count):
+            b = maskable([1] * tokens, [(i * 5) % 7 for i in range(tokens)], heads, kv, dim, prefix, dtype, seed=count + first)
+            keep = run_of(first, count, prefix)
+            b.kp[~keep, :, -1] = low
+            b.run(own=own)
+            check_without(b, keep, some, own)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("dim", [64, 128, 136])
+@pytest.mark.parametrize("size", [1.0, -1.0, 0.37, -0.37])
+@pytest.mark.parametrize("prefix,tokens", [(40, 5), (130, 5), (1300, 5), (1300, 500), (20000, 3)])
+def test_equal_scores_of_any_size(prefix, tokens, size, dim, dtype):
+    # the same score for every key, as far out as the type goes: the mean of the values
+    heads, kv = 4, 2
+    b = Batch([1] * tokens, [0] * tokens, heads, kv, dim, prefix, dtype, seed=3)
+    f = torch.finfo(dtype)
+    for power in (0, 10, 15, 30, 60, 100, 127):
+        if 2.0 ** power > f.max:
+            continue
+        b.q.zero_()
+        b.q[..., 0] = 1.0 if dtype == BF16 else f.max
+        b.kp[..., 0] = size * 2.0 ** power
+        b.run(own=False)
+        v = b.vp.double().repeat_interleave(heads // kv, 1)
+        want, mass = v.mean(0), v.abs().mean(0)
+        # one weight for all keys of a part, 1 times a power of two where scores are large; the sums of a CTA's part,
+        # their join, the quotient, and half a step of the type.  Small scores have the operands' rounding of the weights too, which
+        # is the same for all keys and for their sum is not.
+        u = f.eps / 2
+        tol = mass * (u + 2.0 ** -17 + 2 * (prefix + 8) * 2.0 ** -24) + u * want.abs()
+        assert bool(((b.out.double() - want).abs() <= tol).all()), power
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("prefix", [1300, 20000])
+def test_large_scores_are_compared_as_they_round(dim, prefix):
+    # one key above all others by a step of the type, far out: it alone has weight
+    b = Batch([1] * 5, [0] * 5, 4, 2, dim, prefix, BF16, seed=4)
+    b.q.zero_()
+    b.q[..., 0] = 1.0
+    for size in (2.0 ** 28, 2.0 ** 60, -(2.0 ** 28)):
+        for at in (0, 127, 128, 700, prefix - 1):
+            b.kp[..., 0] = size
+            b.kp[at, :, 0] = size * (1 + 2.0 ** -7) if size > 0 else size * (1 - 2.0 ** -8)
+            b.run(own=False)
+            want = b.vp[at].double().repeat_interleave(2, 0)
+            assert bool(((b.out.double() - want).abs() <= 2.0 ** -8 * want.abs()).all()), (size, at)
+
+
+@pytest.mark.parametrize("dtype,scale", [(BF16, 1.0), (BF16, 0.1), (F16, 1.0), (F16, 30000.0)])
+@pytest.mark.parametrize("dim", [64, 128, 136])
+@pytest.mark.parametrize("prefix,tokens", [(0, 3), (40, 3), (300, 3), (20000, 3), (300, 900)])
+def test_every_key_with_the_lowest_value(prefix, tokens, dim, dtype, scale):
+    # a row that is masked throughout by the type's lowest number is the mean of its values
+    heads, kv, own = 4, 2, 21
+    b = Batch([1] * tokens, [own] * tokens, heads, kv, dim, prefix, dtype, seed=5)
+    f = torch.finfo(dtype)
+    b.q.zero_()
+    b.q[..., 0] = 1.0 if dtype == BF16 else f.max
+    b.kp[..., 0] = f.min
+    b.ko[..., 0] = f.min
+    b.run(scale=scale)
+    count, u = prefix + own, f.eps / 2
+    vo = b.vo.double().view(tokens, own, kv, dim)
+    both = lambda p, o: ((p.double().sum(0) + o.sum(1)) / count).repeat_interleave(heads // kv, 1)
+    want, mass = both(b.vp, vo), both(b.vp.abs(), vo.abs())
+    tol = mass * (u + 2.0 ** -17 + 2 * (count + 8) * 2.0 ** -24) + u * want.abs()
+    assert bool(((b.out.double() - want).abs() <= tol).all())
+    top = float(b.q[0, 0, 0].double() * f.min * scale)
+    assert bool(((b.lse.double() - top).abs() <= 2.0 ** -22 * abs(top)).all())
