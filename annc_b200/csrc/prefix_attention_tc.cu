@@ -1238,7 +1238,8 @@ size_t tc_workspace_bytes(long long tokens, int heads, int kv_heads, int dim) {
 
 bool tc_supported(const Params& p, int) {
   if (p.dim % 8 || p.dim > 128 || p.group > kTileRows) return false;
-  if (p.prefix > 0 && !(p.scale >= 0.0f && std::isfinite(p.scale * kLog2e))) return false;  // (the prefix kernel takes the maximum of the unscaled scores)
+  // the prefix kernel takes the maximum of the unscaled scores, multiplies by scale * log2 e, and far out by 1 / scale
+  if (p.prefix > 0 && p.scale != 0.0f && !(p.scale >= 1e-30f && std::isfinite(p.scale * kLog2e))) return false;
   const Plan plan = plan_of(p.tokens, p.kv_heads, p.group, p.prefix);
   if ((long long)plan.row_items * p.kv_heads * (plan.kv_tiles > 0 ? plan.kv_tiles : 1) >= (1LL << 30) || p.tokens * p.kv_heads >= (1LL << 30)) return false;
   if (!rows_ok(p.q, p.tokens, p.heads, true) || p.q.head * p.group >= (1LL << 39)) return false;

@@ -713,7 +713,7 @@ int annc_rotary_dev(const annc_rotary_desc* desc, void* stream);
  * annc_prefix_attention_workspace_bytes(tokens, heads, kv_heads, head_dim) bytes (for at most so
  * many tokens), one call at a time: calls that may overlap (two streams, two graphs) need one each.
  * Head sizes that are multiples of 8 up to 128, rows and heads of all tensors on 16 bytes, at most
- * 128 heads to a key head and scale >= 0 run on the tensor cores; other calls a row at a time, some
+ * 128 heads to a key head and a scale of 0 or 1e-30 and more run on the tensor cores; other calls a row at a time, some
  * ten times slower.  annc_gemm_check reports a bounded wait that ran out, as for the products. */
 typedef struct annc_prefix_attention_desc {
   int32_t dtype;                 /* ANNC_BF16 or ANNC_F16: q, keys, values, out */

@@ -202,3 +202,17 @@ def test_every_key_with_the_lowest_value(prefix, tokens, dim, dtype, scale):
     assert bool(((b.out.double() - want).abs() <= tol).all())
     top = float(b.q[0, 0, 0].double() * f.min * scale)
     assert bool(((b.lse.double() - top).abs() <= 2.0 ** -22 * abs(top)).all())
+
+
+@pytest.mark.parametrize("scale", [0.0, 1e-45, 1e-38, 1e-30, 3e38])
+def test_scales_at_the_ends_of_their_range(scale):
+    b = maskable([1] * 3, [0, 4, 1], 4, 2, 64, 400, BF16, seed=6)
+    b.q[..., :-1] *= 1e-3
+    keep = run_of(100, 40 if scale else 0, 400)
+    b.kp[~keep, :, -1] = -INF
+    if scale > 1:  # scores within the range of 32 bits
+        b.q *= 2.0 ** -126
+    b.run(scale=scale)
+    c = copy.copy(b)
+    c.kp, c.vp = b.kp[keep], b.vp[keep]
+    c.check(scale=scale)
