@@ -60,6 +60,12 @@ constexpr float kFar = 2097152.0f;     // scores from here on are rounded before
 // Maxima start here, not at -inf: where every score is -inf the numerators are then 0, not exp(-inf + inf).
 constexpr float kLowest = -3.402823466e38f;
 
+// Numerators of f16 are raised by a power of two, so that its range goes to small ones: 2^8 of slack and 2^7 are half of
+// 65504, and a numerator is off by at most 2^-25 of what it is then, 2^-32 of the row's largest.  (As they are, 2^17 weights of 2^-26
+// beside one of 1 were lost.)  The join kernel, whose maxima move at once, has 2^15.
+template <typename T>
+__host__ __device__ constexpr int raise_of(int slack) { return std::is_same<T, __half>::value ? 15 - slack : 0; }
+
 template <int DP>
 struct Shape {
   static constexpr int kTile = kTileKeys * DP * 2;  // bytes of 128 rows: DP / 64 blocks of 128 bytes x 128
@@ -310,7 +316,8 @@ __device__ __forceinline__ bool softmax_tile(uint32_t t_s, uint32_t t_p, uint32_
   const bool moves = first || now - top > kSlack, far = fabsf(now) >= kFar;
   const float old_top = top;
   if (moves) top = fmaxf(now, kLowest);
-  float minus = -top * kLog2e;
+  constexpr float kRaise = raise_of<T>(8);
+  float minus = kRaise - top * kLog2e;
   if (__any_sync(0xffffffffu, far || (moves && !first))) {
     if (!first) {
       // (the products before this are complete)
@@ -331,7 +338,7 @@ __device__ __forceinline__ bool softmax_tile(uint32_t t_s, uint32_t t_p, uint32_
       // their place as if it had come out of the product.  (Finite products that the scale takes to -inf, with nothing
       // above them so far, become NaN.)
       const float base = top == kLowest && most != -INFINITY ? now : top, up = 1.0f / scale;
-      minus = 0.0f;
+      minus = kRaise;
       auto settle = [&](uint32_t (&r)[32]) {
 #pragma unroll
         for (int j = 0; j < 32; ++j)
@@ -588,7 +595,9 @@ prefix_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
         if (!ok) break;
         ++parts;
       }
-      float weight = 1.0f, other = 0.0f;  // of this chain's O, of the other one's
+      constexpr float kLower = 1.0f / (1 << raise_of<T>(8));
+      sum *= kLower;
+      float weight = kLower, other = 0.0f;  // of this chain's O, of the other one's
       if (!g.dual && g.steps(1) > 0) {
         float2* const exchange = reinterpret_cast<float2*>(smem_raw + (base + S::kExchange - raw));
         if (c == 1) {
@@ -605,6 +614,8 @@ prefix_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
         weight = exp2_approx((top - now) * kLog2e);
         other = exp2_approx((o.x - now) * kLog2e);
         sum = sum * weight + o.y * other;
+        weight *= kLower;
+        other *= kLower;
         top = now;
       } else if (!g.dual && c == 1) {
         continue;
@@ -753,6 +764,7 @@ __device__ __forceinline__ int quotient(int i, int d, uint32_t magic) {
 template <typename T, int DP, int WPU, bool SHORT>
 __global__ void __launch_bounds__(WPU > 1 ? 32 * WPU : 128, WPU > 1 ? 1 : DP == 128 ? 4 : 5) join_kernel(JoinParams p) {
   constexpr int NT = DP / 8;  // values a lane holds of a column
+  constexpr float kRaise = raise_of<T>(0);  // (of all sums: it drops out of the quotient)
   extern __shared__ float join_smem[];  // (WPU > 1) per warp: 8 columns of DP, 8 x (maximum, sum)
   constexpr int kWarp = 8 * DP + 16;
   pdl_trigger();
@@ -812,7 +824,7 @@ __global__ void __launch_bounds__(WPU > 1 ? 32 * WPU : 128, WPU > 1 ? 1 : DP == 
     // that their way from memory is under the own keys'.)
     auto fold = [&](int e, float2 st, const float4 (&v)[NT / 4]) {
       const float now = fmaxf(top[e], st.x);
-      const float keep = exp2_approx((top[e] - now) * kLog2e), weight = exp2_approx((st.x - now) * kLog2e);
+      const float keep = exp2_approx((top[e] - now) * kLog2e), weight = exp2_approx(fmaf(st.x - now, kLog2e, kRaise));
       top[e] = now;
       sum[e] = sum[e] * keep + st.y * weight;
 #pragma unroll
@@ -833,12 +845,13 @@ __global__ void __launch_bounds__(WPU > 1 ? 32 * WPU : 128, WPU > 1 ? 1 : DP == 
         for (int e = 0; e < 2; ++e) {
           if (2 * quad + e >= columns) continue;
           const float2 st = stats_of(slot, e);
+          constexpr float up = 1 << raise_of<T>(0);
           top[e] = st.x;
-          sum[e] = st.y;
+          sum[e] = st.y * up;
 #pragma unroll
           for (int x = 0; x < NT / 4; ++x) {
             const float4 v = value_of(slot, e, x);
-            o[e][4 * x] = v.x; o[e][4 * x + 1] = v.y; o[e][4 * x + 2] = v.z; o[e][4 * x + 3] = v.w;
+            o[e][4 * x] = v.x * up; o[e][4 * x + 1] = v.y * up; o[e][4 * x + 2] = v.z * up; o[e][4 * x + 3] = v.w * up;
           }
         }
       }
@@ -957,8 +970,8 @@ __global__ void __launch_bounds__(WPU > 1 ? 32 * WPU : 128, WPU > 1 ? 1 : DP == 
 #pragma unroll
           for (int d = 4; d < 32; d <<= 1) now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, d));
           keep[e] = exp2_approx((top[e] - now) * kLog2e);
-          pr[e] = in0 ? exp2_approx(__fsub_rn(s0, now) * kLog2e) : 0.0f;
-          pr[2 + e] = in1 ? exp2_approx(__fsub_rn(s1, now) * kLog2e) : 0.0f;
+          pr[e] = in0 ? exp2_approx(fmaf(__fsub_rn(s0, now), kLog2e, kRaise)) : 0.0f;
+          pr[2 + e] = in1 ? exp2_approx(fmaf(__fsub_rn(s1, now), kLog2e, kRaise)) : 0.0f;
           if (active[e]) {
             top[e] = now;
             sum[e] = sum[e] * keep[e] + pr[e] + pr[2 + e];
@@ -1040,7 +1053,7 @@ __global__ void __launch_bounds__(WPU > 1 ? 32 * WPU : 128, WPU > 1 ? 1 : DP == 
             *reinterpret_cast<uint4*>(out + 8 * x) =
                 make_uint4(pack2<T>(o[e][8 * x] * inv, o[e][8 * x + 1] * inv), pack2<T>(o[e][8 * x + 2] * inv, o[e][8 * x + 3] * inv),
                            pack2<T>(o[e][8 * x + 4] * inv, o[e][8 * x + 5] * inv), pack2<T>(o[e][8 * x + 6] * inv, o[e][8 * x + 7] * inv));
-        if (a.lse && dn == 0) a.lse[token * a.heads + head] = none ? -INFINITY : top[e] + log2f(sum[e]) * kLn2;
+        if (a.lse && dn == 0) a.lse[token * a.heads + head] = none ? -INFINITY : top[e] + (log2f(sum[e]) - kRaise) * kLn2;
       }
     }
     if (WPU > 1) __syncthreads();

@@ -216,3 +216,51 @@ def test_scales_at_the_ends_of_their_range(scale):
     c = copy.copy(b)
     c.kp, c.vp = b.kp[keep], b.vp[keep]
     c.check(scale=scale)
+
+
+# ---------------------------------------------------------------- many small weights of f16
+
+@pytest.mark.parametrize("dim,kv", [(64, 148), (128, 74)])
+@pytest.mark.parametrize("at", [0, 50001, (1 << 17) - 1])
+def test_many_small_weights_beside_a_large_one(dim, kv, at):
+    # one key of weight 1 and 2^17 - 1 of some 2^-26 each, that a CTA has all or half of: they make up 1/512 of the sum, and
+    # all of the output.  A numerator in f16 is off by at most 2^-25 of its unit, which is 2^-7 of the row's largest or less.
+    prefix = 1 << 17
+    b = Batch([1], [0], kv, kv, dim, prefix, F16, seed=at)
+    b.q.zero_()
+    b.q[..., 0] = 1.0
+    b.kp[..., 0] = -18.0 + 0.3 * torch.sin(torch.arange(prefix, device="cuda"))[:, None]
+    b.kp[at, :, 0] = 0
+    b.vp.abs_()  # (every lost weight shows)
+    b.vp[at] = 0
+    b.run(own=False, scale=1.0)
+    u = 2.0 ** -11
+    for h in (0, 1, kv // 2, kv - 1):
+        p, v = torch.softmax(b.kp[:, h, 0].double(), 0), b.vp[:, h].double()
+        want = p @ v
+        tol = want * (u + 2.0 ** -17 + 2 * (prefix + 8) * 2.0 ** -24) + prefix * 2.0 ** -32 * v.amax() * p.max() + u * want
+        got = b.out[0, h].double()
+        assert bool(((got - want).abs() <= tol).all()), float(((got - want).abs() / tol).max())
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("prefix", [0, 60])
+def test_many_small_weights_of_own_keys(dim, prefix):
+    rows = 200000
+    b = Batch([1], [rows], 2, 1, dim, prefix, F16, seed=2)
+    b.q.zero_()
+    b.q[..., 0] = 1.0
+    b.ko[..., 0] = -18.0
+    b.kp[..., 0] = -18.0
+    b.ko[77, :, 0] = 0
+    b.vo.abs_()
+    b.vo[77] = 0
+    b.run(scale=1.0)
+    s = torch.cat([b.kp[:, 0, 0], b.ko[:, 0, 0]]).double()
+    v = torch.cat([b.vp[:, 0], b.vo[:, 0]]).double()
+    want = torch.softmax(s, 0) @ v
+    u, count = 2.0 ** -11, len(s)
+    mass = torch.softmax(s, 0) @ v.abs()
+    tol = mass * (u + 2.0 ** -17 + 2 * (count + 8) * 2.0 ** -24) + count * 2.0 ** -40 * v.abs().amax() + u * want.abs()
+    got = b.out.double()
+    assert bool(((got - want).abs() <= tol).all()), float(((got - want).abs() / tol).max())
