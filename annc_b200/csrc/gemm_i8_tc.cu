@@ -179,8 +179,8 @@ gemm_i8_split_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
   float* const scales = reinterpret_cast<float*>(gen_base + S::kStages * S::kStage);
   constexpr int kBars = S::kStages * S::kStage + S::kScales;
   const uint32_t bars = base + kBars;
-  const uint32_t bar_full = bars, bar_empty = bars + 8 * S::kStages, bar_done = bars + 16 * S::kStages;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gen_base + kBars + 16 * S::kStages + 8);
+  const uint32_t bar_full = bars, bar_empty = bars + 8 * S::kStages, bar_done = bars + 16 * S::kStages, bar_out = bar_done + 8;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gen_base + kBars + 16 * S::kStages + 16);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;  // (known to be uniform)
@@ -198,6 +198,7 @@ gemm_i8_split_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
       mbar_init(bar_empty + 8 * s, 1);
     }
     mbar_init(bar_done, 1);
+    mbar_init(bar_out, 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     // The weight's bytes are on their way to L2 while the kernel before this one (which quantises the tokens)
@@ -218,10 +219,11 @@ gemm_i8_split_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
   pdl_wait();
   const bool poisoned = *reinterpret_cast<volatile int*>(error_word) != 0;  // an earlier launch gave up
   bool ok = !poisoned;
+  uint32_t issued = 0;  // k-steps, by the producer
 
   if (ok && warp == 0) {
     if (lane == 0) {
-      for (int kt = 0; kt < KT && ok; ++kt) {
+      for (int kt = 0; kt < KT && ok; ++kt, ++issued) {
         const int s = kt % S::kStages;
         ok = mbar_wait(bar_empty + 8 * s, ((kt / S::kStages) & 1u) ^ 1u, abort_flag, error_word);
         if (!ok) break;
@@ -336,6 +338,14 @@ gemm_i8_split_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
   }
   tc_fence_before();
   __syncthreads();
+  if (*abort_flag) {  // given up
+    if (warp == 0 && lane == 0) ring_settle(bar_full, S::kStages, issued);
+    if (warp == 1) {
+      commit_elected(bar_out);
+      mbar_settle(bar_out, 0);
+    }
+    __syncwarp();
+  }
   if (warp == 1) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"((uint32_t)S::kCols) : "memory");
@@ -379,8 +389,8 @@ gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
   constexpr int kBars = kPairStages * kPairStage + kPairStaging;
   const uint32_t bars = base + kBars;
   const uint32_t bar_full = bars, bar_empty = bars + 8 * kPairStages;
-  const uint32_t bar_tfull = bars + 16 * kPairStages, bar_tempty = bar_tfull + 16;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gen_base + kBars + 16 * kPairStages + 32);
+  const uint32_t bar_tfull = bars + 16 * kPairStages, bar_tempty = bar_tfull + 16, bar_out = bar_tempty + 16;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gen_base + kBars + 16 * kPairStages + 40);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;  // (known to be uniform)
@@ -401,6 +411,7 @@ gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
       mbar_init(bar_tfull + 8 * a, 1);
       mbar_init(bar_tempty + 8 * a, 16);  // the epilogue warps of both CTAs
     }
+    mbar_init(bar_out, 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -414,10 +425,10 @@ gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
   pdl_wait();
   const bool poisoned = *reinterpret_cast<volatile int*>(error_word) != 0;  // an earlier launch gave up
 
+  uint32_t kit = 0;  // k-steps: issued by the producer, multiplied by the issuer of the products
   if (!poisoned) {
     if (warp == 0) {
       if (lane == 0) {
-        uint32_t kit = 0;
         bool ok = true;
         for (int tile = pair; tile < tiles.count && ok; tile += pairs) {
           int m0, n0;
@@ -439,7 +450,7 @@ gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
     } else if (warp == 1) {
       if (leader) {
         const uint64_t a_desc = smem_desc(base, 16, 1024, 2), b_desc = smem_desc(base + kPairStage / 2, 16, 1024, 2);
-        uint32_t kit = 0, count = 0;
+        uint32_t count = 0;
         bool ok = true;
         for (int tile = pair; tile < tiles.count && ok; tile += pairs, ++count) {
           const uint32_t acc = count & 1u;
@@ -599,6 +610,18 @@ gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
   __syncwarp();
   tc_fence_before();
   __syncthreads();
+  if (*abort_flag) {  // given up
+    if (warp == 0 && lane == 0) {
+      // both CTAs' copies count on the leader's barriers; the other one cannot wait there and gives its own their time
+      if (leader) ring_settle(bar_full, kPairStages, kit);
+      else for (const unsigned long long t0 = global_ns(); global_ns() - t0 < 1000000ull;) {}
+    }
+    if (warp == 1 && leader) {
+      commit_pair_elected(bar_out);
+      mbar_settle(bar_out, 0);
+    }
+    __syncwarp();
+  }
   cluster_sync_all();  // the peer may read this CTA's shared memory until its last MMA is done
   if (warp == 1) {
     tc_fence_after();

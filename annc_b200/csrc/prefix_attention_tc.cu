@@ -385,9 +385,10 @@ prefix_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
   const uint32_t bar_full = bars, bar_empty = bars + 8 * S::kSlots;
   const uint32_t bar_q = bars + 16 * S::kSlots, bar_qfree = bar_q + 8;
   const uint32_t bar_s = bar_q + 16, bar_p = bar_q + 32, bar_o = bar_q + 48, bar_ofree = bar_q + 64, bar_h = bar_q + 80;  // per chain
-  const uint32_t bar_x = bar_q + 96, bar_read = bar_q + 104, bar_pv = bar_q + 120;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem_raw + (bar_q + 136 - raw));
+  const uint32_t bar_x = bar_q + 96, bar_read = bar_q + 104, bar_pv = bar_q + 120, bar_out = bar_q + 136;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem_raw + (bar_q + 144 - raw));
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  volatile uint32_t* issued = tmem_slot + 2;  // by the loader: tiles of keys and values, segments' rows
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;  // (known to be uniform)
   if (threadIdx.x == 0) {
@@ -410,7 +411,9 @@ prefix_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
       mbar_init(bar_pv + 8 * c, 1);    // (P apart) P is used
     }
     mbar_init(bar_x, 4);
+    mbar_init(bar_out, 1);
     *abort_flag = 0;
+    issued[0] = issued[1] = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 9) {
@@ -432,7 +435,7 @@ prefix_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
   registers_down();
   if (warp == 8) {
     if (ok && lane == 0) {
-      uint32_t n = 0, segments = 0;
+      uint32_t n = 0, segments = 0, rows_issued = 0;
       const uint32_t q_bytes = (uint32_t)(p.plan.tile_tokens * p.group) * 128u * (DP / 64);
       auto load = [&](const CUtensorMap* map, int head, int tile) {
         const int s = n % S::kSlots;
@@ -449,6 +452,7 @@ prefix_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
         at += g.count;
         ok = wait(bar_qfree, (segments & 1u) ^ 1u, abort_flag, p.error_word);
         if (!ok) break;
+        ++rows_issued;
         mbar_expect_tx(bar_q, g.dual ? 2 * q_bytes : q_bytes);
         for (int c = 0; c < (g.dual ? 2 : 1); ++c)
 #pragma unroll
@@ -459,13 +463,8 @@ prefix_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
           if (ok) load(&tmap_v, g.head, g.first + t);
         }
       }
-      if (!ok) {
-        // given up: the copies still in flight write this CTA's shared memory, so they are waited for (with a limit)
-        const uint32_t from = n > (uint32_t)S::kSlots ? n - S::kSlots : 0;
-        for (uint32_t i = from; i < n; ++i)
-          for (int k = 0; k < 1000000 && !mbar_try_wait(bar_full + 8 * (i % S::kSlots), (i / S::kSlots) & 1u); ++k) {
-          }
-      }
+      issued[0] = n;
+      issued[1] = rows_issued;
     }
   } else if (warp == 9) {
     if (ok) {
@@ -677,6 +676,17 @@ prefix_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
   __syncwarp();
   tc_fence_before();
   __syncthreads();
+  if (*abort_flag) {  // given up
+    if (warp == 8 && lane == 0) {
+      ring_settle(bar_full, S::kSlots, issued[0]);
+      if (issued[1] > 0) mbar_settle(bar_q, (issued[1] - 1) & 1u);
+    }
+    if (warp == 9) {
+      umma_commit_elected(bar_out);
+      mbar_settle(bar_out, 0);
+    }
+    __syncwarp();
+  }
   if (warp == 9) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");

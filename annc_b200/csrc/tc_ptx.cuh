@@ -56,6 +56,16 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
     }
   }
 }
+// On the way out of a kernel that has given up: copies and products that are still under way read and write the block's
+// shared and tensor memory, so they are waited for, a millisecond each at most (a copy takes microseconds).
+__device__ __forceinline__ void mbar_settle(uint32_t bar, uint32_t parity) {
+  for (const unsigned long long t0 = global_ns(); !mbar_try_wait(bar, parity) && global_ns() - t0 < 1000000ull;) {
+  }
+}
+// ... the copies into a ring of `stages`, of which `issued` were issued so far, copy i on barrier i % stages.
+__device__ __forceinline__ void ring_settle(uint32_t bar_full, uint32_t stages, uint32_t issued) {
+  for (uint32_t i = issued > stages ? issued - stages : 0; i < issued; ++i) mbar_settle(bar_full + 8 * (i % stages), (i / stages) & 1u);
+}
 __device__ __forceinline__ void prefetch_tensormap(const CUtensorMap* map) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
 }
