@@ -735,11 +735,10 @@ __device__ __forceinline__ bool own_keys_of_warp(const Params& p, int token, int
     behind = p.q_begin[seq + 1] - 1 - token;
   }
   if (!p.own_len) return true;
-  const long long begin = p.own_begin[seq];
-  const int len = p.own_len[seq] - behind;
+  const long long begin = p.own_begin[seq], len = (long long)p.own_len[seq] - behind;
   if (len <= 0 || begin < 0 || begin >= p.own_rows) return true;
   *first = begin;
-  *count = (int)min((long long)len, p.own_rows - begin);
+  *count = (int)min(len, p.own_rows - begin);
   return true;
 }
 

@@ -264,3 +264,15 @@ def test_many_small_weights_of_own_keys(dim, prefix):
     tol = mass * (u + 2.0 ** -17 + 2 * (count + 8) * 2.0 ** -24) + count * 2.0 ** -40 * v.abs().amax() + u * want.abs()
     got = b.out.double()
     assert bool(((got - want).abs() <= tol).all()), float(((got - want).abs() / tol).max())
+
+
+# ---------------------------------------------------------------- lists
+
+@pytest.mark.parametrize("prefix", [30, 500])
+def test_lengths_far_below_zero(prefix):
+    # a sequence of several tokens with the lowest length there is: no own keys for any of them
+    b = Batch([1, 4, 3], [3, 5, 4], 4, 2, 64, prefix)
+    b.own_len[1] = -(1 << 31)
+    b.run()
+    b.no[1] = 0
+    b.check()
