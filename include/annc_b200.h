@@ -706,15 +706,18 @@ int annc_rotary_dev(const annc_rotary_desc* desc, void* stream);
  * outside all sequences are left as they are in out and lse.  A token that sees no key gets zeros
  * and lse -inf; lse is the natural logarithm of the sum of exp(scale * q . k).  A key whose score
  * is -inf has weight zero; a token that sees only such keys gets NaN and lse -inf.  Scores are f32:
- * a token with scores beyond its range may get NaN.  own_begin /
- * own_len entries that reach outside 0 .. own_rows are clamped to it.  out and lse must not overlap
- * an input.
- * The prefix is read once for all tokens.  workspace: 16-byte aligned scratch of
- * annc_prefix_attention_workspace_bytes(tokens, heads, kv_heads, head_dim) bytes (for at most so
- * many tokens), one call at a time: calls that may overlap (two streams, two graphs) need one each.
+ * a token with scores beyond its range may get NaN.  An own list that begins outside
+ * 0 .. own_rows - 1 or has a length below one counts as empty, one that would end behind own_rows
+ * ends there.  out and lse must not overlap an input.
+ * Every 256 rows (token, head of a key head's group) read the prefix once, from L2 where it fits,
+ * and a short prefix (64 keys, some 300 with few tokens) every token or few.
+ * workspace: 16-byte aligned scratch of annc_prefix_attention_workspace_bytes(tokens, heads,
+ * kv_heads, head_dim) bytes (for at most so many tokens), one call at a time: calls that may
+ * overlap (two streams, two graphs) need one each.
  * Head sizes that are multiples of 8 up to 128, rows and heads of all tensors on 16 bytes, at most
- * 128 heads to a key head and a scale of 0 or 1e-30 and more run on the tensor cores; other calls a row at a time, some
- * ten times slower.  annc_gemm_check reports a bounded wait that ran out, as for the products. */
+ * 128 heads to a key head and a scale of 0 or 1e-30 and more run on the tensor cores; other calls
+ * a row at a time, a hundred times slower and more (64 tokens of 32 heads of 128 over 4096 keys
+ * 2.8 ms for 29 us).  annc_gemm_check reports a bounded wait that ran out, as for the products. */
 typedef struct annc_prefix_attention_desc {
   int32_t dtype;                 /* ANNC_BF16 or ANNC_F16: q, keys, values, out */
   int32_t heads, kv_heads, head_dim; /* head_dim 1 .. 256 */
