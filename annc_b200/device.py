@@ -443,9 +443,33 @@ def gemm_i8_kernel_name(a, scale_a, b, scale_b, c, bias=None, activation: int = 
     return lib.annc_gemm_i8_kernel_name(_gemm_i8_desc(_current("a", a), a, scale_a, b, scale_b, c, bias, activation)).decode()
 
 
-class Rotary:
+class _Plan:
+    """Device memory that a plan keeps: made on one stream, used on any."""
+
+    def _keep(self, memory: torch.Tensor) -> torch.Tensor:
+        stream = torch.cuda.current_stream(memory.device)
+        self._memory, self._streams = memory, {stream.cuda_stream}
+        self._made = None if torch.cuda.is_current_stream_capturing() else stream.record_event()
+        return memory
+
+    def _stream(self, dev: int) -> int:
+        """The current stream of the device, which may use the memory from now on: behind what had it before the
+        plan, and the allocator hands it out again only behind what is queued there when the plan is dropped."""
+        raw = torch._C._cuda_getCurrentRawStream(dev)
+        if raw not in self._streams:
+            stream = torch.cuda.current_stream(dev)
+            self._memory.record_stream(stream)
+            if not torch.cuda.is_current_stream_capturing():  # (a capture cannot wait for what is outside it)
+                if self._made is not None:
+                    stream.wait_event(self._made)
+                self._streams.add(raw)
+        return raw
+
+
+class Rotary(_Plan):
     """Rotary positions (annc_rotary_dev): holds the frequencies of annc_rotary_frequencies on the device.
-    layout "half" or "interleaved"; scaling "none", "linear", "ntk" or "yarn" by `factor`."""
+    layout "half" or "interleaved"; scaling "none", "linear", "ntk" or "yarn" by `factor`.  Runs on any stream; a
+    captured graph needs the plan as long as it is replayed."""
 
     def __init__(self, rot_dim: int, *, base: float = 10000.0, layout: str = "half", scaling: str = "none",
                  factor: float = 1.0, original_len: int = 4096, beta_fast: float = 32.0, beta_slow: float = 1.0,
@@ -460,7 +484,7 @@ class Rotary:
         check(lib.annc_rotary_frequencies(self.rot_dim, base, scalings[scaling], factor, original_len, beta_fast,
                                           beta_slow, host, C.byref(size)))
         self.size = size.value
-        self.freq = torch.tensor(list(host), dtype=torch.float64, device=device or "cuda")
+        self.freq = self._keep(torch.tensor(list(host), dtype=torch.float64, device=device or "cuda"))
 
     def run(self, positions: torch.Tensor, q: torch.Tensor, out_q: torch.Tensor, k: Optional[torch.Tensor] = None,
             out_k: Optional[torch.Tensor] = None, *, transposed: bool = False) -> None:
@@ -493,14 +517,15 @@ class Rotary:
             PACK_ROTARY.pack(_DTYPES[q.dtype], dim, self.rot_dim, self.layout, pos_type, 1 if transposed else 0, tokens, pos,
                              self.freq.data_ptr(), self.size, 0, q.data_ptr(), out_q.data_ptr(), heads, s[0], s[1], so[0],
                              so[1], *second),
-            torch._C._cuda_getCurrentRawStream(dev))
+            self._stream(dev))
         if rc:
             check(rc)
 
 
-class PrefixAttention:
+class PrefixAttention(_Plan):
     """Attention of up to max_tokens tokens that share one prefix (annc_prefix_attention_dev); holds the workspace.
-    One run() at a time: runs on different streams that may overlap, captured graphs among them, need a plan each."""
+    One run() at a time: runs on different streams that may overlap, captured graphs among them, need a plan each, and
+    a captured graph needs it as long as it is replayed."""
 
     def __init__(self, heads: int, kv_heads: int, head_dim: int, max_tokens: int, *, dtype=torch.bfloat16, device=None):
         if dtype not in (torch.bfloat16, torch.float16):
@@ -509,7 +534,7 @@ class PrefixAttention:
         self.max_tokens, self.dtype = int(max_tokens), dtype
         self.ws_bytes = int(lib.annc_prefix_attention_workspace_bytes(self.max_tokens, self.heads, self.kv_heads,
                                                                       self.head_dim))
-        self.ws = torch.empty(max(self.ws_bytes, 16), dtype=torch.uint8, device=device or "cuda")
+        self.ws = self._keep(torch.empty(max(self.ws_bytes, 16), dtype=torch.uint8, device=device or "cuda"))
 
     def run(self, q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: torch.Tensor, out: torch.Tensor, *,
             k_own: Optional[torch.Tensor] = None, v_own: Optional[torch.Tensor] = None,
@@ -566,6 +591,6 @@ class PrefixAttention:
                                        dim ** -0.5 if scale is None else scale, 0, q.data_ptr(), sq[0], sq[1],
                                        k_prefix.data_ptr(), sk[0], sk[1], v_prefix.data_ptr(), sv[0], sv[1], *own, *lists,
                                        q_ptr, out.data_ptr(), so[0], so[1], lse_ptr, self.ws.data_ptr(), self.ws_bytes),
-            torch._C._cuda_getCurrentRawStream(dev))
+            self._stream(dev))
         if rc:
             check(rc)
