@@ -331,6 +331,7 @@ class BagPrepass:
 
 # ---------------------------------------------------------------- sequence operators
 
+_F32_MAX = torch.finfo(torch.float32).max
 _DTYPES = {torch.float32: ANNC_F32, torch.bfloat16: ANNC_BF16, torch.float16: ANNC_F16}
 
 
@@ -545,6 +546,9 @@ class PrefixAttention(_Plan):
         kv_heads, head_dim] with own_begin i64[sequences] and own_len i32[sequences]; q_begin i32[sequences + 1],
         without it a token is a sequence; scale head_dim ** -0.5 unless given; lse f32[tokens, heads]."""
         heads, kv, dim, dtypes = self.heads, self.kv_heads, self.head_dim, (self.dtype,)
+        scale = dim ** -0.5 if scale is None else scale
+        if not -_F32_MAX <= scale <= _F32_MAX:
+            _refuse(f"scale: {scale} is not a finite f32")
         dev = _current("q", q)
         shape, sq = _dense("q", q, dev, dtypes, 3)
         tokens = shape[0]
@@ -588,7 +592,7 @@ class PrefixAttention(_Plan):
             lse_ptr = lse.data_ptr()
         rc = lib.annc_prefix_attention_dev(
             PACK_PREFIX_ATTENTION.pack(_DTYPES[self.dtype], heads, kv, dim, tokens, sequences, prefix, rows,
-                                       dim ** -0.5 if scale is None else scale, 0, q.data_ptr(), sq[0], sq[1],
+                                       scale, 0, q.data_ptr(), sq[0], sq[1],
                                        k_prefix.data_ptr(), sk[0], sk[1], v_prefix.data_ptr(), sv[0], sv[1], *own, *lists,
                                        q_ptr, out.data_ptr(), so[0], so[1], lse_ptr, self.ws.data_ptr(), self.ws_bytes),
             self._stream(dev))
