@@ -290,7 +290,7 @@ __device__ __forceinline__ void exp32(const uint32_t (&r)[32], int first, int va
   }
 }
 template <typename T, int DP, bool TAIL>
-__device__ __forceinline__ bool softmax_tile(uint32_t t_s, uint32_t t_p, uint32_t t_o, float scale, float scale2, bool first, int valid,
+__device__ __forceinline__ bool softmax_tile(uint32_t t_s, uint32_t t_p, uint32_t t_o, float scale, float scale2, bool mine, bool first, int valid,
                                              float& top, float& sum, uint32_t half_ready, uint32_t scores_read, uint32_t p_used, uint32_t p_phase,
                                              volatile int* abort_flag, int* error_word) {
   bool ok = true;
@@ -303,7 +303,9 @@ __device__ __forceinline__ bool softmax_tile(uint32_t t_s, uint32_t t_p, uint32_
   const float m0 = max32<TAIL>(r0, 0, valid, -INFINITY), m1 = max32<TAIL>(r1, 32, valid, -INFINITY);
   tmem_ld_wait();
   const float m2 = max32<TAIL>(r2, 64, valid, -INFINITY), m3 = max32<TAIL>(r3, 96, valid, -INFINITY);
-  const float most = max3(max3(m0, m1, m2), m3, m3), now = most * scale;
+  // (A row of the tile that is not there holds what lay in shared memory: it must not send the warp the long ways below.
+  // 2000 tokens of three heads to each of two key heads of 64 over 8192 keys: 60 us, 44 so.)
+  const float most = mine ? max3(max3(m0, m1, m2), m3, m3) : 0.0f, now = most * scale;
   if (Shape<DP>::kOwnP) {
     tc_fence_before();
     __syncwarp();
@@ -569,10 +571,10 @@ prefix_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
           // (two copies of the code: selects for every value of every tile would be a third of its instructions)
           const uint32_t p_phase = (done & 1u) ^ 1u;
           if (valid >= kTileKeys)
-            ok = softmax_tile<T, DP, false>(t_s, t_p, t_o, p.scale, p.scale2, step == 0, valid, top, sum, bar_h + 8 * c, bar_read + 8 * c,
+            ok = softmax_tile<T, DP, false>(t_s, t_p, t_o, p.scale, p.scale2, row < rows, step == 0, valid, top, sum, bar_h + 8 * c, bar_read + 8 * c,
                                             bar_pv + 8 * c, p_phase, abort_flag, p.error_word);
           else
-            ok = softmax_tile<T, DP, true>(t_s, t_p, t_o, p.scale, p.scale2, step == 0, valid, top, sum, bar_h + 8 * c, bar_read + 8 * c,
+            ok = softmax_tile<T, DP, true>(t_s, t_p, t_o, p.scale, p.scale2, row < rows, step == 0, valid, top, sum, bar_h + 8 * c, bar_read + 8 * c,
                                            bar_pv + 8 * c, p_phase, abort_flag, p.error_word);
           if (!ok) break;
           tc_fence_before();
