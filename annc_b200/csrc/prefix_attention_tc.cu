@@ -10,7 +10,9 @@
 // in the item the two are its two row tiles, sharing the key tiles; else they take the key tiles in turn and are added
 // at the end of the segment, the first one reading the other's O from tensor memory.  The running maximum of a row only
 // moves when a score passes it by more than 2^8 in the exponential: until then O keeps its scale, the numerators grow to
-// at most 256, and O is rescaled hardly ever.
+// at most 256, and O is rescaled hardly ever.  (Of f16 they are raised by 2^7 on top, so that small ones keep their bits.)
+// A tile with a row whose maximum is beyond 2^21, or -inf, goes a longer way: 2048 tokens of 16 heads
+// (two key heads) of 64 over 1024 keys 25 us, 20 else.
 //
 // What bounds it: with 64 values the 16 exponentials a cycle of the SM (2048 of some 2560 cycles for two tiles of 128 x 128;
 // a half, a third, a quarter or a sixth of them on the multiply-add units by a polynomial: 212, 187, 181 and 188 us where
@@ -29,7 +31,8 @@
 // written by the prefix kernel.
 //
 // Sums, maxima and O are held in fp32; the numerators are rounded to the operands' type for the second product, as the
-// tensor cores want them, while their sum is of the unrounded ones.
+// tensor cores want them, while their sum is of the unrounded ones: half a step a weight, which the row kernel, on fp32
+// weights, does not have (error relative to 64 bits 2.3e-3 in bf16, 2.9e-4 in f16; with fp32 weights 1.7e-3 and 2.1e-4).
 #include <cuda.h>
 
 #include <cmath>
@@ -1240,7 +1243,9 @@ int run_as(const Params& a, void* workspace, cudaStream_t s) {
   }
   // A unit of work fills a warp.  Small groups: several tokens' heads, if that leaves eight warps for every SM.  Few units with
   // something to do for more than one warp (chunks of own keys, going by the size of their buffer, and parts): four
-  // or eight warps for each.
+  // or eight warps for each.  The lengths themselves are on the device: a buffer of wide slots with few keys in each gets
+  // more warps than they need (four keys a token, packed / in slots of 512: 500 tokens of two key heads over 40 keys 6.9 / 12.9 us, 100
+  // tokens of eight over 300 17.0 / 22.5; with 64 tokens over 16 or 4096 keys the same).
   const long long units = a.tokens * a.kv_heads;
   const long long own = a.own_len && a.sequences > 0 ? a.own_rows / a.sequences : 0;
   const long long chunks = (own + j.short_prefix + 15) / 16 + (short_prefix ? 0 : p.plan.kv_tiles / p.plan.per_cta + 1);
