@@ -453,6 +453,13 @@ class _Plan:
         self._made = None if torch.cuda.is_current_stream_capturing() else stream.record_event()
         return memory
 
+    def __getstate__(self):
+        return {k: v for k, v in self.__dict__.items() if k not in ("_streams", "_made")}
+
+    def __setstate__(self, state) -> None:  # (a copy of a plan, made on the stream that is current now)
+        self.__dict__.update(state)
+        self._keep(self._memory)
+
     def _stream(self, dev: int) -> int:
         """The current stream of the device, which may use the memory from now on: behind what had it before the
         plan, and the allocator hands it out again only behind what is queued there when the plan is dropped."""

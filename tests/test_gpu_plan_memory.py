@@ -86,3 +86,28 @@ def test_first_use_of_a_plan_in_a_capture_on_another_stream(case):
         run(plan)
     side.synchronize()
     assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("case", CASES)
+def test_copies_of_a_plan(case):
+    import copy
+    import io
+    make, run, kept, out = case()
+    plan = make()
+    run(plan)
+    want = out.clone()
+    stored = io.BytesIO()
+    torch.save(plan, stored)
+    stored.seek(0)
+    side = torch.cuda.Stream()
+    for other in (copy.deepcopy(plan), torch.load(stored, weights_only=False)):
+        assert kept(other).data_ptr() != kept(plan).data_ptr()
+        out.zero_()
+        run(other)
+        assert torch.equal(out, want)
+        out.zero_()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            run(other)
+        side.synchronize()
+        assert torch.equal(out, want)
